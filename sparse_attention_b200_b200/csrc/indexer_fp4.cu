@@ -19,31 +19,14 @@
 #include <cstdlib>
 #include "topk.cuh"
 #include "fp4_exact.cuh"
+#include "nvfp4_quantize.cuh"
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 
 namespace sb {
 namespace {
 
-// ---------------------------------------------------------------- quantiser
-// Rule (no counterpart in the reference, which feeds random bytes):
-//   scale_g = e4m3_rne(min(amax_g / 6, 448)); code = nearest e2m1 to x / scale_g,
-//   ties to the even code, saturating at 6; scale 0 -> codes 0.
-// With group > 1 the input row is the fp32 mean, in head order, of `group`
-// consecutive heads (index vector of a GQA group).
-__device__ __forceinline__ uint32_t e2m1_code(float ratio) {
-  const float a = fabsf(ratio);
-  uint32_t c = 0;
-  c = (a > 0.25f) ? 1u : c;                  // tie 0.25 -> 0
-  c = (a >= 0.75f) ? 2u : c;                 // tie 0.75 -> 1.0 (code 2)
-  c = (a > 1.25f) ? 3u : c;                  // tie 1.25 -> 1.0
-  c = (a >= 1.75f) ? 4u : c;                 // tie 1.75 -> 2.0
-  c = (a > 2.5f) ? 5u : c;                   // tie 2.5 -> 2.0
-  c = (a >= 3.5f) ? 6u : c;                  // tie 3.5 -> 4.0
-  c = (a > 5.0f) ? 7u : c;                   // tie 5.0 -> 4.0
-  return (c != 0 && ratio < 0.f) ? (c | 8u) : c;
-}
-
+// ---------------------------------------------------------------- quantiser (nvfp4_quantize.cuh)
 // x: [B, H_in, S, 128] bf16. Output row (b, h, s) quantises the fp32 mean, in
 // head order, of heads h*group .. h*group+group-1 (group = 1: the head itself).
 // Row placement: token-major [(b*S + s), h] (query index vectors) or paged
@@ -83,19 +66,8 @@ __global__ void __launch_bounds__(256) quantize_kernel(const __nv_bfloat16* __re
 #pragma unroll
     for (int e = 0; e < 16; ++e) v[e] = __fdiv_rn(v[e], gf);
   }
-  float amax = 0.f;
-#pragma unroll
-  for (int e = 0; e < 16; ++e) amax = fmaxf(amax, fabsf(v[e]));
-  const float want = fminf(__fdiv_rn(amax, 6.0f), 448.0f);
-  const __nv_fp8_storage_t sbits = __nv_cvt_float_to_fp8(want, __NV_SATFINITE, __NV_E4M3);
-  const float sc = __half2float(__half(__nv_cvt_fp8_to_halfraw(sbits, __NV_E4M3)));
-  uint32_t lo = 0, hi = 0;
-  if (sc > 0.f) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) lo |= e2m1_code(__fdiv_rn(v[e], sc)) << (4 * e);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) hi |= e2m1_code(__fdiv_rn(v[8 + e], sc)) << (4 * e);
-  }
+  uint32_t lo, hi;
+  const __nv_fp8_storage_t sbits = quantize_nvfp4_group(v, lo, hi);
   long long dst;
   if (paged)
     dst = ((b * (seq >> 7) + (s_pos >> 7)) * heads_out + h) * 128 + (s_pos & 127);
