@@ -378,6 +378,71 @@ int sparse_b200_indexer_summary_noalloc(const void* q, const void* k, float* sco
                                         int hq, int hkv, int sq, int skv, int representatives, int topk,
                                         void* stream);
 
+/* ---- Serving over a paged 8-bit cache. Forward only, as the rest of the library; no counterpart in the reference, whose
+ * scorer reads a paged key cache that nothing else there writes, selects from or attends to.
+ *
+ * A page holds 128 tokens. k_pages, v_pages [pages, Hkv, 128, 128] e4m3 codes, k_scale, v_scale [pages, Hkv] fp32: a value is
+ * its code times its page's scale. k_index [pages, Hkv, 128, 64] u8 and k_index_scale [pages, Hkv, 128, 8] e4m3 are the NVFP4
+ * index vectors of the keys, as sparse_b200_fp4_scores_varlen reads them. block_table [B, table_stride] int32: the pages of a
+ * request in order, table_width of them at most. seq_lens [B]: keys of a request, new ones included, unless said otherwise.
+ * Rows of new tokens are packed request after request; cu_seqlens_q [B + 1] gives their places, rows behind the last one are
+ * not read and not written. B <= 4096.
+ *
+ * Lists: `tile` (a power of two, 1 to 128) consecutive tokens of a request share a list of pages, given as places in the
+ * request's block table row. page_ids [Hkv, rows, TopK]: with tile 1 the list of a token has the token's row (rows =
+ * total_q); else tile i of request r has row cu_seqlens_q[r] / tile + r + i (rows = total_q / tile + B).
+ *
+ * extend_pages: pages for the new tokens, and every table of a step, from the lengths. seq_lens here are the tokens that the
+ * cache holds so far, new_lens the new ones; negative lengths count as 0. New pages are taken from the end of free_pages
+ * [free_count], by request; block_table gets them. A request whose pages do not fit its table row, or are not free (counted
+ * over the requests before it, in order), is refused: its length stays, its slots are -1. Written: seq_lens_out [B],
+ * cu_seqlens_q / cu_seqlens_k / cu_page_offsets [B + 1], kv_indices [total_pages] (pages of all requests in order, -1
+ * behind), slots [total_q] (page * 128 + row of every new token, -1 behind), free_count_out [1], status [1]: 1 pages ran out,
+ * 2 a table row is too short, 4 more new tokens than total_q, 8 more pages than total_pages, 16 a sum is beyond int32 (kept
+ * at its largest). The inputs other than block_table stay as they are, so a call may be repeated.
+ *
+ * append_tokens: k, v [total_q, Hkv, 128] bf16 rows (strides in elements, multiples of 8; a row itself is dense) into the
+ * pages that slots names: the first token's slot of a request and of each page after it count, rows follow in order. Scale of
+ * a page: the smallest power of two (at least 2^-100) with which the largest finite magnitude of its rows is at most 448;
+ * where new rows make it grow, the rows before them are rescaled. Codes are rounded to nearest even, +-inf becomes +-448 times
+ * the scale, NaN stays NaN. Rows behind the new ones are left as they were. Two requests must not append to one page.
+ * k_index / k_index_scale may be NULL.
+ *
+ * select_pages: scores [Hidx, score_pages, total_q] fp32 (sparse_b200_fp4_scores_varlen) -> page_ids. The score of a page for
+ * a list is the largest over the list's tokens and the Hidx / Hkv index heads of the KV head. The first `sink` and last
+ * `recent` pages that the list's last token sees are always listed, the others by (score descending, page ascending); pages
+ * with no score above -inf are not. A list is ascending, -1 behind; rows without a tile are -1.
+ *
+ * paged_attention: q [total_q, Hq, 128] bf16 (strides in elements, multiples of 8) against all pages of its request
+ * (page_ids NULL) or the listed ones; causal: token i of n sees keys j <= i + seq_len - n. A page listed twice counts twice,
+ * entries that are not pages of the request are skipped. out [total_q, Hq, 128] bf16, lse [total_q, Hq] fp32 or NULL; a row
+ * that sees no key, or only keys of score -inf, is 0 with LSE -inf. What lies in the cache behind a request's last key, or is
+ * hidden from a token, does not reach its row, whatever its bits. Hq / Hkv <= 64. max_seqlen_q (a hint: the largest number of
+ * new tokens) sets how many tokens share a pass over a page. workspace: sparse_b200_paged_attention_workspace_bytes bytes
+ * that are the call's own while it runs. */
+int sparse_b200_extend_pages(int32_t* block_table, int64_t table_stride, int table_width, const int32_t* seq_lens,
+                             const int32_t* new_lens, const int32_t* free_pages, int free_capacity,
+                             const int32_t* free_count, int32_t* seq_lens_out, int32_t* cu_seqlens_q,
+                             int32_t* cu_seqlens_k, int32_t* cu_page_offsets, int32_t* kv_indices, int64_t* slots,
+                             int32_t* free_count_out, int32_t* status, int batch, int total_q, int total_pages,
+                             void* stream);
+int sparse_b200_append_tokens(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                              int64_t v_token_stride, int64_t v_head_stride, const int32_t* cu_seqlens_q,
+                              const int64_t* slots, void* k_pages, void* v_pages, float* k_scale, float* v_scale,
+                              void* k_index, void* k_index_scale, int batch, int hkv, int total_q, int64_t pages,
+                              void* stream);
+int sparse_b200_select_pages(const float* scores, const int32_t* cu_seqlens_q, const int32_t* seq_lens, int32_t* page_ids,
+                             int batch, int hidx, int hkv, int score_pages, int total_q, int topk, int tile, int sink,
+                             int recent, int causal, void* stream);
+int64_t sparse_b200_paged_attention_workspace_bytes(int hq, int hkv, int tile, int max_seqlen_q, int has_ids);
+int sparse_b200_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_pages,
+                                const void* v_pages, const float* k_scale, const float* v_scale,
+                                const int32_t* block_table, int64_t table_stride, int table_width,
+                                const int32_t* seq_lens, const int32_t* cu_seqlens_q, const int32_t* page_ids, void* out,
+                                float* lse, void* workspace, int64_t workspace_bytes, int batch, int hq, int hkv,
+                                int total_q, int64_t pages, int topk, int tile, int max_seqlen_q, int causal, float scale,
+                                void* stream);
+
 #ifdef __cplusplus
 }
 #endif

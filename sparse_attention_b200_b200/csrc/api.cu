@@ -2,6 +2,7 @@
 // No entry point throws, synchronises the device or allocates on the stream
 // path (the only allocation is a 4-byte status word per device, on first use).
 #include "internal.h"
+#include "paged.cuh"
 #include "../../include/sparse_b200.h"
 
 #include <cstdio>
@@ -701,6 +702,117 @@ int sparse_b200_indexed_attention_fp4(const void* q, const void* k, const void* 
   if (rc) return rc;
   // same stream: the ids written by the indexer are ready for the attention kernel
   return sparse_b200_q_centric(q, k, v, block_idx, nullptr, out, lse, batch, hq, hkv, sq, skv, topk, stream);
+}
+
+// ---------------------------------------------------------------- paged serving path
+static int check_batch(int batch, int total_q) {
+  REQUIRE(batch > 0 && batch <= PAGED_MAX_BATCH, "a step has 1 to 4096 requests");
+  REQUIRE(total_q >= 0, "negative token count");
+  return SB_OK;
+}
+
+int sparse_b200_extend_pages(int32_t* block_table, int64_t table_stride, int table_width, const int32_t* seq_lens,
+                             const int32_t* new_lens, const int32_t* free_pages, int free_capacity,
+                             const int32_t* free_count, int32_t* seq_lens_out, int32_t* cu_seqlens_q,
+                             int32_t* cu_seqlens_k, int32_t* cu_page_offsets, int32_t* kv_indices, int64_t* slots,
+                             int32_t* free_count_out, int32_t* status, int batch, int total_q, int total_pages,
+                             void* stream) {
+  REQUIRE(block_table && seq_lens && new_lens && free_count && seq_lens_out && cu_seqlens_q && cu_seqlens_k &&
+              cu_page_offsets && free_count_out && status, "null pointer");
+  REQUIRE((kv_indices || total_pages == 0) && (slots || total_q == 0) && (free_pages || free_capacity == 0), "null pointer");
+  int rc = check_batch(batch, total_q);
+  if (rc) return rc;
+  REQUIRE(total_pages >= 0 && free_capacity >= 0, "negative page count");
+  REQUIRE(table_width > 0 && table_width < (1 << 24) && table_stride >= table_width,
+          "a table row holds 1 to 2^24 - 1 pages and is at most as long as the row stride");
+  REQUIRE(seq_lens_out != seq_lens && free_count_out != free_count, "lengths and free count are not updated in place");
+  return launch_extend_pages(block_table, table_stride, table_width, seq_lens, new_lens, free_pages, free_capacity,
+                             free_count, seq_lens_out, cu_seqlens_q, cu_seqlens_k, cu_page_offsets, kv_indices,
+                             reinterpret_cast<long long*>(slots), free_count_out, status, batch, total_q, total_pages,
+                             static_cast<cudaStream_t>(stream));
+}
+
+int sparse_b200_append_tokens(const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                              int64_t v_token_stride, int64_t v_head_stride, const int32_t* cu_seqlens_q,
+                              const int64_t* slots, void* k_pages, void* v_pages, float* k_scale, float* v_scale,
+                              void* k_index, void* k_index_scale, int batch, int hkv, int total_q, int64_t pages,
+                              void* stream) {
+  int rc = check_batch(batch, total_q);
+  if (rc) return rc;
+  REQUIRE(hkv > 0 && hkv <= 65535, "1 to 65535 KV heads");
+  REQUIRE(pages > 0 && pages < (1LL << 31), "page count must be positive and fit int32");
+  if (total_q == 0) return SB_OK;
+  REQUIRE(k && v && cu_seqlens_q && slots && k_pages && v_pages && k_scale && v_scale, "null pointer");
+  REQUIRE(!k_index == !k_index_scale, "index codes and scales go together");
+  REQUIRE(aligned16(k) && aligned16(v) && aligned16(k_pages) && aligned16(v_pages) && aligned16(k_index),
+          "rows and pages must be 16-byte aligned");
+  REQUIRE(k_token_stride % 8 == 0 && k_head_stride % 8 == 0 && v_token_stride % 8 == 0 && v_head_stride % 8 == 0,
+          "row strides must be multiples of 8 elements");
+  const AppendArgs a{k, v, k_token_stride, k_head_stride, v_token_stride, v_head_stride, cu_seqlens_q,
+                     reinterpret_cast<const long long*>(slots), k_pages, v_pages, k_scale, v_scale, k_index, k_index_scale,
+                     batch, hkv, total_q, pages};
+  return launch_append_tokens(a, static_cast<cudaStream_t>(stream));
+}
+
+static int check_lists(int topk, int tile) {
+  REQUIRE(topk > 0, "a list takes at least one page");
+  REQUIRE(tile >= 1 && tile <= 128 && (tile & (tile - 1)) == 0, "tile must be a power of two from 1 to 128");
+  return SB_OK;
+}
+
+int sparse_b200_select_pages(const float* scores, const int32_t* cu_seqlens_q, const int32_t* seq_lens, int32_t* page_ids,
+                             int batch, int hidx, int hkv, int score_pages, int total_q, int topk, int tile, int sink,
+                             int recent, int causal, void* stream) {
+  int rc = check_batch(batch, total_q);
+  if (rc) return rc;
+  rc = check_lists(topk, tile);
+  if (rc) return rc;
+  REQUIRE(hkv > 0 && hkv <= 65535 && hidx >= hkv && hidx % hkv == 0, "index heads must be a positive multiple of KV heads");
+  REQUIRE(score_pages > 0, "page count must be positive");
+  REQUIRE(sink >= 0 && recent >= 0 && sink <= topk && recent <= topk - sink, "sink and recent pages must fit the list");
+  REQUIRE(static_cast<long long>(total_q / tile + batch) * topk < (1LL << 40), "lists too large");
+  if (total_q == 0 && tile == 1) return SB_OK;
+  REQUIRE((scores || total_q == 0) && cu_seqlens_q && seq_lens && page_ids, "null pointer");
+  return launch_select_pages(scores, cu_seqlens_q, seq_lens, page_ids, batch, hidx, hkv, score_pages, total_q, topk, tile,
+                             sink, recent, causal != 0, static_cast<cudaStream_t>(stream));
+}
+
+int64_t sparse_b200_paged_attention_workspace_bytes(int hq, int hkv, int tile, int max_seqlen_q, int has_ids) {
+  REQUIRE(hkv > 0 && hq >= hkv && hq % hkv == 0 && tile >= 1, "sizes as in sparse_b200_paged_attention");
+  DeviceCtx* ctx = device_ctx();
+  if (!ctx) return SB_ERR_CUDA;
+  return paged_attention_workspace_bytes(hq, hkv, tile, max_seqlen_q, has_ids != 0, ctx->sm_count);
+}
+
+int sparse_b200_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_pages,
+                                const void* v_pages, const float* k_scale, const float* v_scale,
+                                const int32_t* block_table, int64_t table_stride, int table_width,
+                                const int32_t* seq_lens, const int32_t* cu_seqlens_q, const int32_t* page_ids, void* out,
+                                float* lse, void* workspace, int64_t workspace_bytes, int batch, int hq, int hkv,
+                                int total_q, int64_t pages, int topk, int tile, int max_seqlen_q, int causal, float scale,
+                                void* stream) {
+  int rc = check_batch(batch, total_q);
+  if (rc) return rc;
+  REQUIRE(hkv > 0 && hkv <= 65535 && hq >= hkv && hq % hkv == 0 && hq / hkv <= 64,
+          "Hq must be a multiple of Hkv, at most 64 query heads to a KV head");
+  REQUIRE(pages > 0 && pages * hkv * 128 < (1LL << 31), "rows of the cache must fit int32 (TMA row coordinates)");
+  REQUIRE(table_width > 0 && table_width < (1 << 24) && (batch == 1 || table_stride >= table_width),
+          "a table row holds 1 to 2^24 - 1 pages and is at most as long as the row stride");
+  if (page_ids) {
+    rc = check_lists(topk, tile);
+    if (rc) return rc;
+  }
+  if (total_q == 0) return SB_OK;
+  REQUIRE(q && k_pages && v_pages && k_scale && v_scale && block_table && seq_lens && cu_seqlens_q && out, "null pointer");
+  REQUIRE(aligned16(q) && aligned16(k_pages) && aligned16(v_pages) && aligned16(out) && aligned16(workspace),
+          "q, pages, out and workspace must be 16-byte aligned");
+  REQUIRE(q_token_stride % 8 == 0 && q_head_stride % 8 == 0, "row strides must be multiples of 8 elements");
+  REQUIRE(out != q && out != k_pages && out != v_pages, "output must not alias inputs");
+  REQUIRE(scale == scale && scale - scale == 0.f, "scale must be finite");
+  const PagedAttentionArgs a{q, q_token_stride, q_head_stride, k_pages, v_pages, k_scale, v_scale, block_table, table_stride,
+                             table_width, seq_lens, cu_seqlens_q, page_ids, out, lse, workspace, workspace_bytes, batch, hq,
+                             hkv, total_q, topk, tile, max_seqlen_q, causal != 0, pages, scale};
+  return launch_paged_attention(a, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -20,6 +20,7 @@ struct DeviceCtx {
   int misc_attr[8] = {0};
   int tc_attr = 0;
   int small_attr = 0;
+  int paged_attr[8] = {0};
 };
 DeviceCtx* device_ctx();
 
@@ -110,6 +111,45 @@ int launch_tile_max_topk(const float* query_scores, int32_t* ids, int batch, int
                          cudaStream_t stream);
 int launch_row_topk(const float* tile_scores, int32_t* ids, long long rows, int tiles, int topk, cudaStream_t stream,
                     bool after_scorer = false);
+// paged serving path (paged_*.cu)
+int launch_extend_pages(int32_t* table, long long table_stride, int width, const int32_t* seq, const int32_t* added,
+                        const int32_t* free_pages, int free_capacity, const int32_t* free_count, int32_t* seq_out,
+                        int32_t* cu_q, int32_t* cu_k, int32_t* cu_pages, int32_t* kv_indices, long long* slots,
+                        int32_t* free_out, int32_t* status, int batch, int total_q, int total_pages, cudaStream_t stream);
+struct AppendArgs {
+  const void *k, *v;                       // bf16 rows, strides in elements
+  long long k_token, k_head, v_token, v_head;
+  const int32_t* cu_q;
+  const long long* slots;
+  void *k_cache, *v_cache;
+  float *k_scale, *v_scale;
+  void *k_index, *k_index_scale;           // may be null
+  int batch, heads, total_q;
+  long long pages;
+};
+int launch_append_tokens(const AppendArgs& a, cudaStream_t stream);
+int launch_select_pages(const float* scores, const int32_t* cu_q, const int32_t* seq, int32_t* ids, int batch, int heads_in,
+                        int heads, int pages, int total_q, int topk, int tile, int sink, int recent, int causal,
+                        cudaStream_t stream);
+struct PagedAttentionArgs {
+  const void* q;                           // bf16 rows, strides in elements
+  long long q_token, q_head;
+  const void *k, *v;
+  const float *k_scale, *v_scale;
+  const int32_t* table;
+  long long table_stride;
+  int width;
+  const int32_t *seq, *cu_q, *ids;         // ids may be null
+  void* out;
+  float* lse;                              // may be null
+  void* workspace;
+  long long workspace_bytes;
+  int batch, hq, hkv, total_q, topk, tile, max_q, causal;
+  long long pages;
+  float scale;
+};
+int launch_paged_attention(const PagedAttentionArgs& a, cudaStream_t stream);
+long long paged_attention_workspace_bytes(int hq, int hkv, int tile, int max_q, bool listed, int sm_count);
 int launch_bounded_wait_selftest(long long limit_cycles, int* observed, cudaStream_t stream);
 
 }  // namespace sb

@@ -1,0 +1,267 @@
+"""Serving over a paged 8-bit cache: page tables, cache writer, page lists and attention, bound to the C ABI.
+
+extend_pages     lengths of a step -> pages from a free stack, block table, slot map, cumulative lengths, page list
+append_tokens    bf16 keys and values -> e4m3 pages with a scale per (page, head), and NVFP4 index vectors
+select_pages     scores of indexers.fp4_block_scores_varlen -> lists of pages
+paged_attention  new tokens over all pages of their requests, or over listed ones
+paged_step       all of them in order: one layer's step of a serving loop
+
+A page holds 128 tokens, a head has 128 features. Rows of new tokens are packed request after request, `cu_seqlens_q`
+[B + 1] gives their places. Everything runs on the current stream, nothing synchronises, and all entry points can be
+captured in a CUDA graph after one eager call. No counterpart in the reference, whose ragged scorer
+(indexers/fp4/vendor_minimax_msa/fp4_indexer_interface.py:745-811) reads a paged key cache that nothing else there uses."""
+import collections
+import ctypes
+
+import torch
+
+from . import _lib
+from .indexers import fp4_block_scores_varlen
+
+PAGE = 128
+_i64 = ctypes.c_int64
+
+PageBatch = collections.namedtuple(
+    "PageBatch", "seq_lens cu_seqlens_q cu_seqlens_k cu_page_offsets kv_indices slots free_count status")
+STATUS_NO_PAGES, STATUS_TABLE_FULL, STATUS_TOKENS, STATUS_PAGES, STATUS_OVERFLOW = 1, 2, 4, 8, 16
+
+
+def _bad(message):
+    raise _lib.SparseB200Error(message)
+
+
+def _dense(name, t, dtype, shape, device):
+    if not (t.is_cuda and t.device == device and t.dtype == dtype and tuple(t.shape) == tuple(shape) and t.is_contiguous()):
+        _bad(f"{name} must be a contiguous {dtype} tensor {list(shape)} on {device}")
+
+
+def _rows(name, t, heads, device=None, total=None):
+    """Packed bf16 rows [T, H, 128]: any token and head stride that keeps rows on 16 bytes."""
+    if not (t.is_cuda and t.dtype == torch.bfloat16 and t.dim() == 3 and t.shape[2] == 128):
+        _bad(f"{name} must be a bfloat16 CUDA tensor [T,H,128]")
+    if device is not None and t.device != device:
+        _bad(f"{name} must be on {device}")
+    if heads is not None and t.shape[1] != heads or total is not None and t.shape[0] != total:
+        _bad(f"{name} must have shape [{total if total is not None else 'T'},{heads},128]")
+    if t.requires_grad:
+        _bad("the paged path is forward-only")
+    s = t.stride()
+    if s[2] != 1 or s[0] % 8 or s[1] % 8 or t.data_ptr() % 16:
+        _bad(f"{name}: rows must be dense, 16-byte aligned and at strides that are multiples of 8 elements")
+
+
+def _table(block_table, batch, device):
+    if not (block_table.is_cuda and block_table.device == device and block_table.dtype == torch.int32
+            and block_table.dim() == 2 and block_table.shape[0] == batch and block_table.shape[1] > 0
+            and block_table.stride(1) == 1 and (batch == 1 or block_table.stride(0) >= block_table.shape[1])):
+        _bad("block_table must be int32 [B, pages per request] with dense rows on the same device")
+    return max(int(block_table.stride(0)), int(block_table.shape[1]))
+
+
+class PagedCache:
+    """Keys and values of one layer in pages of 128 tokens: e4m3 codes k, v [pages,Hkv,128,128] and scales k_scale, v_scale
+    [pages,Hkv] fp32, and with index=True the NVFP4 index vectors of the keys, k_index [pages,Hkv,128,64] u8 and
+    k_index_scale [pages,Hkv,128,8] e4m3, as fp4_block_scores_varlen takes them."""
+
+    def __init__(self, pages, kv_heads, device="cuda", index=True):
+        if pages <= 0 or kv_heads <= 0:
+            _bad("pages and KV heads must be positive")
+        shape = (pages, kv_heads, PAGE, 128)
+        self._set(torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn),
+                  torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn),
+                  torch.ones(shape[:2], dtype=torch.float32, device=device),
+                  torch.ones(shape[:2], dtype=torch.float32, device=device),
+                  torch.zeros((*shape[:3], 64), dtype=torch.uint8, device=device) if index else None,
+                  torch.zeros((*shape[:3], 8), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) if index else None)
+
+    @classmethod
+    def from_tensors(cls, k, v, k_scale, v_scale, k_index=None, k_index_scale=None):
+        """A cache over tensors that exist already (checked, not copied)."""
+        cache = cls.__new__(cls)
+        cache._set(k, v, k_scale, v_scale, k_index, k_index_scale)
+        return cache
+
+    def _set(self, k, v, k_scale, v_scale, k_index, k_index_scale):
+        if k.dim() != 4 or tuple(k.shape[2:]) != (PAGE, 128) or not k.is_cuda:
+            _bad("cache pages must be CUDA tensors [pages,Hkv,128,128]")
+        self.pages, self.kv_heads, self.device = int(k.shape[0]), int(k.shape[1]), k.device
+        lead = (self.pages, self.kv_heads)
+        _dense("k", k, torch.float8_e4m3fn, (*lead, PAGE, 128), k.device)
+        _dense("v", v, torch.float8_e4m3fn, (*lead, PAGE, 128), k.device)
+        _dense("k_scale", k_scale, torch.float32, lead, k.device)
+        _dense("v_scale", v_scale, torch.float32, lead, k.device)
+        if (k_index is None) != (k_index_scale is None):
+            _bad("index codes and scales go together")
+        if k_index is not None:
+            _dense("k_index", k_index, torch.uint8, (*lead, PAGE, 64), k.device)
+            _dense("k_index_scale", k_index_scale, torch.float8_e4m3fn, (*lead, PAGE, 8), k.device)
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.k_index, self.k_index_scale = k_index, k_index_scale
+
+
+def extend_pages(block_table, seq_lens, new_lens, free_pages, free_count, *, total_q, total_pages):
+    """Pages for new_lens [B] tokens behind the seq_lens [B] that the requests hold, taken from the end of free_pages
+    [free_count], and the tables of the step. block_table [B, W] is extended in place; everything else is new (PageBatch):
+    seq_lens with the new tokens, cu_seqlens_q / cu_seqlens_k / cu_page_offsets [B+1], kv_indices [total_pages], slots
+    [total_q] int64, free_count [1], status [1] (STATUS_* bits; 0: all is well). total_q and total_pages are the sizes of the
+    tables; what is behind the last token or page is -1. A request that gets no pages is refused: its length stays, its slots
+    are -1."""
+    batch, dev = int(seq_lens.numel()), seq_lens.device
+    if not seq_lens.is_cuda or batch == 0:
+        _bad("seq_lens must be a CUDA tensor of at least one request")
+    _dense("seq_lens", seq_lens, torch.int32, (batch,), dev)
+    _dense("new_lens", new_lens, torch.int32, (batch,), dev)
+    _dense("free_pages", free_pages, torch.int32, (free_pages.numel(),), dev)
+    _dense("free_count", free_count, torch.int32, (1,), dev)
+    stride = _table(block_table, batch, dev)
+    total_q, total_pages = int(total_q), int(total_pages)
+    if total_q < 0 or total_pages < 0:
+        _bad("table sizes must not be negative")
+    with torch.cuda.device(dev):
+        out = torch.empty(4 * batch + 5 + total_pages, dtype=torch.int32, device=dev)
+        slots = torch.empty(total_q, dtype=torch.int64, device=dev)
+        seq, cu_q, cu_k, cu_pages, count, status, kv = out.split(
+            [batch, batch + 1, batch + 1, batch + 1, 1, 1, total_pages])
+        _lib.check(_lib.lib().sparse_b200_extend_pages(
+            _lib.ptr(block_table), _i64(stride), int(block_table.shape[1]), _lib.ptr(seq_lens), _lib.ptr(new_lens),
+            _lib.ptr(free_pages), int(free_pages.numel()), _lib.ptr(free_count), _lib.ptr(seq), _lib.ptr(cu_q),
+            _lib.ptr(cu_k), _lib.ptr(cu_pages), _lib.ptr(kv), _lib.ptr(slots), _lib.ptr(count), _lib.ptr(status), batch,
+            total_q, total_pages, _lib.current_stream()))
+    return PageBatch(seq, cu_q, cu_k, cu_pages, kv, slots, count, status)
+
+
+def append_tokens(cache, k, v, cu_seqlens_q, slots):
+    """k, v [T,Hkv,128] bf16 -> the rows of the cache that slots [T] (extend_pages) names: the tokens of a request lie in
+    order from its first slot, page after page. A page's scale is the smallest power of two that holds its rows; the rows
+    before the new ones are rescaled where it grows. Index vectors are written where the cache has them."""
+    total, dev = int(slots.numel()), cache.device
+    _rows("k", k, cache.kv_heads, dev, total)
+    _rows("v", v, cache.kv_heads, dev, total)
+    batch = int(cu_seqlens_q.numel()) - 1
+    _dense("cu_seqlens_q", cu_seqlens_q, torch.int32, (batch + 1,), dev)
+    _dense("slots", slots, torch.int64, (total,), dev)
+    ks, vs = k.stride(), v.stride()
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().sparse_b200_append_tokens(
+            _lib.ptr(k), _i64(ks[0]), _i64(ks[1]), _lib.ptr(v), _i64(vs[0]), _i64(vs[1]), _lib.ptr(cu_seqlens_q),
+            _lib.ptr(slots), _lib.ptr(cache.k), _lib.ptr(cache.v), _lib.ptr(cache.k_scale), _lib.ptr(cache.v_scale),
+            _lib.ptr(cache.k_index), _lib.ptr(cache.k_index_scale), batch, cache.kv_heads, total, _i64(cache.pages),
+            _lib.current_stream()))
+
+
+def list_rows(total_q, batch, tile):
+    """Rows of the lists of a step: tile i of request r has row cu_seqlens_q[r] // tile + r + i (tile 1: the token's row)."""
+    return total_q if tile == 1 else total_q // tile + batch
+
+
+def select_pages(scores, cu_seqlens_q, seq_lens, *, kv_heads, topk, tile=1, sink=1, recent=1, causal=True, ids=None):
+    """scores [Hidx, pages, T] fp32 (fp4_block_scores_varlen) -> ids [kv_heads, list_rows(T, B, tile), topk] int32: for every
+    `tile` consecutive tokens of a request the best pages by (score descending, page ascending), written ascending with -1
+    behind them. The first `sink` and the last `recent` pages that the tile's last token sees are always among them."""
+    if not (scores.is_cuda and scores.dtype == torch.float32 and scores.is_contiguous() and scores.dim() == 3):
+        _bad("scores must be contiguous float32 [Hidx,pages,T] on CUDA")
+    hidx, pages, total = (int(n) for n in scores.shape)
+    dev, batch = scores.device, int(seq_lens.numel())
+    _dense("seq_lens", seq_lens, torch.int32, (batch,), dev)
+    _dense("cu_seqlens_q", cu_seqlens_q, torch.int32, (batch + 1,), dev)
+    if tile < 1 or tile & (tile - 1):
+        _bad("tile must be a power of two from 1 to 128")
+    shape = (kv_heads, list_rows(total, batch, tile), topk)
+    if kv_heads < 1 or topk < 1:
+        _bad("KV heads and topk must be positive")
+    if ids is None:
+        ids = torch.empty(shape, dtype=torch.int32, device=dev)
+    else:
+        _dense("ids", ids, torch.int32, shape, dev)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().sparse_b200_select_pages(
+            _lib.ptr(scores), _lib.ptr(cu_seqlens_q), _lib.ptr(seq_lens), _lib.ptr(ids), batch, hidx, kv_heads, pages, total,
+            topk, tile, sink, recent, int(bool(causal)), _lib.current_stream()))
+    return ids
+
+
+def paged_attention(q, cache, block_table, seq_lens, cu_seqlens_q, ids=None, *, tile=1, max_seqlen_q=None, causal=True,
+                    scale=None, out=None, lse=None, return_lse=False):
+    """softmax(scale q k^T) v of q [T,Hq,128] bf16 over the pages of each request (ids=None) or the listed ones (ids
+    [Hkv, list_rows(T, B, tile), topk] of select_pages). seq_lens [B] count the new tokens in; causal: token i of n sees the
+    keys j <= i + seq_len - n. Returns out [T,Hq,128] bf16, with return_lse also the natural-log LSE [T,Hq] fp32; rows behind
+    the last token of out and lse are left as they were. max_seqlen_q: the largest number of new tokens, for how many of them
+    share a pass over a page (default: T). scale: default 128^-0.5."""
+    _rows("q", q, None, cache.device)
+    total, hq = int(q.shape[0]), int(q.shape[1])
+    hkv, dev, batch = cache.kv_heads, cache.device, int(seq_lens.numel())
+    if hq < hkv or hq % hkv or hq // hkv > 64:
+        _bad("Hq must be a multiple of Hkv, at most 64 query heads to a KV head")
+    _dense("seq_lens", seq_lens, torch.int32, (batch,), dev)
+    _dense("cu_seqlens_q", cu_seqlens_q, torch.int32, (batch + 1,), dev)
+    stride = _table(block_table, batch, dev)
+    topk = 0
+    if ids is not None:
+        if ids.dim() != 3 or ids.shape[2] < 1 or tile < 1 or tile > 128 or tile & (tile - 1):
+            _bad("ids must be [Hkv, list rows, topk] for a tile that is a power of two from 1 to 128")
+        topk = int(ids.shape[2])
+        _dense("ids", ids, torch.int32, (hkv, list_rows(total, batch, tile), topk), dev)
+    if out is None:
+        out = torch.empty((total, hq, 128), dtype=torch.bfloat16, device=dev)
+    else:
+        _dense("out", out, torch.bfloat16, (total, hq, 128), dev)
+        for t in (q, cache.k, cache.v):
+            if out.untyped_storage().data_ptr() == t.untyped_storage().data_ptr():
+                _bad("output must not alias inputs")
+    if lse is not None:
+        _dense("lse", lse, torch.float32, (total, hq), dev)
+    elif return_lse:
+        lse = torch.empty((total, hq), dtype=torch.float32, device=dev)
+    max_q = total if max_seqlen_q is None else int(max_seqlen_q)
+    lib = _lib.lib()
+    lib.sparse_b200_paged_attention_workspace_bytes.restype = ctypes.c_int64
+    with torch.cuda.device(dev):
+        need = lib.sparse_b200_paged_attention_workspace_bytes(hq, hkv, tile, max_q, int(ids is not None))
+        if need < 0:
+            _lib.check(need)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        _lib.check(lib.sparse_b200_paged_attention(
+            _lib.ptr(q), _i64(q.stride(0)), _i64(q.stride(1)), _lib.ptr(cache.k), _lib.ptr(cache.v), _lib.ptr(cache.k_scale),
+            _lib.ptr(cache.v_scale), _lib.ptr(block_table), _i64(stride), int(block_table.shape[1]), _lib.ptr(seq_lens),
+            _lib.ptr(cu_seqlens_q), _lib.ptr(ids), _lib.ptr(out), _lib.ptr(lse), _lib.ptr(ws), _i64(need), batch, hq, hkv,
+            total, _i64(cache.pages), topk, tile, max_q, int(bool(causal)),
+            ctypes.c_float(128 ** -0.5 if scale is None else scale), _lib.current_stream()))
+    return (out, lse) if return_lse else out
+
+
+def paged_step(q, k, v, cache, block_table, batch, *, topk=None, tile=1, max_seqlen_q, max_seqlen_k, sink=1, recent=1,
+               scale=None):
+    """One layer's step over a PageBatch: append k, v to the cache, score the pages of every request with the NVFP4 index
+    vectors (one index head per KV head: the mean of its query heads), select topk of them and attend. topk=None: attend to
+    whole sequences, without index vectors. Returns (out, ids)."""
+    append_tokens(cache, k, v, batch.cu_seqlens_q, batch.slots)
+    ids = None
+    if topk is not None:
+        if cache.k_index is None:
+            _bad("selection needs a cache with index vectors")
+        total, hq = int(q.shape[0]), int(q.shape[1])
+        codes, scales = quantize_rows(q, cache.kv_heads)
+        scores = fp4_block_scores_varlen(codes, cache.k_index, scales, cache.k_index_scale, batch.cu_seqlens_q,
+                                         batch.cu_seqlens_k, batch.cu_page_offsets, max_seqlen_q=max_seqlen_q,
+                                         max_seqlen_k=max_seqlen_k, kv_indices=batch.kv_indices, causal=True, exact=False)
+        ids = select_pages(scores, batch.cu_seqlens_q, batch.seq_lens, kv_heads=cache.kv_heads, topk=topk, tile=tile,
+                           sink=sink, recent=recent)
+    out = paged_attention(q, cache, block_table, batch.seq_lens, batch.cu_seqlens_q, ids, tile=tile,
+                          max_seqlen_q=max_seqlen_q, scale=scale)
+    return out, ids
+
+
+def quantize_rows(q, hidx):
+    """Packed rows q [T,Hq,128] bf16 (contiguous) -> NVFP4 query index vectors (codes [T,hidx,64], scales [T,hidx,8]): the
+    mean over the Hq/hidx heads of a group, as indexers.quantize_queries for whole sequences."""
+    _rows("q", q, None)
+    total, hq = int(q.shape[0]), int(q.shape[1])
+    if hq % hidx or not q.is_contiguous():
+        _bad("q must be contiguous and Hq a multiple of the index head count")
+    codes = torch.empty((total, hidx, 64), dtype=torch.uint8, device=q.device)
+    scales = torch.empty((total, hidx, 8), dtype=torch.float8_e4m3fn, device=q.device)
+    if total:
+        with torch.cuda.device(q.device):      # T batches of one token: their heads are T rows apart by Hq, as the kernel wants
+            _lib.check(_lib.lib().sparse_b200_nvfp4_quantize(_lib.ptr(q), _lib.ptr(codes), _lib.ptr(scales), total, hidx,
+                                                             hq // hidx, 1, 0, _lib.current_stream()))
+    return codes, scales
