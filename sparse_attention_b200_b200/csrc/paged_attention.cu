@@ -1,9 +1,29 @@
-// Attention of new tokens over the 8-bit paged cache.
+// Attention of new tokens over the 8-bit paged cache, on the tensor cores, straight from the e4m3 codes.
 //
 //   s_ij = scale * q_i . (k_scale * k_j)          keys j <= i + k_len - q_len of the request (causal) in the pages taken
 //   o_i = sum_j softmax(s_i)_j v_scale v_j        lse_i = ln sum_j exp s_ij;  no key: o = 0, lse = -inf
 //
-// One CTA per (token, KV head): thread = key for the scores, feature for the output.
+// Mathematics. A work item is `pack` tokens of a request and a KV head: R rows (token, query head) that share a pass over the
+// pages. Keys are the M dimension of both products, so that even one token of a few heads fills the instruction:
+//   S^T [128 keys, R] = K [128 keys, 128] Q^T       O^T [128 features, R] = V^T [128 features, 128 keys] P^T
+// The tensor core multiplies e4m3 by e4m3 (kind::f8f6f4), and the codes of a page are its operands as they lie in memory:
+// nothing is dequantised. The other operand is split in two e4m3 terms in columns of their own, x = hi + lo / 16: a bf16 has
+// eight significant bits and an e4m3 code four, so a query (scaled by a power of two to [128, 256) by its row's largest
+// feature) is carried exactly but for features below 2^-22 of the largest; a probability (times 256, against the maximum of
+// its own page, so that no page's weights fall below the format's range) is cut at four bits and the rest rounded to four:
+// within 2^-8 of its value, half a step of bf16. Maxima, sums and outputs are fp32; every page's output is added
+// to registers with the page's own factor exp2(page maximum - running maximum) * v_scale.
+//
+// A softmax thread owns a key (a TMEM lane of S^T) and 16 rows; a row's maximum over the page is a warp reduction
+// (redux.sync on fp32) and an exchange between four warps. In the second product the same thread owns a feature.
+//
+// Work split. Pages of all items, in the order (head, request, tile, page), are cut in equal shares, one per CTA: long and
+// short requests balance whatever their lengths, known on the device only. Every CTA finds its share itself, from closed sums
+// over a request's tiles and a scan over the requests. An item that lies in several shares is left as partial sums (fp32, with
+// its maximum and sum) that paged_merge_kernel adds in order: no atomics, the same bits every time.
+//
+// CTA: R / 16 softmax warpgroups, a loader warp (TMA, one 16 KB tile of K or V to a slot of a ring), an MMA warp, two warps
+// that bring and split the queries of the next item. Entries (start of an item, page, end) go through a ring of their own.
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 #include "internal.h"
@@ -11,112 +31,843 @@
 #include "ptx.cuh"
 
 namespace sb {
-namespace {
+namespace pa {
 
-constexpr int THREADS = 128;
-constexpr int HEADS = 8;      // query heads of one pass
+constexpr int TILE_BYTES = 128 * 128;
+constexpr int INFO = 16;                          // entries in flight
+constexpr int START = 1, PAGE = 2, END = 3, STOP = 4;
+constexpr int MIN_SHARE = 4;                      // pages of a CTA at least
 
-__device__ __forceinline__ float2 decode2(uint32_t codes) {
-  return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(codes), __NV_E4M3)));
+struct Params {
+  PagedAttentionArgs a;
+  int group, pack, ctas;
+  float* part_o;                                  // [2 ctas, R, 128]
+  float* part_ml;                                 // [2 ctas, R, 2]
+  int* part_meta;                                 // [2 ctas, 8]
+};
+
+template <int R_>
+struct Config {
+  static constexpr int R = R_, N = 2 * R, GROUPS = R / 16;
+  static constexpr int SOFTMAX_WARPS = 4 * GROUPS;
+  static constexpr int LOADER = SOFTMAX_WARPS, MMA = LOADER + 1, QWARP = MMA + 1, WARPS = QWARP + 2;
+  static constexpr int THREADS = 32 * WARPS;
+  static constexpr int CTAS = R == 64 ? 1 : 2;    // per SM
+  static constexpr int SLOTS = R == 16 ? 5 : R == 32 ? 4 : 8;
+  static constexpr int OFF_RING = 0;
+  static constexpr int OFF_Q = OFF_RING + SLOTS * TILE_BYTES;       // two buffers of N rows of 128 bytes
+  static constexpr int OFF_P = OFF_Q + 2 * N * 128;                 // two buffers of 128 keys x N columns
+  static constexpr int OFF_FACTOR = OFF_P + 2 * N * 128;            // float4 [softmax warp][16]
+  static constexpr int OFF_OUT = OFF_FACTOR + SOFTMAX_WARPS * 256;  // float2 [2][softmax warp][16]
+  static constexpr int OFF_MAX = OFF_OUT + 2 * SOFTMAX_WARPS * 128; // float [2][softmax warp][16]
+  static constexpr int OFF_SUM = OFF_MAX + 2 * SOFTMAX_WARPS * 64;  // float [2][softmax warp][16]
+  static constexpr int OFF_QF = OFF_SUM + 2 * SOFTMAX_WARPS * 64;   // float [2][R]: what a row's scores are multiplied by
+  static constexpr int OFF_INFO = OFF_QF + 2 * R * 4;               // int [INFO][8]
+  static constexpr int OFF_BAR = OFF_INFO + INFO * 32;
+  static constexpr int B_INFO_FULL = 0, B_INFO_EMPTY = INFO, B_FULL = 2 * INFO, B_EMPTY = B_FULL + SLOTS;
+  static constexpr int B_S_FULL = B_EMPTY + SLOTS, B_S_EMPTY = B_S_FULL + 2, B_P_FULL = B_S_EMPTY + 2, B_O_FULL = B_P_FULL + 2,
+                       B_O_EMPTY = B_O_FULL + 2, B_Q_FULL = B_O_EMPTY + 2, B_Q_EMPTY = B_Q_FULL + 2, B_MAX = B_Q_EMPTY + 2,
+                       B_SUM = B_MAX + 2 * GROUPS, B_DONE = B_SUM + 2 * GROUPS, BARS = B_DONE + 1;
+  static constexpr int OFF_MISC = OFF_BAR + BARS * 8;
+  static constexpr int SMEM = OFF_MISC + 64 + 1024;                 // 1024: alignment of the tiles
+  static constexpr int TMEM = 4 * N < 32 ? 32 : 4 * N;              // S0, S1, O0, O1
+};
+
+// kind::f8f6f4 instruction descriptor: e4m3 x e4m3 -> fp32, M = 128.
+__host__ __device__ constexpr uint32_t idesc_e4m3(int n, bool mn_major) {
+  return (1u << 4) | (mn_major ? (1u << 15) | (1u << 16) : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
+}
+__device__ __forceinline__ void mma_e4m3(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+      "}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// MN-major operand in panels of 32 columns, 32-byte swizzle: a key's 32 bytes of a panel, eight keys 256 bytes apart, panels
+// 4096 bytes apart.
+__device__ __forceinline__ uint64_t desc_sw32_mnmajor(uint32_t addr) {
+  return desc_field(addr) | (desc_field(4096) << 16) | (desc_field(256) << 32) | (1ULL << 46) | (6ULL << 61);
+}
+__device__ __forceinline__ float warp_max(float x) {
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ float from_e4m3(uint32_t code) {
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(code), __NV_E4M3)));
 }
 
-__device__ __forceinline__ float block_max(float x, float* scratch) {
-  for (int by = 16; by; by >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, by));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = x;
-  __syncthreads();
-  return fmaxf(fmaxf(scratch[0], scratch[1]), fmaxf(scratch[2], scratch[3]));
-}
-
-__device__ __forceinline__ float block_sum(float x, float* scratch) {
-  for (int by = 16; by; by >>= 1) x += __shfl_xor_sync(0xffffffffu, x, by);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = x;
-  __syncthreads();
-  return (scratch[0] + scratch[1]) + (scratch[2] + scratch[3]);
-}
-
-__global__ void __launch_bounds__(THREADS) paged_attention_kernel(PagedAttentionArgs a) {
-  __shared__ float s_q[HEADS][128], s_p[HEADS][128], scratch[4];
-  const int tid = threadIdx.x, token = blockIdx.x, head = blockIdx.y;
-  const int group = a.hq / a.hkv;
-  const auto start = [&](int r) { return min(max(__ldg(a.cu_q + r), 0), a.total_q); };
-  const int r = warp_last_at_most(a.batch, token, [&](int i) { return static_cast<long long>(start(i)); });
-  const int begin = start(r), end = start(r + 1);
-  if (token < begin || token >= end) return;
-  const int k_len = max(__ldg(a.seq + r), 0);
-  const int limit = a.causal ? k_len - (end - token) + 1 : k_len;      // keys seen
-  const int held = min((k_len + 127) >> 7, a.width);
-  const int32_t* list = nullptr;
-  int steps = held;
-  if (a.ids) {
-    const long long lists = a.tile == 1 ? a.total_q : a.total_q / a.tile + a.batch;
-    const long long row = first_list_row(begin, r, a.tile) + (token - begin) / a.tile;
-    list = a.ids + (head * lists + row) * a.topk;
-    steps = a.topk;
+// ------------------------------------------------------------------ the work of a request
+struct Request {
+  int begin, n, k_len, held, tiles;
+  __device__ __forceinline__ void set(const Params& p, int cu0, int cu1, int seq) {
+    begin = min(max(cu0, 0), p.a.total_q);
+    n = max(min(max(cu1, 0), p.a.total_q) - begin, 0);
+    k_len = max(seq, 0);
+    held = min((k_len >> 7) + ((k_len & 127) != 0), p.a.width);
+    tiles = (n + p.pack - 1) / p.pack;
   }
-  for (int g0 = 0; g0 < group; g0 += HEADS) {
-    const int heads = min(HEADS, group - g0);
-    __syncthreads();
-    for (int g = 0; g < heads; ++g)
-      s_q[g][tid] = __bfloat162float(static_cast<const __nv_bfloat16*>(
-          a.q)[token * a.q_token + (head * group + g0 + g) * a.q_head + tid]) * a.scale;
-    __syncthreads();
-    float top[HEADS], sum[HEADS], o[HEADS];
-    for (int g = 0; g < HEADS; ++g) top[g] = -INFINITY, sum[g] = o[g] = 0.f;
-    for (int step = 0; step < steps; ++step) {
-      const int j = list ? __ldg(list + step) : step;
-      if (j < 0 || j >= held || j * 128LL >= limit) continue;
-      const int page = __ldg(a.table + r * a.table_stride + j);
-      if (page < 0 || page >= a.pages) continue;
-      const int seen = min(limit - j * 128, 128);
-      const long long at = static_cast<long long>(page) * a.hkv + head;
-      const float k_scale = __ldg(a.k_scale + at), v_scale = __ldg(a.v_scale + at);
-      const uint32_t* k = static_cast<const uint32_t*>(a.k) + (at * 128 + tid) * 32;
-      const uint8_t* v = static_cast<const uint8_t*>(a.v) + at * (128 * 128);
-      float x[HEADS];
-      for (int g = 0; g < HEADS; ++g) x[g] = 0.f;
-      for (int d = 0; d < 32; ++d) {
-        const uint32_t w = __ldg(k + d);
-        const float2 lo = decode2(w), hi = decode2(w >> 16);
-        for (int g = 0; g < HEADS; ++g)
-          x[g] += s_q[g][4 * d] * lo.x + s_q[g][4 * d + 1] * lo.y + s_q[g][4 * d + 2] * hi.x + s_q[g][4 * d + 3] * hi.y;
-      }
-      for (int g = 0; g < heads; ++g) {
-        const float s = tid < seen ? x[g] * k_scale : -INFINITY;
-        const float m = fmaxf(top[g], block_max(s, scratch));
-        const float base = m == -INFINITY ? 0.f : m;
-        const float p = tid < seen ? expf(s - base) : 0.f;
-        const float keep = expf(top[g] - base);
-        top[g] = m;
-        sum[g] = sum[g] * keep + p;
-        o[g] *= keep;
-        s_p[g][tid] = p;
-      }
-      __syncthreads();
-      for (int i = 0; i < seen; ++i) {
-        const float value = decode2(__ldg(v + i * 128 + tid)).x * v_scale;
-        for (int g = 0; g < heads; ++g) o[g] += s_p[g][i] * value;
-      }
-      __syncthreads();
+};
+// Pages of the first `tiles` tiles of a request: a list's length each, or the pages that a tile's last token sees (one at
+// least, so that every item has a place): min(held, ceil((k - n + (i + 1) pack) / 128)) summed over i. With pack = 128 / m the
+// ceiling is floor((first + i) / m), whose sums have a closed form.
+__device__ __forceinline__ long long pages_before(const Params& p, const Request& r, int tiles) {
+  if (p.a.ids) return static_cast<long long>(tiles) * p.a.topk;
+  const long long most = max(r.held, 1);
+  if (!p.a.causal) return tiles * most;
+  const int m = 128 / p.pack, shift = 31 - __clz(p.pack), mshift = 7 - shift;
+  const long long first = ((static_cast<long long>(r.k_len) - r.n + 127) >> shift) + 1;
+  const auto clamp = [&](long long x) { return x < 0 ? 0 : x > tiles ? tiles : x; };
+  const long long ones = clamp(m - first), full = max(clamp(most * m - first), ones);
+  const auto sum = [&](long long x) {             // sum of floor(t / m) over 0 <= t < x
+    const long long q = x >> mshift, rest = x & (m - 1);
+    return m * (q * (q - 1) / 2) + rest * q;
+  };
+  const long long middle = full > ones ? sum(first + full) - sum(first + ones) : 0;
+  return ones + middle + (tiles - full) * most;
+}
+
+// ------------------------------------------------------------------ kernel
+template <int R_>
+__global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
+    paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const Params p,
+                           int* status) {
+  using C = Config<R_>;
+  constexpr int R = C::R, N = C::N, SLOTS = C::SLOTS;
+  extern __shared__ unsigned char raw[];
+  const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+  unsigned char* gbase = raw + (base - smem_u32(raw));
+  volatile int* misc = reinterpret_cast<volatile int*>(gbase + C::OFF_MISC);     // [0] TMEM, [1] abort
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Guard guard{misc + 1, status};
+  const auto bar = [&](int i) { return base + C::OFF_BAR + 8 * i; };
+  __shared__ long long s_scan[C::WARPS];
+  __shared__ long long s_place[2];                // unit within the request, request
+
+  if (tid == 0) {
+    misc[1] = 0;
+    for (int i = 0; i < INFO; ++i) {
+      mbar_init(bar(C::B_INFO_FULL + i), 1);
+      mbar_init(bar(C::B_INFO_EMPTY + i), C::SOFTMAX_WARPS + 3);
     }
-    for (int g = 0; g < heads; ++g) {
-      const float total = block_sum(sum[g], scratch);
-      const long long row = static_cast<long long>(token) * a.hq + head * group + g0 + g;
-      const bool dead = total == 0.f;
-      static_cast<__nv_bfloat16*>(a.out)[row * 128 + tid] = __float2bfloat16(dead ? 0.f : o[g] / total);
-      if (a.lse && tid == 0) a.lse[row] = dead ? -INFINITY : top[g] + logf(total);
+    for (int i = 0; i < SLOTS; ++i) {
+      mbar_init(bar(C::B_FULL + i), 1);
+      mbar_init(bar(C::B_EMPTY + i), 1);
     }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(C::B_S_FULL + i), 1);
+      mbar_init(bar(C::B_S_EMPTY + i), C::SOFTMAX_WARPS);
+      mbar_init(bar(C::B_P_FULL + i), C::SOFTMAX_WARPS);
+      mbar_init(bar(C::B_O_FULL + i), 1);
+      mbar_init(bar(C::B_O_EMPTY + i), C::SOFTMAX_WARPS);
+      mbar_init(bar(C::B_Q_FULL + i), 2);
+      mbar_init(bar(C::B_Q_EMPTY + i), C::SOFTMAX_WARPS + 1);
+    }
+    for (int i = 0; i < 4 * C::GROUPS; ++i) mbar_init(bar(C::B_MAX + i), 4);
+    mbar_init(bar(C::B_DONE), 1);
+    fence_mbar_init();
+    p.part_meta[16 * blockIdx.x] = 0;             // no part yet in either of this CTA's places
+    p.part_meta[16 * blockIdx.x + 8] = 0;
+  }
+  if (warp == C::MMA) {
+    tmem_alloc(smem_u32(const_cast<int*>(misc)), C::TMEM);
+    tmem_relinquish();
+  }
+  if (warp == C::LOADER && lane == 0) {
+    prefetch_tmap(&k_map);
+    prefetch_tmap(&v_map);
+  }
+  // The share of this CTA: a scan over the requests' pages.
+  const int each = (p.a.batch + C::THREADS - 1) / C::THREADS;
+  const int lo = min(tid * each, p.a.batch), hi = min(lo + each, p.a.batch);
+  long long mine = 0;
+  for (int r = lo; r < hi; ++r) {
+    Request q;
+    q.set(p, __ldg(p.a.cu_q + r), __ldg(p.a.cu_q + r + 1), __ldg(p.a.seq + r));
+    mine += pages_before(p, q, q.tiles);
+  }
+  long long upto = mine;
+  for (int by = 1; by < 32; by <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, upto, by);
+    if (lane >= by) upto += x;
+  }
+  if (lane == 31) s_scan[warp] = upto;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  long long per_head = 0;
+  upto -= mine;
+  for (int w = 0; w < C::WARPS; ++w) {
+    if (w < warp) upto += s_scan[w];
+    per_head += s_scan[w];
+  }
+  const long long total = per_head * p.a.hkv;
+  const long long share = max((total + p.ctas - 1) / p.ctas, static_cast<long long>(MIN_SHARE));
+  const long long unit0 = blockIdx.x * share, unit1 = min(unit0 + share, total);
+  const int head0 = unit0 < total ? static_cast<int>(unit0 / per_head) : 0;
+  if (unit0 < total) {
+    long long at = unit0 - head0 * per_head - upto;
+    if (at >= 0 && at < mine) {
+      for (int r = lo; r < hi; ++r) {
+        Request q;
+        q.set(p, __ldg(p.a.cu_q + r), __ldg(p.a.cu_q + r + 1), __ldg(p.a.seq + r));
+        const long long w = pages_before(p, q, q.tiles);
+        if (at < w) {
+          s_place[0] = at;
+          s_place[1] = r;
+          break;
+        }
+        at -= w;
+      }
+    }
+  }
+  __syncthreads();
+  const uint32_t tmem = static_cast<uint32_t>(misc[0]);
+  uint32_t fills = 0;
+
+  if (warp == C::LOADER) {
+    // --------------------------------------------------------------- loader
+    int entries = 0, slot = 0, phase = 0;
+    bool ok = true;
+    const auto post = [&](int type, int x0, int x1, int x2, int x3, int x4, int x5) {
+      const int e = entries % INFO;
+      ok = ok && mbar_wait_warp(bar(C::B_INFO_EMPTY + e), ((entries / INFO) & 1) ^ 1, guard, 0xc00);
+      if (!ok) return;
+      if (lane == 0) {
+        int4* to = reinterpret_cast<int4*>(gbase + C::OFF_INFO + 32 * e);
+        to[0] = make_int4(type, x0, x1, x2);
+        to[1] = make_int4(x3, x4, x5, 0);
+        mbar_arrive(bar(C::B_INFO_FULL + e));
+      }
+      ++entries;
+    };
+    const auto load = [&](const CUtensorMap* map, int row) {
+      ok = ok && mbar_wait_warp(bar(C::B_EMPTY + slot), phase ^ 1, guard, 0xc01);
+      if (!ok) return;
+      if (elect_one()) {
+        mbar_expect_tx(bar(C::B_FULL + slot), TILE_BYTES);
+        tma_load_2d(base + C::OFF_RING + slot * TILE_BYTES, map, 0, row, bar(C::B_FULL + slot));
+      }
+      __syncwarp();
+      ++fills;
+      if (++slot == SLOTS) {
+        slot = 0;
+        phase ^= 1;
+      }
+    };
+    if (unit0 < total) {
+      long long left = unit1 - unit0;
+      int head = head0, r = static_cast<int>(s_place[1]), tile;
+      long long off = s_place[0];
+      // requests come 32 at a time, one per lane
+      int block = -1, c0 = 0, c1 = 0, sq = 0;
+      Request q;
+      const auto fetch = [&](int want) {
+        if (want >> 5 != block) {
+          block = want >> 5;
+          const int i = block * 32 + lane;
+          const bool in = i < p.a.batch;
+          c0 = in ? __ldg(p.a.cu_q + i) : 0;
+          c1 = in ? __ldg(p.a.cu_q + i + 1) : 0;
+          sq = in ? __ldg(p.a.seq + i) : 0;
+        }
+        q.set(p, __shfl_sync(0xffffffffu, c0, want & 31), __shfl_sync(0xffffffffu, c1, want & 31),
+              __shfl_sync(0xffffffffu, sq, want & 31));
+      };
+      fetch(r);
+      tile = warp_last_at_most(q.tiles, off, [&](int t) { return pages_before(p, q, t); });
+      off -= pages_before(p, q, tile);
+      long long start = unit0 - off;               // first unit of the item
+      while (ok && left > 0) {
+        const int token0 = tile * p.pack, tokens = min(p.pack, q.n - token0);
+        const long long seen0 = p.a.causal ? static_cast<long long>(q.k_len) - q.n + token0 + 1 : q.k_len;   // keys of token 0
+        const long long seen = p.a.causal ? seen0 + tokens - 1 : q.k_len;
+        const int count = static_cast<int>(pages_before(p, q, tile + 1) - pages_before(p, q, tile));
+        const int from = static_cast<int>(off), to = static_cast<int>(min(static_cast<long long>(count), off + left));
+        const int x0 = static_cast<int>(start / share), x1 = static_cast<int>((start + count - 1) / share);
+        post(START, q.begin + token0, tokens, head, x0 == x1 ? -1 : 2 * static_cast<int>(blockIdx.x) + (x0 == static_cast<int>(blockIdx.x)), x0, x1);
+        const int32_t* list = nullptr;
+        if (p.a.ids) {
+          const long long lists = p.a.tile == 1 ? p.a.total_q : p.a.total_q / p.a.tile + p.a.batch;
+          list = p.a.ids + (head * lists + first_list_row(q.begin, r, p.a.tile) + token0 / p.a.tile) * p.a.topk;
+        }
+        const int32_t* table = p.a.table + r * p.a.table_stride;
+        for (int at = from; ok && at < to; at += 32) {
+          int j = at + lane;
+          bool live = j < to;
+          if (live && list) j = __ldg(list + j);
+          live = live && j >= 0 && j < q.held && j * 128LL < seen;
+          int row = 0;
+          float ks = 0.f, vs = 0.f;
+          if (live) {
+            const int page = __ldg(table + j);
+            live = page >= 0 && page < p.a.pages;
+            if (live) {
+              row = page * p.a.hkv + head;
+              ks = __ldg(p.a.k_scale + row);
+              vs = __ldg(p.a.v_scale + row);
+            }
+          }
+          uint32_t todo = __ballot_sync(0xffffffffu, live);
+          while (ok && todo) {
+            const int l = __ffs(todo) - 1;
+            todo &= todo - 1;
+            const int pj = __shfl_sync(0xffffffffu, j, l), prow = __shfl_sync(0xffffffffu, row, l);
+            const int pks = __shfl_sync(0xffffffffu, __float_as_int(ks), l), pvs = __shfl_sync(0xffffffffu, __float_as_int(vs), l);
+            const int valid = static_cast<int>(min(128LL, q.k_len - pj * 128LL));
+            // keys of the page that the first token sees; the others one more each. Not causal: all see the same.
+            const int limit = static_cast<int>(max(-128LL, min(128LL, seen0 - pj * 128LL)));
+            post(PAGE, prow, valid, limit, pks, pvs, 0);
+            load(&k_map, prow * 128);
+            load(&v_map, prow * 128);
+          }
+        }
+        post(END, 0, 0, 0, 0, 0, 0);
+        left -= to - from;
+        start += count;
+        off = 0;
+        if (++tile >= q.tiles && left > 0) {       // the next request that has tokens; behind the last one the next head
+          tile = 0;
+          do {
+            if (++r == p.a.batch) {
+              r = 0;
+              ++head;
+            }
+            fetch(r);
+          } while (q.tiles == 0);
+        }
+      }
+    }
+    post(STOP, 0, 0, 0, 0, 0, 0);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  } else if (warp == C::MMA) {
+    // --------------------------------------------------------------- MMA issuer
+    constexpr uint32_t ID_QK = idesc_e4m3(N, false), ID_PV = idesc_e4m3(N, true);
+    bool ok = true;
+    int entries = 0, items = 0, pages = 0, pending = -1;
+    bool new_item = false;
+    const auto second_product = [&]() {            // of page `pending`
+      const int i = pending, b = i & 1, use = i >> 1, n = 2 * i + 1, s = n % SLOTS;
+      ok = ok && mbar_wait_warp(bar(C::B_P_FULL + b), use & 1, guard, 0xc10) &&
+           mbar_wait_warp(bar(C::B_FULL + s), (n / SLOTS) & 1, guard, 0xc11) &&
+           mbar_wait_warp(bar(C::B_O_EMPTY + b), (use & 1) ^ 1, guard, 0xc12);
+      pending = -1;
+      if (!ok) return;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t v = base + C::OFF_RING + s * TILE_BYTES, pr = base + C::OFF_P + b * N * 128;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          mma_e4m3(tmem + 2 * N + b * N, desc_sw128_mnmajor(v + k * 4096, TILE_BYTES, 1024), desc_sw32_mnmajor(pr + k * 1024), ID_PV, k > 0);
+        tc_commit(bar(C::B_O_FULL + b));
+        tc_commit(bar(C::B_EMPTY + s));
+      }
+      __syncwarp();
+    };
+    // Waits for a barrier; issues the second product of the last page as soon as its probabilities are there.
+    const auto wait_for = [&](int which, uint32_t parity, int code) {
+      const long long t0 = clock64();
+      while (ok && pending >= 0 && !__all_sync(0xffffffffu, mbar_test_wait(bar(which), parity))) {
+        if (__all_sync(0xffffffffu, mbar_test_wait(bar(C::B_P_FULL + (pending & 1)), (pending >> 1) & 1))) second_product();
+        if (__any_sync(0xffffffffu, clock64() - t0 > WAIT_LIMIT_CYCLES || *guard.abort_flag)) break;   // the wait below settles it
+      }
+      ok = ok && mbar_wait_warp(bar(which), parity, guard, code);
+    };
+    while (ok) {
+      const int e = entries % INFO;
+      wait_for(C::B_INFO_FULL + e, (entries / INFO) & 1, 0xc13);
+      if (!ok) break;
+      const int type = *reinterpret_cast<volatile int*>(gbase + C::OFF_INFO + 32 * e);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(C::B_INFO_EMPTY + e));
+      ++entries;
+      if (type == STOP) break;
+      if (type == START) {
+        new_item = true;
+      } else if (type == END) {
+        if (new_item) wait_for(C::B_Q_FULL + (items & 1), (items >> 1) & 1, 0xc14);   // an item without pages
+        if (ok && elect_one()) tc_commit(bar(C::B_Q_EMPTY + (items & 1)));
+        __syncwarp();
+        ++items;
+      } else {
+        const int b = pages & 1, n = 2 * pages, s = n % SLOTS;
+        if (new_item) wait_for(C::B_Q_FULL + (items & 1), (items >> 1) & 1, 0xc15);
+        new_item = false;
+        wait_for(C::B_FULL + s, (n / SLOTS) & 1, 0xc16);
+        wait_for(C::B_S_EMPTY + b, ((pages >> 1) & 1) ^ 1, 0xc17);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t kt = base + C::OFF_RING + s * TILE_BYTES, qt = base + C::OFF_Q + (items & 1) * N * 128;
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mma_e4m3(tmem + b * N, desc_sw128_kmajor(kt + k * 32), desc_sw128_kmajor(qt + k * 32), ID_QK, k > 0);
+          tc_commit(bar(C::B_S_FULL + b));
+          tc_commit(bar(C::B_EMPTY + s));
+        }
+        __syncwarp();
+        if (pending >= 0) second_product();
+        pending = pages++;
+      }
+    }
+    if (ok && pending >= 0) second_product();
+    // nothing of the tensor core's is in flight when the CTA gives up its memory
+    if (elect_one()) tc_commit(bar(C::B_DONE));
+    __syncwarp();
+    mbar_wait_drain(bar(C::B_DONE), 0);
+  } else if (warp >= C::QWARP) {
+    // --------------------------------------------------------------- queries of the next item
+    const int half = warp - C::QWARP;
+    bool ok = true;
+    int entries = 0, items = 0;
+    const float sign = p.a.scale < 0.f ? -1.f : 1.f, factor = fabsf(p.a.scale) * 1.4426950408889634f;
+    while (ok) {
+      const int e = entries % INFO;
+      ok = mbar_wait_warp(bar(C::B_INFO_FULL + e), (entries / INFO) & 1, guard, 0xc20);
+      if (!ok) break;
+      const int4 x = *reinterpret_cast<const int4*>(gbase + C::OFF_INFO + 32 * e);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(C::B_INFO_EMPTY + e));
+      ++entries;
+      if (x.x == STOP) break;
+      if (x.x != START) continue;
+      const int buf = items & 1;
+      ok = mbar_wait_warp(bar(C::B_Q_EMPTY + buf), ((items >> 1) & 1) ^ 1, guard, 0xc21);
+      if (!ok) break;
+      const int rows = x.z * p.group;              // tokens x heads of the KV head
+      unsigned char* q8 = gbase + C::OFF_Q + buf * N * 128;
+      float* qf = reinterpret_cast<float*>(gbase + C::OFF_QF) + buf * R;
+      const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.a.q) + x.y * p.a.q_token +
+                                 static_cast<long long>(x.w) * p.group * p.a.q_head + lane * 4;
+      for (int r0 = half * 8; r0 < R; r0 += 16) {
+        uint2 w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int row = r0 + i, t = row / p.group, g = row - t * p.group;
+          w[i] = row < rows ? __ldg(reinterpret_cast<const uint2*>(src + t * p.a.q_token + g * p.a.q_head)) : make_uint2(0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int row = r0 + i;
+          const uint32_t m = __vmaxu2(w[i].x & 0x7fff7fffu, w[i].y & 0x7fff7fffu);
+          const uint32_t top = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
+          // times 2^e the largest feature lies in [128, 256); a row with infinities or NaN is taken as it is and ends as NaN
+          const int e = top == 0 || top >= 0x7f80u ? 0 : min(134 - static_cast<int>(top >> 7), 126);
+          const float by = power_of_two(e) * sign;
+          const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i].x));
+          const float2 c = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i].y));
+          const float v[4] = {a.x * by, a.y * by, c.x * by, c.y * by};
+          uint32_t hi = e4m3x2(v[0], v[1]) | (e4m3x2(v[2], v[3]) << 16), rest = 0;
+          float low[4];
+#pragma unroll
+          for (int d = 0; d < 4; ++d) low[d] = (v[d] - from_e4m3(hi >> (8 * d) & 0xffu)) * 16.f;
+          rest = e4m3x2(low[0], low[1]) | (e4m3x2(low[2], low[3]) << 16);
+          if (top >= 0x7f80u) {
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+              if (!(fabsf(v[d]) < INFINITY)) hi |= 0x7fu << (8 * d);
+          }
+          const int chunk = ((lane >> 2) ^ (row & 7)) * 16 + (lane & 3) * 4;
+          *reinterpret_cast<uint32_t*>(q8 + row * 128 + chunk) = hi;
+          *reinterpret_cast<uint32_t*>(q8 + (R + row) * 128 + chunk) = rest;
+          if (lane == 0) qf[row] = factor * power_of_two(-e);
+        }
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(C::B_Q_FULL + buf));
+      ++items;
+    }
+  } else {
+    // --------------------------------------------------------------- softmax: lane = key, then lane = feature
+    const int wg = warp >> 2, quarter = warp & 3, key = quarter * 32 + lane, row0 = wg * 16, r16 = lane & 15;
+    const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+    float4* factors = reinterpret_cast<float4*>(gbase + C::OFF_FACTOR) + warp * 16;
+    float2* outs = reinterpret_cast<float2*>(gbase + C::OFF_OUT) + warp * 16;           // + parity * SOFTMAX_WARPS * 16
+    float* maxima = reinterpret_cast<float*>(gbase + C::OFF_MAX) + wg * 64;             // [4][16]
+    float* sums = reinterpret_cast<float*>(gbase + C::OFF_SUM) + wg * 64;
+    const float* qf = reinterpret_cast<const float*>(gbase + C::OFF_QF);
+    float acc[16], l[16], m = -INFINITY, scale_row = 0.f;
+    int entries = 0, items = 0, pages = 0, pending = -1, masked = 0;
+    int token0 = 0, tokens = 0, head = 0, place = -1, x0 = 0, x1 = 0;
+    // of the pending page, for rows that do not see all of its keys
+    int p_row = 0, p_limit = 0, p_valid = 0;
+    bool ok = true, fresh = false;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[i] = l[i] = 0.f;
+
+    // adds the output of page `pending` to acc
+    const auto add_output = [&]() {
+      const int b = pending & 1;
+      ok = ok && mbar_wait_warp(bar(C::B_O_FULL + b), (pending >> 1) & 1, guard, 0xc30);
+      const int i = pending;
+      pending = -1;
+      if (!ok) return;
+      tc_fence_after();
+      uint32_t h[16], w[16];
+      tmem_ld16(tmem + lane_base + 2 * N + b * N + row0, h);
+      tmem_ld16(tmem + lane_base + 2 * N + b * N + R + row0, w);
+      tc_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(C::B_O_EMPTY + b));
+      const float2* f = outs + (i & 1) * C::SOFTMAX_WARPS * 16;
+      float o[16];
+#pragma unroll
+      for (int j = 0; j < 16; ++j) o[j] = fmaf(__uint_as_float(w[j]), 0.0625f, __uint_as_float(h[j]));
+      if (masked) {
+        // A key that is hidden from a row has probability 0 there, and 0 times a NaN of its value is not 0: such a sum is
+        // done again over the keys that the row sees, from the probabilities in shared memory.
+#pragma unroll 1
+        for (int j = 0; j < 16; ++j) {
+          float x = 0.f;
+#pragma unroll
+          for (int jj = 0; jj < 16; ++jj) x = jj == j ? o[jj] : x;
+          if (x == x) continue;
+          const int limit = min(p.a.causal ? p_limit + (row0 + j) / p.group : p_limit, p_valid);
+          const uint8_t* pr = gbase + C::OFF_P + (i & 1) * N * 128;
+          const uint8_t* v = static_cast<const uint8_t*>(p.a.v) + static_cast<long long>(p_row) * TILE_BYTES + key;
+          const int c0 = row0 + j, c1 = R + row0 + j;
+          x = 0.f;
+          for (int n = 0; n < limit; ++n) {
+            const auto at = [&](int c) { return from_e4m3(pr[(c >> 5) * 4096 + n * 32 + ((((c >> 4) ^ (n >> 2)) & 1) << 4) + (c & 15)]); };
+            x = fmaf(fmaf(at(c1), 0.0625f, at(c0)), from_e4m3(__ldg(v + n * 128)), x);
+          }
+#pragma unroll
+          for (int jj = 0; jj < 16; ++jj) o[jj] = jj == j ? x : o[jj];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float2 c = f[j];
+        acc[j] = fmaf(acc[j], c.x, o[j] * c.y);
+      }
+    };
+
+    while (ok) {
+      const int e = entries % INFO;
+      ok = mbar_wait_warp(bar(C::B_INFO_FULL + e), (entries / INFO) & 1, guard, 0xc31);
+      if (!ok) break;
+      const int4 x = *reinterpret_cast<const int4*>(gbase + C::OFF_INFO + 32 * e);
+      const int4 y = *reinterpret_cast<const int4*>(gbase + C::OFF_INFO + 32 * e + 16);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(C::B_INFO_EMPTY + e));
+      ++entries;
+      if (x.x == STOP) break;
+      if (x.x == START) {
+        token0 = x.y;
+        tokens = x.z;
+        head = x.w;
+        place = y.x;
+        x0 = y.y;
+        x1 = y.z;
+        m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[i] = l[i] = 0.f;
+        fresh = true;
+        continue;
+      }
+      if (x.x == PAGE) {
+        const int b = pages & 1, row = x.y, valid = x.z, limit = x.w;
+        const float ks = __int_as_float(y.x), vs = __int_as_float(y.y);
+        if (fresh) {
+          ok = mbar_wait_warp(bar(C::B_Q_FULL + (items & 1)), (items >> 1) & 1, guard, 0xc32);
+          if (!ok) break;
+          scale_row = qf[(items & 1) * R + row0 + r16];
+          fresh = false;
+        }
+        ok = mbar_wait_warp(bar(C::B_S_FULL + b), (pages >> 1) & 1, guard, 0xc33);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t h[16], w[16];
+        tmem_ld16(tmem + lane_base + b * N + row0, h);
+        tmem_ld16(tmem + lane_base + b * N + R + row0, w);
+        tc_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::B_S_EMPTY + b));
+        float s[16];
+        const bool partial = valid < 128 || limit < 128;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[j] = fmaf(__uint_as_float(w[j]), 0.0625f, __uint_as_float(h[j]));
+        uint32_t hidden = 0;                       // rows that do not see this key
+        if (partial) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int sees = min(p.a.causal ? limit + (row0 + j) / p.group : limit, valid);
+            if (key >= sees) {
+              hidden |= 1u << j;
+              s[j] = -INFINITY;
+            }
+          }
+        }
+        float top = 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float t = warp_max(s[j]);
+          top = r16 == j ? t : top;
+        }
+        float* mx = maxima + b * C::SOFTMAX_WARPS * 16;
+        if (lane < 16) mx[quarter * 16 + lane] = top;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::B_MAX + 2 * wg + b));
+        ok = mbar_wait_warp(bar(C::B_MAX + 2 * wg + b), (pages >> 1) & 1, guard, 0xc36);
+        if (!ok) break;
+        top = fmaxf(fmaxf(mx[r16], mx[16 + r16]), fmaxf(mx[32 + r16], mx[48 + r16]));
+        {
+          const float f = scale_row * ks;
+          const bool none = top == -INFINITY;
+          const float mu = none ? -INFINITY : top * f;
+          const float next = fmaxf(m, mu);
+          const float c1 = m == -INFINITY ? 0.f : ex2_approx(m - next);
+          const float c2 = none ? 0.f : ex2_approx(mu - next);
+          m = next;
+          if (lane < 16) {
+            factors[lane] = make_float4(f, none ? 0.f : 8.f - mu, c1, c2);
+            outs[(pages & 1) * C::SOFTMAX_WARPS * 16 + lane] = make_float2(c1, c2 * vs * 0.00390625f);
+          }
+        }
+        __syncwarp();
+        uint32_t ph[4], pl[4];
+#pragma unroll
+        for (int j4 = 0; j4 < 4; ++j4) {
+          float pr[4], cut[4];
+#pragma unroll
+          for (int jj = 0; jj < 4; ++jj) {
+            const int j = 4 * j4 + jj;
+            const float4 f = factors[j];
+            float v = ex2_approx(fmaf(s[j], f.x, f.y));
+            if (partial && (hidden >> j & 1)) v = 0.f;
+            l[j] = fmaf(l[j], f.z, v * f.w);
+            cut[jj] = __uint_as_float(__float_as_uint(v) & 0xfff00000u);     // four significant bits
+            pr[jj] = (v - cut[jj]) * 16.f;
+          }
+          ph[j4] = e4m3x2(cut[0], cut[1]) | (e4m3x2(cut[2], cut[3]) << 16);
+          pl[j4] = e4m3x2(pr[0], pr[1]) | (e4m3x2(pr[2], pr[3]) << 16);
+        }
+        unsigned char* to = gbase + C::OFF_P + b * N * 128 + key * 32;
+        const auto column = [&](int c) { return to + (c >> 5) * 4096 + ((((c >> 4) ^ (key >> 2)) & 1) << 4); };
+        *reinterpret_cast<uint4*>(column(row0)) = make_uint4(ph[0], ph[1], ph[2], ph[3]);
+        *reinterpret_cast<uint4*>(column(R + row0)) = make_uint4(pl[0], pl[1], pl[2], pl[3]);
+        if (valid < 128 && wg == 0) {
+          // rows behind the sequence may hold anything: they become zeros before the second product reads them
+          const int n = 2 * pages + 1, vslot = n % SLOTS;
+          ok = mbar_wait_warp(bar(C::B_FULL + vslot), (n / SLOTS) & 1, guard, 0xc34);
+          if (!ok) break;
+          if (key >= valid) {
+            uint4* v = reinterpret_cast<uint4*>(gbase + C::OFF_RING + vslot * TILE_BYTES + key * 128);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = make_uint4(0, 0, 0, 0);
+          }
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::B_P_FULL + b));
+        if (pending >= 0) add_output();
+        pending = pages++;
+        masked = limit < valid;
+        p_row = row;
+        p_limit = limit;
+        p_valid = valid;
+        continue;
+      }
+      // END
+      if (pending >= 0) add_output();
+      if (!ok) break;
+      if (fresh) {                                 // an item without pages
+        ok = mbar_wait_warp(bar(C::B_Q_FULL + (items & 1)), (items >> 1) & 1, guard, 0xc35);
+        if (!ok) break;
+        fresh = false;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(C::B_Q_EMPTY + (items & 1)));
+      float* sm = sums + (items & 1) * C::SOFTMAX_WARPS * 16;
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        float t = l[j];
+#pragma unroll
+        for (int by = 16; by; by >>= 1) t += __shfl_xor_sync(0xffffffffu, t, by);
+        sum = r16 == j ? t : sum;
+      }
+      if (lane < 16) sm[quarter * 16 + lane] = sum;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(C::B_SUM + 2 * wg + (items & 1)));
+      ok = mbar_wait_warp(bar(C::B_SUM + 2 * wg + (items & 1)), (items >> 1) & 1, guard, 0xc37);
+      if (!ok) break;
+      const int rows = tokens * p.group;
+      if (place < 0) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int row = row0 + j;
+          if (row >= rows) break;
+          const float t = ((sm[j] + sm[16 + j]) + (sm[32 + j] + sm[48 + j])) * 0.00390625f;
+          const int tok = row / p.group;
+          const long long to = (static_cast<long long>(token0) + tok) * p.a.hq + head * p.group + (row - tok * p.group);
+          static_cast<__nv_bfloat16*>(p.a.out)[to * 128 + key] = __float2bfloat16(t == 0.f ? 0.f : acc[j] / t);
+        }
+        if (p.a.lse && quarter == 0 && lane < 16 && row0 + lane < rows) {
+          const float t = ((sm[lane] + sm[16 + lane]) + (sm[32 + lane] + sm[48 + lane])) * 0.00390625f;
+          const int row = row0 + lane, tok = row / p.group;
+          p.a.lse[(static_cast<long long>(token0) + tok) * p.a.hq + head * p.group + (row - tok * p.group)] =
+              t == 0.f ? -INFINITY : (m + log2f(t)) * 0.6931471805599453f;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          if (row0 + j >= rows) break;
+          p.part_o[(static_cast<long long>(place) * R + row0 + j) * 128 + key] = acc[j];
+        }
+        if (quarter == 0 && lane < 16)
+          *reinterpret_cast<float2*>(p.part_ml + (static_cast<long long>(place) * R + row0 + lane) * 2) =
+              make_float2(m, ((sm[lane] + sm[16 + lane]) + (sm[32 + lane] + sm[48 + lane])) * 0.00390625f);
+        if (warp == 0 && lane == 0) {
+          int* meta = p.part_meta + 8 * place;
+          meta[1] = x0;
+          meta[2] = x1;
+          meta[3] = token0;
+          meta[4] = tokens;
+          meta[5] = head;
+          meta[0] = 1;
+        }
+      }
+      ++items;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == C::LOADER && misc[1]) {               // a wait was given up: copies in flight land before the CTA leaves
+    for (uint32_t f = fills > SLOTS ? fills - SLOTS : 0; f < fills; ++f) mbar_wait_drain(bar(C::B_FULL + f % SLOTS), (f / SLOTS) & 1);
+  }
+  if (warp == C::MMA) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::TMEM);
   }
 }
 
-}  // namespace
+// Adds the parts of the items that lie in several shares, in order:
+//   M = max_i m_i, w_i = exp2(m_i - M), out = sum w_i acc_i / sum w_i l_i, lse = ln 2 (M + log2 sum w_i l_i)
+// CTA x stands at the border of shares x and x + 1; the n - 1 CTAs at the borders inside an item of n parts divide its rows
+// and features among them: a piece is a row's 32 features, done by a whole CTA, a warp takes every eighth part.
+constexpr int MERGE_WARPS = 8;
+template <int R>
+__global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const Params p) {
+  __shared__ float s_w[MERGE_WARPS], s_acc[MERGE_WARPS][32], s_l[MERGE_WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int x = blockIdx.x + 1;
+  const int* meta = p.part_meta + 16 * x;          // the part that comes from the share before
+  if (meta[0] == 0) return;
+  const int x0 = meta[1], x1 = meta[2], token0 = meta[3], tokens = meta[4], head = meta[5];
+  const int parts = x1 - x0 + 1, pieces = tokens * p.group * 4;
+  for (int piece = x - x0 - 1; piece < pieces; piece += parts - 1) {
+    const int row = piece >> 2, d = (piece & 3) * 32 + lane;
+    const auto place = [&](int i) { return static_cast<long long>(2 * (x0 + i) + (i == 0)) * R + row; };
+    float top = -INFINITY;
+    for (int i = threadIdx.x; i < parts; i += 32 * MERGE_WARPS) top = fmaxf(top, p.part_ml[place(i) * 2]);
+    top = pa::warp_max(top);
+    if (lane == 0) s_w[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < MERGE_WARPS; ++w) top = fmaxf(top, s_w[w]);
+    float acc = 0.f, l = 0.f;
+#pragma unroll 8
+    for (int i = warp; i < parts; i += MERGE_WARPS) {
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + place(i) * 2);
+      const float o = p.part_o[place(i) * 128 + d];
+      const float w = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - top);
+      acc = fmaf(w, o, acc);
+      l = fmaf(w, ml.y, l);
+    }
+    s_acc[warp][lane] = acc;
+    if (lane == 0) s_l[warp] = l;
+    __syncthreads();
+    if (warp == 0) {
+      acc = l = 0.f;
+#pragma unroll
+      for (int w = 0; w < MERGE_WARPS; ++w) {
+        acc += s_acc[w][lane];
+        l += s_l[w];
+      }
+      const int tok = row / p.group;
+      const long long to = (static_cast<long long>(token0) + tok) * p.a.hq + head * p.group + (row - tok * p.group);
+      static_cast<__nv_bfloat16*>(p.a.out)[to * 128 + d] = __float2bfloat16(l == 0.f ? 0.f : acc / l);
+      if (p.a.lse && d == 0) p.a.lse[to] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+    }
+    __syncthreads();
+  }
+}
 
-long long paged_attention_workspace_bytes(int, int, int, int, bool, int) { return 0; }
+// Tokens that share a pass over the pages: as many as 64 rows hold, a power of two, no more than there are.
+static int pack_of(int group, int tile, int max_q, bool listed) {
+  int pack = 1;
+  while (2 * pack * group <= 64 && pack < max_q && (!listed || 2 * pack <= tile)) pack *= 2;
+  return pack;
+}
+static int rows_of(int group, int pack) { return pack * group <= 16 ? 16 : pack * group <= 32 ? 32 : 64; }
+
+template <int R>
+static int launch(const PagedAttentionArgs& a, int pack, DeviceCtx* ctx, int slot, cudaStream_t stream) {
+  using C = Config<R>;
+  Params p{a, a.hq / a.hkv, pack, ctx->sm_count * C::CTAS, nullptr, nullptr, nullptr};
+  unsigned char* ws = static_cast<unsigned char*>(a.workspace);
+  p.part_o = reinterpret_cast<float*>(ws);
+  p.part_ml = p.part_o + static_cast<long long>(2) * p.ctas * R * 128;
+  p.part_meta = reinterpret_cast<int*>(p.part_ml + static_cast<long long>(2) * p.ctas * R * 2);
+  CUtensorMap km, vm;
+  const cuuint64_t dims[2] = {128, static_cast<cuuint64_t>(a.pages) * a.hkv * 128};
+  const cuuint64_t strides[1] = {128};
+  const cuuint32_t box[2] = {128, 128}, steps[2] = {1, 1};
+  for (int i = 0; i < 2; ++i)
+    if (encode_tiled(i ? &vm : &km, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(i ? a.v : a.k), dims, strides, box, steps,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B))
+      return set_error(SB_ERR_CUDA, "tensor map of the cache pages");
+  auto kernel = paged_attention_kernel<R>;
+  if (!ctx->paged_attr[slot]) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
+      return set_error(SB_ERR_CUDA, "shared memory of the paged attention");
+    ctx->paged_attr[slot] = 1;
+  }
+  kernel<<<p.ctas, C::THREADS, C::SMEM, stream>>>(km, vm, p, ctx->status);
+  int rc = check_kernel_launch();
+  if (rc) return rc;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.ctas - 1);
+  cfg.blockDim = dim3(32 * MERGE_WARPS);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_merge_kernel<R>, p);
+  return e == cudaSuccess ? SB_OK : set_error(SB_ERR_CUDA, cudaGetErrorString(e));
+}
+
+}  // namespace pa
+
+long long paged_attention_workspace_bytes(int hq, int hkv, int tile, int max_q, bool listed, int sm_count) {
+  const int rows = pa::rows_of(hq / hkv, pa::pack_of(hq / hkv, tile, max_q, listed));
+  const long long ctas = static_cast<long long>(sm_count) * (rows == 64 ? pa::Config<64>::CTAS : pa::Config<32>::CTAS);
+  return 2 * ctas * (rows * 130 * 4LL + 32);
+}
 
 int launch_paged_attention(const PagedAttentionArgs& a, cudaStream_t stream) {
-  paged_attention_kernel<<<dim3(a.total_q, a.hkv), THREADS, 0, stream>>>(a);
-  return check_kernel_launch();
+  DeviceCtx* ctx = device_ctx();
+  if (!ctx) return SB_ERR_CUDA;
+  const int group = a.hq / a.hkv, pack = pa::pack_of(group, a.tile, a.max_q, a.ids != nullptr), rows = pa::rows_of(group, pack);
+  if (!a.workspace || a.workspace_bytes < paged_attention_workspace_bytes(a.hq, a.hkv, a.tile, a.max_q, a.ids != nullptr, ctx->sm_count))
+    return set_error(SB_ERR_INVALID, "workspace too small (see sparse_b200_paged_attention_workspace_bytes)");
+  return rows == 16 ? pa::launch<16>(a, pack, ctx, 4, stream)
+                    : rows == 32 ? pa::launch<32>(a, pack, ctx, 5, stream) : pa::launch<64>(a, pack, ctx, 6, stream);
 }
 
 }  // namespace sb

@@ -294,10 +294,10 @@ def _check_attention(sp, q, c, table, seq, cu, ids=None, tile=1, causal=True, sc
     assert torch.equal(out.isnan(), want.isnan()) and torch.equal(lse.isnan(), want_lse.isnan())
     assert torch.equal(lse == -math.inf, want_lse == -math.inf)
     ok, ok_l = ~want.isnan(), want_lse.isfinite()
-    # Scores: the 128 products are summed in 32 bits, in four steps of 32 whose terms are aligned to the largest with at least
-    # 13 fractional bits below it in the worst case: 2^-13 of sum |q k| bounds it, and so the natural-log LSE (one more
-    # 2^-20 |lse| for the logarithm and exponentials).
-    score = 2.0 ** -13 * size + 1e-6
+    # Scores: 128 products are summed in 32 bits, each addition rounds by 2^-24 of the sum of magnitudes at most: 2^-17 of
+    # sum |q k|; features of a query below 2^-22 of its largest lose up to 2^-23 of the largest: 128 of them 2^-16. So does the
+    # natural-log LSE (2^-20 |lse| more for the logarithm and the exponentials).
+    score = 2.0 ** -15 * size + 1e-6
     assert ((lse - want_lse).abs()[ok_l] <= (score + 2.0 ** -20 * want_lse.abs())[ok_l]).all()
     # Outputs: each probability carries exp(2 score error) and half a step of its 8-bit mantissa (2^-8), the output half a
     # step of bf16 (2^-8).
@@ -514,7 +514,7 @@ def test_steps_of_a_serving_loop(sp):
         want, _, spread, size = ref.paged_attention(q, host["k"], host["v"], host["k_scale"], host["v_scale"], table.cpu(),
                                                     b.seq_lens.cpu(), cu, ids.cpu(), tile)
         # as in _check_attention
-        bound = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2 * (2.0 ** -13 * size[..., None] + 1e-6)) * spread * 1.01 + 1e-30
+        bound = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2 * (2.0 ** -15 * size[..., None] + 1e-6)) * spread * 1.01 + 1e-30
         assert ((out.cpu().double() - want).abs() <= bound).all()
         dense, none = sp.paged_step(q.cuda(), g[:, hkv * group:-hkv], g[:, -hkv:], cache, table, b, max_seqlen_q=max(lens),
                                     max_seqlen_k=int(b.seq_lens.max()))
