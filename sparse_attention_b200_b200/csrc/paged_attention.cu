@@ -35,7 +35,7 @@ namespace pa {
 
 constexpr int TILE_BYTES = 128 * 128;
 constexpr int INFO = 16;                          // entries in flight
-constexpr int START = 1, PAGE = 2, END = 3, STOP = 4;
+constexpr int START = 1, PAGE = 2, END = 3, EMPTY = 4, STOP = 5;
 constexpr int MIN_SHARE = 4;                      // pages of a CTA at least
 
 struct Params {
@@ -57,18 +57,18 @@ struct Config {
   static constexpr int OFF_RING = 0;
   static constexpr int OFF_Q = OFF_RING + SLOTS * TILE_BYTES;       // two buffers of N rows of 128 bytes
   static constexpr int OFF_P = OFF_Q + 2 * N * 128;                 // two buffers of 128 keys x N columns
-  static constexpr int OFF_FACTOR = OFF_P + 2 * N * 128;            // float4 [softmax warp][16]
-  static constexpr int OFF_OUT = OFF_FACTOR + SOFTMAX_WARPS * 256;  // float2 [2][softmax warp][16]
+  static constexpr int OFF_FACTOR = OFF_P + 2 * N * 128;            // float [softmax warp][3][16]
+  static constexpr int OFF_OUT = OFF_FACTOR + SOFTMAX_WARPS * 192;  // float [2][softmax warp][2][16]
   static constexpr int OFF_MAX = OFF_OUT + 2 * SOFTMAX_WARPS * 128; // float [2][softmax warp][16]
   static constexpr int OFF_SUM = OFF_MAX + 2 * SOFTMAX_WARPS * 64;  // float [2][softmax warp][16]
   static constexpr int OFF_QF = OFF_SUM + 2 * SOFTMAX_WARPS * 64;   // float [2][R]: what a row's scores are multiplied by
   static constexpr int OFF_INFO = OFF_QF + 2 * R * 4;               // int [INFO][8]
   static constexpr int OFF_BAR = OFF_INFO + INFO * 32;
   static constexpr int B_INFO_FULL = 0, B_INFO_EMPTY = INFO, B_FULL = 2 * INFO, B_EMPTY = B_FULL + SLOTS;
-  static constexpr int B_S_FULL = B_EMPTY + SLOTS, B_S_EMPTY = B_S_FULL + 2, B_P_FULL = B_S_EMPTY + 2, B_O_FULL = B_P_FULL + 2,
-                       B_O_EMPTY = B_O_FULL + 2, B_Q_FULL = B_O_EMPTY + 2, B_Q_EMPTY = B_Q_FULL + 2, B_MAX = B_Q_EMPTY + 2,
-                       B_SUM = B_MAX + 2 * GROUPS, B_DONE = B_SUM + 2 * GROUPS, BARS = B_DONE + 1;
-  static constexpr int OFF_MISC = OFF_BAR + BARS * 8;
+  static constexpr int B_S_FULL = B_EMPTY + SLOTS, B_P_FULL = B_S_FULL + 2, B_O_FULL = B_P_FULL + 2, B_Q_FULL = B_O_FULL + 2,
+                       B_Q_EMPTY = B_Q_FULL + 2, B_MAX = B_Q_EMPTY + 2, B_SUM = B_MAX + 2 * GROUPS, B_DONE = B_SUM + 2 * GROUPS, BARS = B_DONE + 1;
+  static constexpr int OFF_FLAG = OFF_BAR + BARS * 8;               // int [SLOTS]: for the MMA warp, with a page's K tile
+  static constexpr int OFF_MISC = (OFF_FLAG + SLOTS * 4 + 15) / 16 * 16;
   static constexpr int SMEM = OFF_MISC + 64 + 1024;                 // 1024: alignment of the tiles
   static constexpr int TMEM = 4 * N < 32 ? 32 : 4 * N;              // S0, S1, O0, O1
 };
@@ -77,25 +77,48 @@ struct Config {
 __host__ __device__ constexpr uint32_t idesc_e4m3(int n, bool mn_major) {
   return (1u << 4) | (mn_major ? (1u << 15) | (1u << 16) : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (8u << 24);
 }
-__device__ __forceinline__ void mma_e4m3(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// Operands by the low words of their descriptors (start address and leading offset, in units of 16 bytes); the high words
+// are constants. KMAJOR / MN128: 128-byte swizzle, eight rows 1024 bytes apart (a K tile and the queries; a V tile, whose 128
+// features are one panel). MN32: panels of 32 columns, a key's 32 bytes after another, eight keys 256 bytes apart, panels 4096
+// (the probabilities).
+constexpr uint32_t HI_128 = (1024u >> 4) | (1u << 14) | (2u << 29), HI_MN32 = (256u >> 4) | (1u << 14) | (6u << 29);
+constexpr uint32_t LO_MN128 = (static_cast<uint32_t>(TILE_BYTES) >> 4) << 16, LO_MN32 = (4096u >> 4) << 16;
+template <uint32_t HI_B>
+__device__ __forceinline__ void mma_e4m3(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t"
       ".reg .pred p;\n\t"
+      ".reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %5};\n\t"
+      "mov.b64 db, {%2, %6};\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %3, p;\n\t"
       "}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(HI_128), "n"(HI_B)
       : "memory");
-}
-// MN-major operand in panels of 32 columns, 32-byte swizzle: a key's 32 bytes of a panel, eight keys 256 bytes apart, panels
-// 4096 bytes apart.
-__device__ __forceinline__ uint64_t desc_sw32_mnmajor(uint32_t addr) {
-  return desc_field(addr) | (desc_field(4096) << 16) | (desc_field(256) << 32) | (1ULL << 46) | (6ULL << 61);
 }
 __device__ __forceinline__ float warp_max(float x) {
   float y;
   asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
   return y;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  f32x2_unpack(f32x2_mul(f32x2_pack(a.x, a.y), f32x2_pack(b.x, b.y)), d.x, d.y);
+  return d;
+}
+// Maxima over the warp of 16 values: lane l gets that of value l % 16. Every step halves the values that a lane holds.
+__device__ __forceinline__ float row_maxima(const float (&s)[16], int lane) {
+  float a[8], b[4], c[2];
+  const bool h8 = lane & 8, h4 = lane & 4, h2 = lane & 2, h1 = lane & 1;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) a[j] = fmaxf(h8 ? s[j + 8] : s[j], __shfl_xor_sync(0xffffffffu, h8 ? s[j] : s[j + 8], 8));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) b[j] = fmaxf(h4 ? a[j + 4] : a[j], __shfl_xor_sync(0xffffffffu, h4 ? a[j] : a[j + 4], 4));
+#pragma unroll
+  for (int j = 0; j < 2; ++j) c[j] = fmaxf(h2 ? b[j + 2] : b[j], __shfl_xor_sync(0xffffffffu, h2 ? b[j] : b[j + 2], 2));
+  const float d = fmaxf(h1 ? c[1] : c[0], __shfl_xor_sync(0xffffffffu, h1 ? c[0] : c[1], 1));
+  return fmaxf(d, __shfl_xor_sync(0xffffffffu, d, 16));
 }
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
@@ -156,7 +179,7 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
     misc[1] = 0;
     for (int i = 0; i < INFO; ++i) {
       mbar_init(bar(C::B_INFO_FULL + i), 1);
-      mbar_init(bar(C::B_INFO_EMPTY + i), C::SOFTMAX_WARPS + 3);
+      mbar_init(bar(C::B_INFO_EMPTY + i), C::SOFTMAX_WARPS + 2);
     }
     for (int i = 0; i < SLOTS; ++i) {
       mbar_init(bar(C::B_FULL + i), 1);
@@ -164,12 +187,10 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(C::B_S_FULL + i), 1);
-      mbar_init(bar(C::B_S_EMPTY + i), C::SOFTMAX_WARPS);
       mbar_init(bar(C::B_P_FULL + i), C::SOFTMAX_WARPS);
       mbar_init(bar(C::B_O_FULL + i), 1);
-      mbar_init(bar(C::B_O_EMPTY + i), C::SOFTMAX_WARPS);
       mbar_init(bar(C::B_Q_FULL + i), 2);
-      mbar_init(bar(C::B_Q_EMPTY + i), C::SOFTMAX_WARPS + 1);
+      mbar_init(bar(C::B_Q_EMPTY + i), C::SOFTMAX_WARPS);
     }
     for (int i = 0; i < 4 * C::GROUPS; ++i) mbar_init(bar(C::B_MAX + i), 4);
     mbar_init(bar(C::B_DONE), 1);
@@ -235,7 +256,7 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
 
   if (warp == C::LOADER) {
     // --------------------------------------------------------------- loader
-    int entries = 0, slot = 0, phase = 0;
+    int entries = 0, items = -1, slot = 0, phase = 0;
     bool ok = true;
     const auto post = [&](int type, int x0, int x1, int x2, int x3, int x4, int x5) {
       const int e = entries % INFO;
@@ -249,12 +270,18 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
       }
       ++entries;
     };
-    const auto load = [&](const CUtensorMap* map, int row) {
+    // flag: what the MMA warp has to know of a K tile: the number of its item, -1 = there are no more tiles
+    const auto load = [&](const CUtensorMap* map, int row, int flag) {
       ok = ok && mbar_wait_warp(bar(C::B_EMPTY + slot), phase ^ 1, guard, 0xc01);
       if (!ok) return;
       if (elect_one()) {
-        mbar_expect_tx(bar(C::B_FULL + slot), TILE_BYTES);
-        tma_load_2d(base + C::OFF_RING + slot * TILE_BYTES, map, 0, row, bar(C::B_FULL + slot));
+        *reinterpret_cast<volatile int*>(gbase + C::OFF_FLAG + 4 * slot) = flag;
+        if (flag < 0) {
+          mbar_arrive(bar(C::B_FULL + slot));
+        } else {
+          mbar_expect_tx(bar(C::B_FULL + slot), TILE_BYTES);
+          tma_load_2d(base + C::OFF_RING + slot * TILE_BYTES, map, 0, row, bar(C::B_FULL + slot));
+        }
       }
       __syncwarp();
       ++fills;
@@ -293,7 +320,8 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
         const int count = static_cast<int>(pages_before(p, q, tile + 1) - pages_before(p, q, tile));
         const int from = static_cast<int>(off), to = static_cast<int>(min(static_cast<long long>(count), off + left));
         const int x0 = static_cast<int>(start / share), x1 = static_cast<int>((start + count - 1) / share);
-        post(START, q.begin + token0, tokens, head, x0 == x1 ? -1 : 2 * static_cast<int>(blockIdx.x) + (x0 == static_cast<int>(blockIdx.x)), x0, x1);
+        const int place = x0 == x1 ? -1 : 2 * static_cast<int>(blockIdx.x) + (x0 == static_cast<int>(blockIdx.x));
+        bool started = false;
         const int32_t* list = nullptr;
         if (p.a.ids) {
           const long long lists = p.a.tile == 1 ? p.a.total_q : p.a.total_q / p.a.tile + p.a.batch;
@@ -325,12 +353,18 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
             const int valid = static_cast<int>(min(128LL, q.k_len - pj * 128LL));
             // keys of the page that the first token sees; the others one more each. Not causal: all see the same.
             const int limit = static_cast<int>(max(-128LL, min(128LL, seen0 - pj * 128LL)));
+            if (!started) {
+              started = true;
+              ++items;
+              post(START, q.begin + token0, tokens, head, place, x0, x1);
+            }
             post(PAGE, prow, valid, limit, pks, pvs, 0);
-            load(&k_map, prow * 128);
-            load(&v_map, prow * 128);
+            load(&k_map, prow * 128, items);
+            load(&v_map, prow * 128, 0);
           }
         }
-        post(END, 0, 0, 0, 0, 0, 0);
+        if (started) post(END, 0, 0, 0, 0, 0, 0);
+        else post(EMPTY, q.begin + token0, tokens, head, place, x0, x1);      // no page of it is taken: its rows are 0
         left -= to - from;
         start += count;
         off = 0;
@@ -347,78 +381,77 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
       }
     }
     post(STOP, 0, 0, 0, 0, 0, 0);
+    load(&k_map, 0, -1);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   } else if (warp == C::MMA) {
     // --------------------------------------------------------------- MMA issuer
+    // Waits by the whole warp, issue by its elected lane. That S and O of a page may be overwritten by the page after the
+    // next needs no barrier: the softmax warps store the probabilities of a page after they have read its S and the O of the
+    // page before the last.
     constexpr uint32_t ID_QK = idesc_e4m3(N, false), ID_PV = idesc_e4m3(N, true);
-    bool ok = true;
-    int entries = 0, items = 0, pages = 0, pending = -1;
-    bool new_item = false;
-    const auto second_product = [&]() {            // of page `pending`
-      const int i = pending, b = i & 1, use = i >> 1, n = 2 * i + 1, s = n % SLOTS;
-      ok = ok && mbar_wait_warp(bar(C::B_P_FULL + b), use & 1, guard, 0xc10) &&
-           mbar_wait_warp(bar(C::B_FULL + s), (n / SLOTS) & 1, guard, 0xc11) &&
-           mbar_wait_warp(bar(C::B_O_EMPTY + b), (use & 1) ^ 1, guard, 0xc12);
-      pending = -1;
+    bool ok = true, pending = false;
+    int pages = 0, item = -1, slot = 0, phase = 0, v_slot = 0, v_phase = 0;
+    const auto second_product = [&]() {            // of page pages - 1; its V tile lies behind its K tile
+      const int i = pages - 1, b = i & 1, s = v_slot, f = v_phase;
+      ok = ok && mbar_wait_warp(bar(C::B_P_FULL + b), (i >> 1) & 1, guard, 0xc10) &&
+           mbar_wait_warp(bar(C::B_FULL + s), f, guard, 0xc11);
+      pending = false;
       if (!ok) return;
       tc_fence_after();
       if (elect_one()) {
-        const uint32_t v = base + C::OFF_RING + s * TILE_BYTES, pr = base + C::OFF_P + b * N * 128;
+        const uint32_t v = ((base + C::OFF_RING + s * TILE_BYTES) >> 4) | LO_MN128;
+        const uint32_t pr = ((base + C::OFF_P + b * N * 128) >> 4) | LO_MN32;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          mma_e4m3(tmem + 2 * N + b * N, desc_sw128_mnmajor(v + k * 4096, TILE_BYTES, 1024), desc_sw32_mnmajor(pr + k * 1024), ID_PV, k > 0);
+        for (int k = 0; k < 4; ++k) mma_e4m3<HI_MN32>(tmem + (2 + b) * N, v + k * 256, pr + k * 64, ID_PV, k > 0);
         tc_commit(bar(C::B_O_FULL + b));
         tc_commit(bar(C::B_EMPTY + s));
       }
       __syncwarp();
     };
-    // Waits for a barrier; issues the second product of the last page as soon as its probabilities are there.
-    const auto wait_for = [&](int which, uint32_t parity, int code) {
-      const long long t0 = clock64();
-      while (ok && pending >= 0 && !__all_sync(0xffffffffu, mbar_test_wait(bar(which), parity))) {
-        if (__all_sync(0xffffffffu, mbar_test_wait(bar(C::B_P_FULL + (pending & 1)), (pending >> 1) & 1))) second_product();
-        if (__any_sync(0xffffffffu, clock64() - t0 > WAIT_LIMIT_CYCLES || *guard.abort_flag)) break;   // the wait below settles it
-      }
-      ok = ok && mbar_wait_warp(bar(which), parity, guard, code);
-    };
     while (ok) {
-      const int e = entries % INFO;
-      wait_for(C::B_INFO_FULL + e, (entries / INFO) & 1, 0xc13);
-      if (!ok) break;
-      const int type = *reinterpret_cast<volatile int*>(gbase + C::OFF_INFO + 32 * e);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(C::B_INFO_EMPTY + e));
-      ++entries;
-      if (type == STOP) break;
-      if (type == START) {
-        new_item = true;
-      } else if (type == END) {
-        if (new_item) wait_for(C::B_Q_FULL + (items & 1), (items >> 1) & 1, 0xc14);   // an item without pages
-        if (ok && elect_one()) tc_commit(bar(C::B_Q_EMPTY + (items & 1)));
-        __syncwarp();
-        ++items;
-      } else {
-        const int b = pages & 1, n = 2 * pages, s = n % SLOTS;
-        if (new_item) wait_for(C::B_Q_FULL + (items & 1), (items >> 1) & 1, 0xc15);
-        new_item = false;
-        wait_for(C::B_FULL + s, (n / SLOTS) & 1, 0xc16);
-        wait_for(C::B_S_EMPTY + b, ((pages >> 1) & 1) ^ 1, 0xc17);
-        if (!ok) break;
-        tc_fence_after();
-        if (elect_one()) {
-          const uint32_t kt = base + C::OFF_RING + s * TILE_BYTES, qt = base + C::OFF_Q + (items & 1) * N * 128;
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mma_e4m3(tmem + b * N, desc_sw128_kmajor(kt + k * 32), desc_sw128_kmajor(qt + k * 32), ID_QK, k > 0);
-          tc_commit(bar(C::B_S_FULL + b));
-          tc_commit(bar(C::B_EMPTY + s));
+      // The second product of the last page goes ahead where its probabilities are there before the next K tile.
+      if (pending) {
+        const long long t0 = clock64();
+        while (pending && !__all_sync(0xffffffffu, mbar_test_wait(bar(C::B_FULL + slot), phase))) {
+          if (__all_sync(0xffffffffu, mbar_test_wait(bar(C::B_P_FULL + ((pages - 1) & 1)), ((pages - 1) >> 1) & 1))) second_product();
+          if (__any_sync(0xffffffffu, clock64() - t0 > WAIT_LIMIT_CYCLES || *guard.abort_flag)) break;   // settled below
         }
-        __syncwarp();
-        if (pending >= 0) second_product();
-        pending = pages++;
       }
+      ok = ok && mbar_wait_warp(bar(C::B_FULL + slot), phase, guard, 0xc12);
+      if (!ok) break;
+      const int flag = *reinterpret_cast<volatile int*>(gbase + C::OFF_FLAG + 4 * slot);
+      if (flag < 0) break;
+      if (flag != item) {
+        item = flag;
+        ok = mbar_wait_warp(bar(C::B_Q_FULL + (item & 1)), (item >> 1) & 1, guard, 0xc13);
+        if (!ok) break;
+      }
+      tc_fence_after();
+      if (elect_one()) {
+        const uint32_t kt = (base + C::OFF_RING + slot * TILE_BYTES) >> 4, qt = (base + C::OFF_Q + (item & 1) * N * 128) >> 4;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mma_e4m3<HI_128>(tmem + (pages & 1) * N, kt + k * 2, qt + k * 2, ID_QK, k > 0);
+        tc_commit(bar(C::B_S_FULL + (pages & 1)));
+        tc_commit(bar(C::B_EMPTY + slot));
+      }
+      __syncwarp();
+      if (pending) second_product();
+      v_slot = slot + 1;
+      v_phase = phase;
+      if (v_slot == SLOTS) {
+        v_slot = 0;
+        v_phase ^= 1;
+      }
+      slot = v_slot + 1;
+      phase = v_phase;
+      if (slot == SLOTS) {
+        slot = 0;
+        phase ^= 1;
+      }
+      pending = true;
+      ++pages;
     }
-    if (ok && pending >= 0) second_product();
+    if (ok && pending) second_product();
     // nothing of the tensor core's is in flight when the CTA gives up its memory
     if (elect_one()) tc_commit(bar(C::B_DONE));
     __syncwarp();
@@ -490,13 +523,15 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
     // --------------------------------------------------------------- softmax: lane = key, then lane = feature
     const int wg = warp >> 2, quarter = warp & 3, key = quarter * 32 + lane, row0 = wg * 16, r16 = lane & 15;
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-    float4* factors = reinterpret_cast<float4*>(gbase + C::OFF_FACTOR) + warp * 16;
-    float2* outs = reinterpret_cast<float2*>(gbase + C::OFF_OUT) + warp * 16;           // + parity * SOFTMAX_WARPS * 16
+    // of the warp's 16 rows: score factor, exponent offset, weight of the page's sum; and, for each of two pages, what the
+    // sums so far and the page's output are multiplied by
+    float* factors = reinterpret_cast<float*>(gbase + C::OFF_FACTOR) + warp * 48;
+    float* outs = reinterpret_cast<float*>(gbase + C::OFF_OUT) + warp * 32;             // + parity * SOFTMAX_WARPS * 32
     float* maxima = reinterpret_cast<float*>(gbase + C::OFF_MAX) + wg * 64;             // [4][16]
     float* sums = reinterpret_cast<float*>(gbase + C::OFF_SUM) + wg * 64;
     const float* qf = reinterpret_cast<const float*>(gbase + C::OFF_QF);
     float acc[16], l[16], m = -INFINITY, scale_row = 0.f;
-    int entries = 0, items = 0, pages = 0, pending = -1, masked = 0;
+    int entries = 0, items = 0, ends = 0, pages = 0, pending = -1, masked = 0;
     int token0 = 0, tokens = 0, head = 0, place = -1, x0 = 0, x1 = 0;
     // of the pending page, for rows that do not see all of its keys
     int p_row = 0, p_limit = 0, p_valid = 0;
@@ -517,12 +552,15 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
       tmem_ld16(tmem + lane_base + 2 * N + b * N + R + row0, w);
       tc_wait_ld();
       tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(C::B_O_EMPTY + b));
-      const float2* f = outs + (i & 1) * C::SOFTMAX_WARPS * 16;
+      const float* f = outs + b * C::SOFTMAX_WARPS * 32;
       float o[16];
 #pragma unroll
-      for (int j = 0; j < 16; ++j) o[j] = fmaf(__uint_as_float(w[j]), 0.0625f, __uint_as_float(h[j]));
+      for (int j = 0; j < 16; j += 2) {
+        const float2 x = fma2(make_float2(__uint_as_float(w[j]), __uint_as_float(w[j + 1])), make_float2(0.0625f, 0.0625f),
+                              make_float2(__uint_as_float(h[j]), __uint_as_float(h[j + 1])));
+        o[j] = x.x;
+        o[j + 1] = x.y;
+      }
       if (masked) {
         // A key that is hidden from a row has probability 0 there, and 0 times a NaN of its value is not 0: such a sum is
         // done again over the keys that the row sees, from the probabilities in shared memory.
@@ -546,9 +584,16 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
         }
       }
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float2 c = f[j];
-        acc[j] = fmaf(acc[j], c.x, o[j] * c.y);
+      for (int j = 0; j < 16; j += 4) {
+        const float4 c1 = *reinterpret_cast<const float4*>(f + j), c2 = *reinterpret_cast<const float4*>(f + 16 + j);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int r = j + 2 * i;
+          const float2 x = mul2(make_float2(o[r], o[r + 1]), i ? make_float2(c2.z, c2.w) : make_float2(c2.x, c2.y));
+          const float2 y = fma2(make_float2(acc[r], acc[r + 1]), i ? make_float2(c1.z, c1.w) : make_float2(c1.x, c1.y), x);
+          acc[r] = y.x;
+          acc[r + 1] = y.y;
+        }
       }
     };
 
@@ -562,7 +607,7 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
       if (lane == 0) mbar_arrive(bar(C::B_INFO_EMPTY + e));
       ++entries;
       if (x.x == STOP) break;
-      if (x.x == START) {
+      if (x.x == START || x.x == EMPTY) {
         token0 = x.y;
         tokens = x.z;
         head = x.w;
@@ -573,8 +618,8 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[i] = l[i] = 0.f;
         fresh = true;
-        continue;
       }
+      if (x.x == START) continue;
       if (x.x == PAGE) {
         const int b = pages & 1, row = x.y, valid = x.z, limit = x.w;
         const float ks = __int_as_float(y.x), vs = __int_as_float(y.y);
@@ -592,12 +637,15 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
         tmem_ld16(tmem + lane_base + b * N + R + row0, w);
         tc_wait_ld();
         tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(C::B_S_EMPTY + b));
         float s[16];
         const bool partial = valid < 128 || limit < 128;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) s[j] = fmaf(__uint_as_float(w[j]), 0.0625f, __uint_as_float(h[j]));
+        for (int j = 0; j < 16; j += 2) {
+          const float2 x = fma2(make_float2(__uint_as_float(w[j]), __uint_as_float(w[j + 1])), make_float2(0.0625f, 0.0625f),
+                                make_float2(__uint_as_float(h[j]), __uint_as_float(h[j + 1])));
+          s[j] = x.x;
+          s[j + 1] = x.y;
+        }
         uint32_t hidden = 0;                       // rows that do not see this key
         if (partial) {
 #pragma unroll
@@ -609,12 +657,7 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
             }
           }
         }
-        float top = 0.f;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float t = warp_max(s[j]);
-          top = r16 == j ? t : top;
-        }
+        float top = row_maxima(s, lane);
         float* mx = maxima + b * C::SOFTMAX_WARPS * 16;
         if (lane < 16) mx[quarter * 16 + lane] = top;
         __syncwarp();
@@ -631,27 +674,44 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
           const float c2 = none ? 0.f : ex2_approx(mu - next);
           m = next;
           if (lane < 16) {
-            factors[lane] = make_float4(f, none ? 0.f : 8.f - mu, c1, c2);
-            outs[(pages & 1) * C::SOFTMAX_WARPS * 16 + lane] = make_float2(c1, c2 * vs * 0.00390625f);
+            factors[lane] = f;
+            factors[16 + lane] = none ? 0.f : 8.f - mu;
+            factors[32 + lane] = c2;
+            float* out = outs + b * C::SOFTMAX_WARPS * 32;
+            out[lane] = c1;
+            out[16 + lane] = c2 * vs * 0.00390625f;
           }
         }
         __syncwarp();
         uint32_t ph[4], pl[4];
 #pragma unroll
         for (int j4 = 0; j4 < 4; ++j4) {
-          float pr[4], cut[4];
+          const float4 f4 = *reinterpret_cast<const float4*>(factors + 4 * j4);
+          const float4 b4 = *reinterpret_cast<const float4*>(factors + 16 + 4 * j4);
+          const float4 w4 = *reinterpret_cast<const float4*>(factors + 32 + 4 * j4);
+          const float4 k4 = *reinterpret_cast<const float4*>(outs + b * C::SOFTMAX_WARPS * 32 + 4 * j4);
+          ph[j4] = pl[j4] = 0;
 #pragma unroll
-          for (int jj = 0; jj < 4; ++jj) {
-            const int j = 4 * j4 + jj;
-            const float4 f = factors[j];
-            float v = ex2_approx(fmaf(s[j], f.x, f.y));
-            if (partial && (hidden >> j & 1)) v = 0.f;
-            l[j] = fmaf(l[j], f.z, v * f.w);
-            cut[jj] = __uint_as_float(__float_as_uint(v) & 0xfff00000u);     // four significant bits
-            pr[jj] = (v - cut[jj]) * 16.f;
+          for (int i = 0; i < 2; ++i) {
+            const int j = 4 * j4 + 2 * i;
+            float2 v = fma2(make_float2(s[j], s[j + 1]), i ? make_float2(f4.z, f4.w) : make_float2(f4.x, f4.y),
+                            i ? make_float2(b4.z, b4.w) : make_float2(b4.x, b4.y));
+            v.x = ex2_approx(v.x);
+            v.y = ex2_approx(v.y);
+            if (partial) {
+              if (hidden >> j & 1) v.x = 0.f;
+              if (hidden >> (j + 1) & 1) v.y = 0.f;
+            }
+            const float2 n = fma2(make_float2(l[j], l[j + 1]), i ? make_float2(k4.z, k4.w) : make_float2(k4.x, k4.y),
+                                  mul2(v, i ? make_float2(w4.z, w4.w) : make_float2(w4.x, w4.y)));
+            l[j] = n.x;
+            l[j + 1] = n.y;
+            const float2 cut = make_float2(__uint_as_float(__float_as_uint(v.x) & 0xfff00000u),     // four significant bits
+                                           __uint_as_float(__float_as_uint(v.y) & 0xfff00000u));
+            const float2 rest = fma2(v, make_float2(16.f, 16.f), mul2(cut, make_float2(-16.f, -16.f)));
+            ph[j4] |= e4m3x2(cut.x, cut.y) << (16 * i);
+            pl[j4] |= e4m3x2(rest.x, rest.y) << (16 * i);
           }
-          ph[j4] = e4m3x2(cut[0], cut[1]) | (e4m3x2(cut[2], cut[3]) << 16);
-          pl[j4] = e4m3x2(pr[0], pr[1]) | (e4m3x2(pr[2], pr[3]) << 16);
         }
         unsigned char* to = gbase + C::OFF_P + b * N * 128 + key * 32;
         const auto column = [&](int c) { return to + (c >> 5) * 4096 + ((((c >> 4) ^ (key >> 2)) & 1) << 4); };
@@ -679,17 +739,15 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
         p_valid = valid;
         continue;
       }
-      // END
+      // END or EMPTY
       if (pending >= 0) add_output();
       if (!ok) break;
-      if (fresh) {                                 // an item without pages
-        ok = mbar_wait_warp(bar(C::B_Q_FULL + (items & 1)), (items >> 1) & 1, guard, 0xc35);
-        if (!ok) break;
-        fresh = false;
+      if (x.x == END) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::B_Q_EMPTY + (items & 1)));
+        ++items;
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(C::B_Q_EMPTY + (items & 1)));
-      float* sm = sums + (items & 1) * C::SOFTMAX_WARPS * 16;
+      float* sm = sums + (ends & 1) * C::SOFTMAX_WARPS * 16;
       float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
@@ -700,8 +758,9 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
       }
       if (lane < 16) sm[quarter * 16 + lane] = sum;
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(C::B_SUM + 2 * wg + (items & 1)));
-      ok = mbar_wait_warp(bar(C::B_SUM + 2 * wg + (items & 1)), (items >> 1) & 1, guard, 0xc37);
+      if (lane == 0) mbar_arrive(bar(C::B_SUM + 2 * wg + (ends & 1)));
+      ok = mbar_wait_warp(bar(C::B_SUM + 2 * wg + (ends & 1)), (ends >> 1) & 1, guard, 0xc35);
+      ++ends;
       if (!ok) break;
       const int rows = tokens * p.group;
       if (place < 0) {
@@ -739,7 +798,6 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
           meta[0] = 1;
         }
       }
-      ++items;
     }
   }
   tc_fence_before();
