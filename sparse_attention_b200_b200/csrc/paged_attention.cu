@@ -40,7 +40,7 @@ constexpr int MIN_SHARE = 4;                      // pages of a CTA at least
 
 struct Params {
   PagedAttentionArgs a;
-  int group, pack, ctas;
+  int group, pack, pack_shift, tile_shift, ctas;
   float* part_o;                                  // [2 ctas, R, 128]
   float* part_ml;                                 // [2 ctas, R, 2]
   int* part_meta;                                 // [2 ctas, 8]
@@ -62,7 +62,9 @@ struct Config {
   static constexpr int OFF_MAX = OFF_OUT + 2 * SOFTMAX_WARPS * 128; // float [2][softmax warp][16]
   static constexpr int OFF_SUM = OFF_MAX + 2 * SOFTMAX_WARPS * 64;  // float [2][softmax warp][16]
   static constexpr int OFF_QF = OFF_SUM + 2 * SOFTMAX_WARPS * 64;   // float [2][R]: what a row's scores are multiplied by
-  static constexpr int OFF_INFO = OFF_QF + 2 * R * 4;               // int [INFO][8]
+  static constexpr int OFF_ROW = OFF_QF + 2 * R * 4;                // int [R]: token << 16 | head of a row
+  static constexpr int OFF_ROW_OUT = OFF_ROW + R * 4;               // int [R]: offset of a row in the output, from the item's first
+  static constexpr int OFF_INFO = OFF_ROW_OUT + R * 4;                  // int [INFO][8]
   static constexpr int OFF_BAR = OFF_INFO + INFO * 32;
   static constexpr int B_INFO_FULL = 0, B_INFO_EMPTY = INFO, B_FULL = 2 * INFO, B_EMPTY = B_FULL + SLOTS;
   static constexpr int B_S_FULL = B_EMPTY + SLOTS, B_P_FULL = B_S_FULL + 2, B_O_FULL = B_P_FULL + 2, B_Q_FULL = B_O_FULL + 2,
@@ -107,25 +109,84 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   f32x2_unpack(f32x2_mul(f32x2_pack(a.x, a.y), f32x2_pack(b.x, b.y)), d.x, d.y);
   return d;
 }
-// Maxima over the warp of 16 values: lane l gets that of value l % 16. Every step halves the values that a lane holds.
-__device__ __forceinline__ float row_maxima(const float (&s)[16], int lane) {
+// A sum or maximum over the warp for each of 16 values: lane l gets that of value l % 16. Every step halves the values that a
+// lane holds: 16 shuffles in all. (redux.sync on fp32 took 40 cycles a value.)
+template <typename F>
+__device__ __forceinline__ float halved(const float (&s)[16], int lane, F op) {
   float a[8], b[4], c[2];
   const bool h8 = lane & 8, h4 = lane & 4, h2 = lane & 2, h1 = lane & 1;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) a[j] = fmaxf(h8 ? s[j + 8] : s[j], __shfl_xor_sync(0xffffffffu, h8 ? s[j] : s[j + 8], 8));
+  for (int j = 0; j < 8; ++j) a[j] = op(h8 ? s[j + 8] : s[j], __shfl_xor_sync(0xffffffffu, h8 ? s[j] : s[j + 8], 8));
 #pragma unroll
-  for (int j = 0; j < 4; ++j) b[j] = fmaxf(h4 ? a[j + 4] : a[j], __shfl_xor_sync(0xffffffffu, h4 ? a[j] : a[j + 4], 4));
+  for (int j = 0; j < 4; ++j) b[j] = op(h4 ? a[j + 4] : a[j], __shfl_xor_sync(0xffffffffu, h4 ? a[j] : a[j + 4], 4));
 #pragma unroll
-  for (int j = 0; j < 2; ++j) c[j] = fmaxf(h2 ? b[j + 2] : b[j], __shfl_xor_sync(0xffffffffu, h2 ? b[j] : b[j + 2], 2));
-  const float d = fmaxf(h1 ? c[1] : c[0], __shfl_xor_sync(0xffffffffu, h1 ? c[0] : c[1], 1));
-  return fmaxf(d, __shfl_xor_sync(0xffffffffu, d, 16));
+  for (int j = 0; j < 2; ++j) c[j] = op(h2 ? b[j + 2] : b[j], __shfl_xor_sync(0xffffffffu, h2 ? b[j] : b[j + 2], 2));
+  const float d = op(h1 ? c[1] : c[0], __shfl_xor_sync(0xffffffffu, h1 ? c[0] : c[1], 1));
+  return op(d, __shfl_xor_sync(0xffffffffu, d, 16));
+}
+// A wait by a whole converged warp whose slow part is not in line: a role's loop has to fit the instruction caches beside the
+// others' (the first build of this kernel had 164 KB of code and ran at a fifth of its speed).
+__device__ __noinline__ bool wait_longer(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  return mbar_wait_warp(bar, parity, Guard{abort_flag, status}, code);
+}
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, const Guard& g, int code) {
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+  return wait_longer(bar, parity, g.abort_flag, g.status, code);
+}
+__device__ __noinline__ bool post_entry(uint32_t full, uint32_t empty, uint32_t parity, unsigned char* to, int4 a, int4 b,
+                                        volatile int* abort_flag, int* status) {
+  if (!mbar_wait_warp(empty, parity, Guard{abort_flag, status}, 0xc00)) return false;
+  if ((threadIdx.x & 31) == 0) {
+    reinterpret_cast<int4*>(to)[0] = a;
+    reinterpret_cast<int4*>(to)[1] = b;
+    mbar_arrive(full);
+  }
+  __syncwarp();
+  return true;
+}
+__device__ __noinline__ bool load_tile(uint32_t full, uint32_t empty, uint32_t parity, uint32_t to, const CUtensorMap* map, int row,
+                                       volatile int* flag_at, int flag, volatile int* abort_flag, int* status) {
+  if (!mbar_wait_warp(empty, parity, Guard{abort_flag, status}, 0xc01)) return false;
+  if (elect_one()) {
+    *flag_at = flag;
+    if (flag < 0) {
+      mbar_arrive(full);
+    } else {
+      mbar_expect_tx(full, TILE_BYTES);
+      tma_load_2d(to, map, 0, row, full);
+    }
+  }
+  __syncwarp();
+  return true;
 }
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
+__device__ __forceinline__ float2 from_e4m3x2(uint32_t codes) {
+  return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(codes), __NV_E4M3)));
+}
 __device__ __forceinline__ float from_e4m3(uint32_t code) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(code), __NV_E4M3)));
+}
+
+// o[j] where it is NaN: the sum of p v over the keys of a page that row row0 + j sees, from the probabilities in shared memory
+// and a feature's codes
+template <int R>
+__device__ __noinline__ void visible_sums(float* o, const unsigned char* pr, const uint8_t* v, const int* row_of, int row0, int limit,
+                                          int valid) {
+#pragma unroll 1
+  for (int j = 0; j < 16; ++j) {
+    if (o[j] == o[j]) continue;
+    const int row = row0 + j, end = min(limit + (row_of[row] >> 16), valid);
+    float x = 0.f;
+#pragma unroll 1
+    for (int n = 0; n < end; ++n) {
+      const auto at = [&](int c) { return from_e4m3(pr[(c >> 5) * 4096 + n * 32 + ((((c >> 4) ^ (n >> 2)) & 1) << 4) + (c & 15)]); };
+      x = fmaf(fmaf(at(R + row), 0.0625f, at(row)), from_e4m3(__ldg(v + n * 128)), x);
+    }
+    o[j] = x;
+  }
 }
 
 // ------------------------------------------------------------------ the work of a request
@@ -136,18 +197,18 @@ struct Request {
     n = max(min(max(cu1, 0), p.a.total_q) - begin, 0);
     k_len = max(seq, 0);
     held = min((k_len >> 7) + ((k_len & 127) != 0), p.a.width);
-    tiles = (n + p.pack - 1) / p.pack;
+    tiles = static_cast<int>((static_cast<long long>(n) + p.pack - 1) >> p.pack_shift);
   }
 };
 // Pages of the first `tiles` tiles of a request: a list's length each, or the pages that a tile's last token sees (one at
 // least, so that every item has a place): min(held, ceil((k - n + (i + 1) pack) / 128)) summed over i. With pack = 128 / m the
 // ceiling is floor((first + i) / m), whose sums have a closed form.
-__device__ __forceinline__ long long pages_before(const Params& p, const Request& r, int tiles) {
-  if (p.a.ids) return static_cast<long long>(tiles) * p.a.topk;
-  const long long most = max(r.held, 1);
-  if (!p.a.causal) return tiles * most;
-  const int m = 128 / p.pack, shift = 31 - __clz(p.pack), mshift = 7 - shift;
-  const long long first = ((static_cast<long long>(r.k_len) - r.n + 127) >> shift) + 1;
+__device__ __noinline__ long long pages_before(int topk, int causal, int shift, int k_len, int n, int held, int tiles) {
+  if (topk) return static_cast<long long>(tiles) * topk;
+  const long long most = max(held, 1);
+  if (!causal) return tiles * most;
+  const int mshift = 7 - shift, m = 1 << mshift;
+  const long long first = ((static_cast<long long>(k_len) - n + 127) >> shift) + 1;
   const auto clamp = [&](long long x) { return x < 0 ? 0 : x > tiles ? tiles : x; };
   const long long ones = clamp(m - first), full = max(clamp(most * m - first), ones);
   const auto sum = [&](long long x) {             // sum of floor(t / m) over 0 <= t < x
@@ -156,6 +217,14 @@ __device__ __forceinline__ long long pages_before(const Params& p, const Request
   };
   const long long middle = full > ones ? sum(first + full) - sum(first + ones) : 0;
   return ones + middle + (tiles - full) * most;
+}
+__device__ __forceinline__ long long pages_before(const Params& p, const Request& r, int tiles) {
+  return pages_before(p.a.topk, p.a.causal, p.pack_shift, r.k_len, r.n, r.held, tiles);
+}
+__device__ __forceinline__ long long pages_of_request(const Params& p, int r) {
+  Request q;
+  q.set(p, __ldg(p.a.cu_q + r), __ldg(p.a.cu_q + r + 1), __ldg(p.a.seq + r));
+  return pages_before(p, q, q.tiles);
 }
 
 // ------------------------------------------------------------------ kernel
@@ -198,6 +267,13 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
     p.part_meta[16 * blockIdx.x] = 0;             // no part yet in either of this CTA's places
     p.part_meta[16 * blockIdx.x + 8] = 0;
   }
+  int* row_of = reinterpret_cast<int*>(gbase + C::OFF_ROW);
+  int* row_out = reinterpret_cast<int*>(gbase + C::OFF_ROW_OUT);
+  if (tid < R) {
+    const int token = tid / p.group, g = tid - token * p.group;
+    row_of[tid] = token << 16 | g;
+    row_out[tid] = (token * p.a.hq + g) * 128;
+  }
   if (warp == C::MMA) {
     tmem_alloc(smem_u32(const_cast<int*>(misc)), C::TMEM);
     tmem_relinquish();
@@ -210,11 +286,8 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
   const int each = (p.a.batch + C::THREADS - 1) / C::THREADS;
   const int lo = min(tid * each, p.a.batch), hi = min(lo + each, p.a.batch);
   long long mine = 0;
-  for (int r = lo; r < hi; ++r) {
-    Request q;
-    q.set(p, __ldg(p.a.cu_q + r), __ldg(p.a.cu_q + r + 1), __ldg(p.a.seq + r));
-    mine += pages_before(p, q, q.tiles);
-  }
+#pragma unroll 1
+  for (int r = lo; r < hi; ++r) mine += pages_of_request(p, r);
   long long upto = mine;
   for (int by = 1; by < 32; by <<= 1) {
     const long long x = __shfl_up_sync(0xffffffffu, upto, by);
@@ -237,10 +310,9 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
   if (unit0 < total) {
     long long at = unit0 - head0 * per_head - upto;
     if (at >= 0 && at < mine) {
+#pragma unroll 1
       for (int r = lo; r < hi; ++r) {
-        Request q;
-        q.set(p, __ldg(p.a.cu_q + r), __ldg(p.a.cu_q + r + 1), __ldg(p.a.seq + r));
-        const long long w = pages_before(p, q, q.tiles);
+        const long long w = pages_of_request(p, r);
         if (at < w) {
           s_place[0] = at;
           s_place[1] = r;
@@ -256,35 +328,20 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
 
   if (warp == C::LOADER) {
     // --------------------------------------------------------------- loader
-    int entries = 0, items = -1, slot = 0, phase = 0;
+    uint32_t entries = 0;
+    int items = -1, slot = 0, phase = 0;
     bool ok = true;
     const auto post = [&](int type, int x0, int x1, int x2, int x3, int x4, int x5) {
-      const int e = entries % INFO;
-      ok = ok && mbar_wait_warp(bar(C::B_INFO_EMPTY + e), ((entries / INFO) & 1) ^ 1, guard, 0xc00);
-      if (!ok) return;
-      if (lane == 0) {
-        int4* to = reinterpret_cast<int4*>(gbase + C::OFF_INFO + 32 * e);
-        to[0] = make_int4(type, x0, x1, x2);
-        to[1] = make_int4(x3, x4, x5, 0);
-        mbar_arrive(bar(C::B_INFO_FULL + e));
-      }
+      const uint32_t e = entries % INFO;
+      if (ok) ok = post_entry(bar(C::B_INFO_FULL + e), bar(C::B_INFO_EMPTY + e), ((entries / INFO) & 1) ^ 1, gbase + C::OFF_INFO + 32 * e,
+                              make_int4(type, x0, x1, x2), make_int4(x3, x4, x5, 0), guard.abort_flag, status);
       ++entries;
     };
     // flag: what the MMA warp has to know of a K tile: the number of its item, -1 = there are no more tiles
     const auto load = [&](const CUtensorMap* map, int row, int flag) {
-      ok = ok && mbar_wait_warp(bar(C::B_EMPTY + slot), phase ^ 1, guard, 0xc01);
-      if (!ok) return;
-      if (elect_one()) {
-        *reinterpret_cast<volatile int*>(gbase + C::OFF_FLAG + 4 * slot) = flag;
-        if (flag < 0) {
-          mbar_arrive(bar(C::B_FULL + slot));
-        } else {
-          mbar_expect_tx(bar(C::B_FULL + slot), TILE_BYTES);
-          tma_load_2d(base + C::OFF_RING + slot * TILE_BYTES, map, 0, row, bar(C::B_FULL + slot));
-        }
-      }
-      __syncwarp();
-      ++fills;
+      if (ok) ok = load_tile(bar(C::B_FULL + slot), bar(C::B_EMPTY + slot), phase ^ 1, base + C::OFF_RING + slot * TILE_BYTES, map, row,
+                             reinterpret_cast<volatile int*>(gbase + C::OFF_FLAG + 4 * slot), flag, guard.abort_flag, status);
+      fills += ok;
       if (++slot == SLOTS) {
         slot = 0;
         phase ^= 1;
@@ -324,10 +381,12 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
         bool started = false;
         const int32_t* list = nullptr;
         if (p.a.ids) {
-          const long long lists = p.a.tile == 1 ? p.a.total_q : p.a.total_q / p.a.tile + p.a.batch;
-          list = p.a.ids + (head * lists + first_list_row(q.begin, r, p.a.tile) + token0 / p.a.tile) * p.a.topk;
+          const int s = p.tile_shift;
+          const long long lists = s ? (p.a.total_q >> s) + p.a.batch : p.a.total_q;
+          list = p.a.ids + (head * lists + (q.begin >> s) + (s ? r : 0) + (token0 >> s)) * p.a.topk;
         }
         const int32_t* table = p.a.table + r * p.a.table_stride;
+#pragma unroll 1
         for (int at = from; ok && at < to; at += 32) {
           int j = at + lane;
           bool live = j < to;
@@ -345,6 +404,7 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
             }
           }
           uint32_t todo = __ballot_sync(0xffffffffu, live);
+#pragma unroll 1
           while (ok && todo) {
             const int l = __ffs(todo) - 1;
             todo &= todo - 1;
@@ -389,69 +449,70 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
     // next needs no barrier: the softmax warps store the probabilities of a page after they have read its S and the O of the
     // page before the last.
     constexpr uint32_t ID_QK = idesc_e4m3(N, false), ID_PV = idesc_e4m3(N, true);
-    bool ok = true, pending = false;
-    int pages = 0, item = -1, slot = 0, phase = 0, v_slot = 0, v_phase = 0;
-    const auto second_product = [&]() {            // of page pages - 1; its V tile lies behind its K tile
-      const int i = pages - 1, b = i & 1, s = v_slot, f = v_phase;
-      ok = ok && mbar_wait_warp(bar(C::B_P_FULL + b), (i >> 1) & 1, guard, 0xc10) &&
-           mbar_wait_warp(bar(C::B_FULL + s), f, guard, 0xc11);
-      pending = false;
-      if (!ok) return;
+    bool ok = true, stopped = false;
+    int first = 0, second = 0, item = -1;          // pages whose first / second product has been issued
+    int slot = 0, phase = 0, v_slot = 1, v_phase = 0;
+    const auto next_page = [&](int& s, int& f) {   // two tiles on
+      s += 2;
+      if (s >= SLOTS) {
+        s -= SLOTS;
+        f ^= 1;
+      }
+    };
+    long long t0 = clock64();
+    while (ok) {
+      // One page ahead of the second products; where its K tile is not there yet and the probabilities of the page before
+      // are, these go first.
+      if (!stopped && first - second < 2 &&
+          (first == second ? ok = wait_warp(bar(C::B_FULL + slot), phase, guard, 0xc10)
+                           : __all_sync(0xffffffffu, mbar_test_wait(bar(C::B_FULL + slot), phase)))) {
+        const int flag = *reinterpret_cast<volatile int*>(gbase + C::OFF_FLAG + 4 * slot);
+        stopped = flag < 0;
+        if (!stopped) {
+          if (flag != item) {
+            item = flag;
+            ok = wait_warp(bar(C::B_Q_FULL + (item & 1)), (item >> 1) & 1, guard, 0xc11);
+            if (!ok) break;
+          }
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t kt = (base + C::OFF_RING + slot * TILE_BYTES) >> 4, qt = (base + C::OFF_Q + (item & 1) * N * 128) >> 4;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mma_e4m3<HI_128>(tmem + (first & 1) * N, kt + k * 2, qt + k * 2, ID_QK, k > 0);
+            tc_commit(bar(C::B_S_FULL + (first & 1)));
+            tc_commit(bar(C::B_EMPTY + slot));
+          }
+          __syncwarp();
+          next_page(slot, phase);
+          ++first;
+          t0 = clock64();
+        }
+      }
+      if (!ok || first == second) {
+        if (stopped || !ok) break;
+        continue;
+      }
+      const int b = second & 1;
+      if (!stopped && first - second < 2 && !__all_sync(0xffffffffu, mbar_test_wait(bar(C::B_P_FULL + b), (second >> 1) & 1))) {
+        const bool late = clock64() - t0 > WAIT_LIMIT_CYCLES || *guard.abort_flag;
+        if (!__any_sync(0xffffffffu, late)) continue;
+      }
+      ok = wait_warp(bar(C::B_P_FULL + b), (second >> 1) & 1, guard, 0xc12) && wait_warp(bar(C::B_FULL + v_slot), v_phase, guard, 0xc13);
+      if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
-        const uint32_t v = ((base + C::OFF_RING + s * TILE_BYTES) >> 4) | LO_MN128;
+        const uint32_t v = ((base + C::OFF_RING + v_slot * TILE_BYTES) >> 4) | LO_MN128;
         const uint32_t pr = ((base + C::OFF_P + b * N * 128) >> 4) | LO_MN32;
 #pragma unroll
         for (int k = 0; k < 4; ++k) mma_e4m3<HI_MN32>(tmem + (2 + b) * N, v + k * 256, pr + k * 64, ID_PV, k > 0);
         tc_commit(bar(C::B_O_FULL + b));
-        tc_commit(bar(C::B_EMPTY + s));
+        tc_commit(bar(C::B_EMPTY + v_slot));
       }
       __syncwarp();
-    };
-    while (ok) {
-      // The second product of the last page goes ahead where its probabilities are there before the next K tile.
-      if (pending) {
-        const long long t0 = clock64();
-        while (pending && !__all_sync(0xffffffffu, mbar_test_wait(bar(C::B_FULL + slot), phase))) {
-          if (__all_sync(0xffffffffu, mbar_test_wait(bar(C::B_P_FULL + ((pages - 1) & 1)), ((pages - 1) >> 1) & 1))) second_product();
-          if (__any_sync(0xffffffffu, clock64() - t0 > WAIT_LIMIT_CYCLES || *guard.abort_flag)) break;   // settled below
-        }
-      }
-      ok = ok && mbar_wait_warp(bar(C::B_FULL + slot), phase, guard, 0xc12);
-      if (!ok) break;
-      const int flag = *reinterpret_cast<volatile int*>(gbase + C::OFF_FLAG + 4 * slot);
-      if (flag < 0) break;
-      if (flag != item) {
-        item = flag;
-        ok = mbar_wait_warp(bar(C::B_Q_FULL + (item & 1)), (item >> 1) & 1, guard, 0xc13);
-        if (!ok) break;
-      }
-      tc_fence_after();
-      if (elect_one()) {
-        const uint32_t kt = (base + C::OFF_RING + slot * TILE_BYTES) >> 4, qt = (base + C::OFF_Q + (item & 1) * N * 128) >> 4;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) mma_e4m3<HI_128>(tmem + (pages & 1) * N, kt + k * 2, qt + k * 2, ID_QK, k > 0);
-        tc_commit(bar(C::B_S_FULL + (pages & 1)));
-        tc_commit(bar(C::B_EMPTY + slot));
-      }
-      __syncwarp();
-      if (pending) second_product();
-      v_slot = slot + 1;
-      v_phase = phase;
-      if (v_slot == SLOTS) {
-        v_slot = 0;
-        v_phase ^= 1;
-      }
-      slot = v_slot + 1;
-      phase = v_phase;
-      if (slot == SLOTS) {
-        slot = 0;
-        phase ^= 1;
-      }
-      pending = true;
-      ++pages;
+      next_page(v_slot, v_phase);
+      ++second;
+      t0 = clock64();
     }
-    if (ok && pending) second_product();
     // nothing of the tensor core's is in flight when the CTA gives up its memory
     if (elect_one()) tc_commit(bar(C::B_DONE));
     __syncwarp();
@@ -460,11 +521,12 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
     // --------------------------------------------------------------- queries of the next item
     const int half = warp - C::QWARP;
     bool ok = true;
-    int entries = 0, items = 0;
+    uint32_t entries = 0;
+    int items = 0;
     const float sign = p.a.scale < 0.f ? -1.f : 1.f, factor = fabsf(p.a.scale) * 1.4426950408889634f;
     while (ok) {
-      const int e = entries % INFO;
-      ok = mbar_wait_warp(bar(C::B_INFO_FULL + e), (entries / INFO) & 1, guard, 0xc20);
+      const uint32_t e = entries % INFO;
+      ok = wait_warp(bar(C::B_INFO_FULL + e), (entries / INFO) & 1, guard, 0xc20);
       if (!ok) break;
       const int4 x = *reinterpret_cast<const int4*>(gbase + C::OFF_INFO + 32 * e);
       __syncwarp();
@@ -473,37 +535,39 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
       if (x.x == STOP) break;
       if (x.x != START) continue;
       const int buf = items & 1;
-      ok = mbar_wait_warp(bar(C::B_Q_EMPTY + buf), ((items >> 1) & 1) ^ 1, guard, 0xc21);
+      ok = wait_warp(bar(C::B_Q_EMPTY + buf), ((items >> 1) & 1) ^ 1, guard, 0xc21);
       if (!ok) break;
       const int rows = x.z * p.group;              // tokens x heads of the KV head
       unsigned char* q8 = gbase + C::OFF_Q + buf * N * 128;
       float* qf = reinterpret_cast<float*>(gbase + C::OFF_QF) + buf * R;
       const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.a.q) + x.y * p.a.q_token +
                                  static_cast<long long>(x.w) * p.group * p.a.q_head + lane * 4;
-      for (int r0 = half * 8; r0 < R; r0 += 16) {
-        uint2 w[8];
+#pragma unroll 1
+      for (int r0 = half * (R / 2); r0 < (half + 1) * (R / 2); r0 += 4) {
+        uint2 w[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int row = r0 + i, t = row / p.group, g = row - t * p.group;
-          w[i] = row < rows ? __ldg(reinterpret_cast<const uint2*>(src + t * p.a.q_token + g * p.a.q_head)) : make_uint2(0, 0);
+        for (int i = 0; i < 4; ++i) {
+          const int at = row_of[r0 + i];
+          w[i] = r0 + i < rows ? __ldg(reinterpret_cast<const uint2*>(src + (at >> 16) * p.a.q_token + (at & 0xffff) * p.a.q_head))
+                               : make_uint2(0, 0);
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4; ++i) {
           const int row = r0 + i;
           const uint32_t m = __vmaxu2(w[i].x & 0x7fff7fffu, w[i].y & 0x7fff7fffu);
           const uint32_t top = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
           // times 2^e the largest feature lies in [128, 256); a row with infinities or NaN is taken as it is and ends as NaN
-          const int e = top == 0 || top >= 0x7f80u ? 0 : min(134 - static_cast<int>(top >> 7), 126);
+          const bool odd = top >= 0x7f80u;
+          const int e = top == 0 || odd ? 0 : min(134 - static_cast<int>(top >> 7), 126);
           const float by = power_of_two(e) * sign;
           const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i].x));
           const float2 c = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i].y));
           const float v[4] = {a.x * by, a.y * by, c.x * by, c.y * by};
-          uint32_t hi = e4m3x2(v[0], v[1]) | (e4m3x2(v[2], v[3]) << 16), rest = 0;
-          float low[4];
-#pragma unroll
-          for (int d = 0; d < 4; ++d) low[d] = (v[d] - from_e4m3(hi >> (8 * d) & 0xffu)) * 16.f;
-          rest = e4m3x2(low[0], low[1]) | (e4m3x2(low[2], low[3]) << 16);
-          if (top >= 0x7f80u) {
+          uint32_t hi = e4m3x2(v[0], v[1]) | (e4m3x2(v[2], v[3]) << 16);
+          const float2 h0 = from_e4m3x2(hi), h1 = from_e4m3x2(hi >> 16);
+          const uint32_t rest = e4m3x2((v[0] - h0.x) * 16.f, (v[1] - h0.y) * 16.f) |
+                                (e4m3x2((v[2] - h1.x) * 16.f, (v[3] - h1.y) * 16.f) << 16);
+          if (odd) {
 #pragma unroll
             for (int d = 0; d < 4; ++d)
               if (!(fabsf(v[d]) < INFINITY)) hi |= 0x7fu << (8 * d);
@@ -531,7 +595,8 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
     float* sums = reinterpret_cast<float*>(gbase + C::OFF_SUM) + wg * 64;
     const float* qf = reinterpret_cast<const float*>(gbase + C::OFF_QF);
     float acc[16], l[16], m = -INFINITY, scale_row = 0.f;
-    int entries = 0, items = 0, ends = 0, pages = 0, pending = -1, masked = 0;
+    uint32_t entries = 0;
+    int items = 0, ends = 0, pages = 0, pending = -1, masked = 0;
     int token0 = 0, tokens = 0, head = 0, place = -1, x0 = 0, x1 = 0;
     // of the pending page, for rows that do not see all of its keys
     int p_row = 0, p_limit = 0, p_valid = 0;
@@ -542,7 +607,7 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
     // adds the output of page `pending` to acc
     const auto add_output = [&]() {
       const int b = pending & 1;
-      ok = ok && mbar_wait_warp(bar(C::B_O_FULL + b), (pending >> 1) & 1, guard, 0xc30);
+      ok = ok && wait_warp(bar(C::B_O_FULL + b), (pending >> 1) & 1, guard, 0xc30);
       const int i = pending;
       pending = -1;
       if (!ok) return;
@@ -563,24 +628,19 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
       }
       if (masked) {
         // A key that is hidden from a row has probability 0 there, and 0 times a NaN of its value is not 0: such a sum is
-        // done again over the keys that the row sees, from the probabilities in shared memory.
-#pragma unroll 1
-        for (int j = 0; j < 16; ++j) {
-          float x = 0.f;
+        // done again over the keys that the row sees.
+        bool odd = false;
 #pragma unroll
-          for (int jj = 0; jj < 16; ++jj) x = jj == j ? o[jj] : x;
-          if (x == x) continue;
-          const int limit = min(p.a.causal ? p_limit + (row0 + j) / p.group : p_limit, p_valid);
-          const uint8_t* pr = gbase + C::OFF_P + (i & 1) * N * 128;
-          const uint8_t* v = static_cast<const uint8_t*>(p.a.v) + static_cast<long long>(p_row) * TILE_BYTES + key;
-          const int c0 = row0 + j, c1 = R + row0 + j;
-          x = 0.f;
-          for (int n = 0; n < limit; ++n) {
-            const auto at = [&](int c) { return from_e4m3(pr[(c >> 5) * 4096 + n * 32 + ((((c >> 4) ^ (n >> 2)) & 1) << 4) + (c & 15)]); };
-            x = fmaf(fmaf(at(c1), 0.0625f, at(c0)), from_e4m3(__ldg(v + n * 128)), x);
-          }
+        for (int j = 0; j < 16; ++j) odd |= o[j] != o[j];
+        if (odd) {
+          float sums[16];
 #pragma unroll
-          for (int jj = 0; jj < 16; ++jj) o[jj] = jj == j ? x : o[jj];
+          for (int j = 0; j < 16; ++j) sums[j] = o[j];
+          visible_sums<R>(sums, gbase + C::OFF_P + (i & 1) * N * 128,
+                          static_cast<const uint8_t*>(p.a.v) + static_cast<long long>(p_row) * TILE_BYTES + key, row_of, row0,
+                          p_limit, p_valid);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[j] = sums[j];
         }
       }
 #pragma unroll
@@ -598,8 +658,8 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
     };
 
     while (ok) {
-      const int e = entries % INFO;
-      ok = mbar_wait_warp(bar(C::B_INFO_FULL + e), (entries / INFO) & 1, guard, 0xc31);
+      const uint32_t e = entries % INFO;
+      ok = wait_warp(bar(C::B_INFO_FULL + e), (entries / INFO) & 1, guard, 0xc31);
       if (!ok) break;
       const int4 x = *reinterpret_cast<const int4*>(gbase + C::OFF_INFO + 32 * e);
       const int4 y = *reinterpret_cast<const int4*>(gbase + C::OFF_INFO + 32 * e + 16);
@@ -624,12 +684,12 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
         const int b = pages & 1, row = x.y, valid = x.z, limit = x.w;
         const float ks = __int_as_float(y.x), vs = __int_as_float(y.y);
         if (fresh) {
-          ok = mbar_wait_warp(bar(C::B_Q_FULL + (items & 1)), (items >> 1) & 1, guard, 0xc32);
+          ok = wait_warp(bar(C::B_Q_FULL + (items & 1)), (items >> 1) & 1, guard, 0xc32);
           if (!ok) break;
           scale_row = qf[(items & 1) * R + row0 + r16];
           fresh = false;
         }
-        ok = mbar_wait_warp(bar(C::B_S_FULL + b), (pages >> 1) & 1, guard, 0xc33);
+        ok = wait_warp(bar(C::B_S_FULL + b), (pages >> 1) & 1, guard, 0xc33);
         if (!ok) break;
         tc_fence_after();
         uint32_t h[16], w[16];
@@ -646,27 +706,25 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
           s[j] = x.x;
           s[j + 1] = x.y;
         }
-        uint32_t hidden = 0;                       // rows that do not see this key
         if (partial) {
+          // Rows are in token order: those that do not see this key are the first ones.
+          const int first = p.a.causal ? (key - limit + 1) * p.group - row0 : key >= limit ? 16 : 0;
+          const int unseen = key >= valid ? 16 : first;
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int sees = min(p.a.causal ? limit + (row0 + j) / p.group : limit, valid);
-            if (key >= sees) {
-              hidden |= 1u << j;
-              s[j] = -INFINITY;
-            }
-          }
+          for (int j = 0; j < 16; ++j)
+            if (j < unseen) s[j] = -INFINITY;
         }
-        float top = row_maxima(s, lane);
+        float top = halved(s, lane, [](float a, float b) { return fmaxf(a, b); });
         float* mx = maxima + b * C::SOFTMAX_WARPS * 16;
         if (lane < 16) mx[quarter * 16 + lane] = top;
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(C::B_MAX + 2 * wg + b));
-        ok = mbar_wait_warp(bar(C::B_MAX + 2 * wg + b), (pages >> 1) & 1, guard, 0xc36);
+        ok = wait_warp(bar(C::B_MAX + 2 * wg + b), (pages >> 1) & 1, guard, 0xc36);
         if (!ok) break;
         top = fmaxf(fmaxf(mx[r16], mx[16 + r16]), fmaxf(mx[32 + r16], mx[48 + r16]));
         {
-          const float f = scale_row * ks;
+          float f = scale_row * ks;
+          if (f == 0.f) f = 1e-37f;                 // hidden keys stay hidden with a scale of 0
           const bool none = top == -INFINITY;
           const float mu = none ? -INFINITY : top * f;
           const float next = fmaxf(m, mu);
@@ -698,10 +756,6 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
                             i ? make_float2(b4.z, b4.w) : make_float2(b4.x, b4.y));
             v.x = ex2_approx(v.x);
             v.y = ex2_approx(v.y);
-            if (partial) {
-              if (hidden >> j & 1) v.x = 0.f;
-              if (hidden >> (j + 1) & 1) v.y = 0.f;
-            }
             const float2 n = fma2(make_float2(l[j], l[j + 1]), i ? make_float2(k4.z, k4.w) : make_float2(k4.x, k4.y),
                                   mul2(v, i ? make_float2(w4.z, w4.w) : make_float2(w4.x, w4.y)));
             l[j] = n.x;
@@ -720,7 +774,7 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
         if (valid < 128 && wg == 0) {
           // rows behind the sequence may hold anything: they become zeros before the second product reads them
           const int n = 2 * pages + 1, vslot = n % SLOTS;
-          ok = mbar_wait_warp(bar(C::B_FULL + vslot), (n / SLOTS) & 1, guard, 0xc34);
+          ok = wait_warp(bar(C::B_FULL + vslot), (n / SLOTS) & 1, guard, 0xc34);
           if (!ok) break;
           if (key >= valid) {
             uint4* v = reinterpret_cast<uint4*>(gbase + C::OFF_RING + vslot * TILE_BYTES + key * 128);
@@ -731,63 +785,56 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(C::B_P_FULL + b));
-        if (pending >= 0) add_output();
+      }
+      if (pending >= 0) {
+        add_output();
+        if (!ok) break;
+      }
+      int type = x.x;
+      asm volatile("" : "+r"(type));               // one copy of add_output for both kinds of entry
+      if (type == PAGE) {
         pending = pages++;
-        masked = limit < valid;
-        p_row = row;
-        p_limit = limit;
-        p_valid = valid;
+        masked = x.w < x.z;
+        p_row = x.y;
+        p_limit = x.w;
+        p_valid = x.z;
         continue;
       }
       // END or EMPTY
-      if (pending >= 0) add_output();
-      if (!ok) break;
       if (x.x == END) {
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(C::B_Q_EMPTY + (items & 1)));
         ++items;
       }
       float* sm = sums + (ends & 1) * C::SOFTMAX_WARPS * 16;
-      float sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        float t = l[j];
-#pragma unroll
-        for (int by = 16; by; by >>= 1) t += __shfl_xor_sync(0xffffffffu, t, by);
-        sum = r16 == j ? t : sum;
-      }
+      const float sum = halved(l, lane, [](float a, float b) { return a + b; });
       if (lane < 16) sm[quarter * 16 + lane] = sum;
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(C::B_SUM + 2 * wg + (ends & 1)));
-      ok = mbar_wait_warp(bar(C::B_SUM + 2 * wg + (ends & 1)), (ends >> 1) & 1, guard, 0xc35);
+      ok = wait_warp(bar(C::B_SUM + 2 * wg + (ends & 1)), (ends >> 1) & 1, guard, 0xc35);
       ++ends;
       if (!ok) break;
       const int rows = tokens * p.group;
+      // lane r: sum of row r
+      const float sum_row = ((sm[r16] + sm[16 + r16]) + (sm[32 + r16] + sm[48 + r16])) * 0.00390625f;
       if (place < 0) {
+        const long long first = static_cast<long long>(token0) * p.a.hq + head * p.group;
+        if (lane < 16) factors[lane] = sum_row == 0.f ? 0.f : 1.f / sum_row;
+        __syncwarp();
+        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.a.out) + first * 128 + key;
+        const int* at = row_out + row0;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int row = row0 + j;
-          if (row >= rows) break;
-          const float t = ((sm[j] + sm[16 + j]) + (sm[32 + j] + sm[48 + j])) * 0.00390625f;
-          const int tok = row / p.group;
-          const long long to = (static_cast<long long>(token0) + tok) * p.a.hq + head * p.group + (row - tok * p.group);
-          static_cast<__nv_bfloat16*>(p.a.out)[to * 128 + key] = __float2bfloat16(t == 0.f ? 0.f : acc[j] / t);
-        }
-        if (p.a.lse && quarter == 0 && lane < 16 && row0 + lane < rows) {
-          const float t = ((sm[lane] + sm[16 + lane]) + (sm[32 + lane] + sm[48 + lane])) * 0.00390625f;
-          const int row = row0 + lane, tok = row / p.group;
-          p.a.lse[(static_cast<long long>(token0) + tok) * p.a.hq + head * p.group + (row - tok * p.group)] =
-              t == 0.f ? -INFINITY : (m + log2f(t)) * 0.6931471805599453f;
-        }
+        for (int j = 0; j < 16; ++j)
+          if (row0 + j < rows) out[at[j]] = __float2bfloat16(acc[j] * factors[j]);
+        if (p.a.lse && quarter == 0 && lane < 16 && row0 + lane < rows)
+          p.a.lse[first + (at[lane] >> 7)] = sum_row == 0.f ? -INFINITY : (m + log2f(sum_row)) * 0.6931471805599453f;
       } else {
+        float* part = p.part_o + (static_cast<long long>(place) * R + row0) * 128 + key;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          if (row0 + j >= rows) break;
-          p.part_o[(static_cast<long long>(place) * R + row0 + j) * 128 + key] = acc[j];
-        }
+        for (int j = 0; j < 16; ++j)
+          if (row0 + j < rows) part[j * 128] = acc[j];
         if (quarter == 0 && lane < 16)
-          *reinterpret_cast<float2*>(p.part_ml + (static_cast<long long>(place) * R + row0 + lane) * 2) =
-              make_float2(m, ((sm[lane] + sm[16 + lane]) + (sm[32 + lane] + sm[48 + lane])) * 0.00390625f);
+          *reinterpret_cast<float2*>(p.part_ml + (static_cast<long long>(place) * R + row0 + lane) * 2) = make_float2(m, sum_row);
         if (warp == 0 && lane == 0) {
           int* meta = p.part_meta + 8 * place;
           meta[1] = x0;
@@ -875,7 +922,10 @@ static int rows_of(int group, int pack) { return pack * group <= 16 ? 16 : pack 
 template <int R>
 static int launch(const PagedAttentionArgs& a, int pack, DeviceCtx* ctx, int slot, cudaStream_t stream) {
   using C = Config<R>;
-  Params p{a, a.hq / a.hkv, pack, ctx->sm_count * C::CTAS, nullptr, nullptr, nullptr};
+  Params p{a, a.hq / a.hkv, pack, 0, 0, ctx->sm_count * C::CTAS, nullptr, nullptr, nullptr};
+  while ((1 << p.pack_shift) < pack) ++p.pack_shift;
+  while (a.ids && (1 << p.tile_shift) < a.tile) ++p.tile_shift;
+  if (!a.ids) p.a.topk = 0;
   unsigned char* ws = static_cast<unsigned char*>(a.workspace);
   p.part_o = reinterpret_cast<float*>(ws);
   p.part_ml = p.part_o + static_cast<long long>(2) * p.ctas * R * 128;
