@@ -99,11 +99,6 @@ __device__ __forceinline__ void mma_e4m3(uint32_t d, uint32_t a, uint32_t b, uin
       "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(HI_128), "n"(HI_B)
       : "memory");
 }
-__device__ __forceinline__ float warp_max(float x) {
-  float y;
-  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 d;
   f32x2_unpack(f32x2_mul(f32x2_pack(a.x, a.y), f32x2_pack(b.x, b.y)), d.x, d.y);
@@ -837,12 +832,8 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
           *reinterpret_cast<float2*>(p.part_ml + (static_cast<long long>(place) * R + row0 + lane) * 2) = make_float2(m, sum_row);
         if (warp == 0 && lane == 0) {
           int* meta = p.part_meta + 8 * place;
-          meta[1] = x0;
-          meta[2] = x1;
-          meta[3] = token0;
-          meta[4] = tokens;
-          meta[5] = head;
-          meta[0] = 1;
+          *reinterpret_cast<int4*>(meta) = make_int4(1, x0, x1, token0);
+          *reinterpret_cast<int2*>(meta + 4) = make_int2(tokens, head);
         }
       }
     }
@@ -860,52 +851,104 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
 
 // Adds the parts of the items that lie in several shares, in order:
 //   M = max_i m_i, w_i = exp2(m_i - M), out = sum w_i acc_i / sum w_i l_i, lse = ln 2 (M + log2 sum w_i l_i)
-// CTA x stands at the border of shares x and x + 1; the n - 1 CTAs at the borders inside an item of n parts divide its rows
-// and features among them: a piece is a row's 32 features, done by a whole CTA, a warp takes every eighth part.
-constexpr int MERGE_WARPS = 8;
+// blockIdx.x stands for the border of shares x and x + 1; the (n - 1) gridDim.y CTAs of the borders inside an item of n parts
+// divide its rows: a row to a half warp (16 lanes, 8 features each) where the parts are few, to a whole CTA (a warp takes
+// every eighth part, 4 features a lane) where they are many. Either way a thread makes two dependent round trips to memory or
+// a few more, which is the kernel's time. (Rows one after another by the CTA of the border: 130 us of the 217 of a batch of
+// speculated tokens, 75 of the 293 of a decode batch over 1.4 GB.)
+constexpr int MERGE_WARPS = 8, FEW = 16;
 template <int R>
 __global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const Params p) {
-  __shared__ float s_w[MERGE_WARPS], s_acc[MERGE_WARPS][32], s_l[MERGE_WARPS];
+  __shared__ float s_top[MERGE_WARPS], s_l[MERGE_WARPS];
+  __shared__ float4 s_acc[MERGE_WARPS][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int x = blockIdx.x + 1;
-  const int* meta = p.part_meta + 16 * x;          // the part that comes from the share before
-  if (meta[0] == 0) return;
-  const int x0 = meta[1], x1 = meta[2], token0 = meta[3], tokens = meta[4], head = meta[5];
-  const int parts = x1 - x0 + 1, pieces = tokens * p.group * 4;
-  for (int piece = x - x0 - 1; piece < pieces; piece += parts - 1) {
-    const int row = piece >> 2, d = (piece & 3) * 32 + lane;
-    const auto place = [&](int i) { return static_cast<long long>(2 * (x0 + i) + (i == 0)) * R + row; };
+  const int4 meta = *reinterpret_cast<const int4*>(p.part_meta + 16 * x);        // the part that comes from the share before
+  if (meta.x == 0) return;
+  const int2 more = *reinterpret_cast<const int2*>(p.part_meta + 16 * x + 4);
+  const int x0 = meta.y, parts = meta.z - x0 + 1, token0 = meta.w, rows = more.x * p.group, head = more.y;
+  const int cta = (x - x0 - 1) * gridDim.y + blockIdx.y, ctas = (parts - 1) * gridDim.y;
+  const auto part_row = [&](int i, int row) { return static_cast<long long>(2 * (x0 + i) + (i == 0)) * R + row; };
+  const auto out_row = [&](int row) {
+    const int token = row / p.group;
+    return (static_cast<long long>(token0) + token) * p.a.hq + head * p.group + (row - token * p.group);
+  };
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.a.out);
+  if (parts <= FEW) {
+    const int l16 = lane & 15;
+    const unsigned half = 0xffffu << (lane & 16);
+    for (int row = cta * 2 * MERGE_WARPS + 2 * warp + (lane >> 4); row < rows; row += ctas * 2 * MERGE_WARPS) {
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (l16 < parts) ml = *reinterpret_cast<const float2*>(p.part_ml + part_row(l16, row) * 2);
+      float top = ml.x;
+#pragma unroll
+      for (int by = 8; by; by >>= 1) top = fmaxf(top, __shfl_xor_sync(half, top, by));
+      const float w = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - top);
+      float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, l = 0.f;
+#pragma unroll 4
+      for (int i = 0; i < parts; ++i) {
+        const float4* from = reinterpret_cast<const float4*>(p.part_o + part_row(i, row) * 128) + 2 * l16;
+        const float4 a = from[0], b = from[1];
+        const float wi = __shfl_sync(half, w, i, 16), li = __shfl_sync(half, ml.y, i, 16);
+        l = fmaf(wi, li, l);
+        acc[0] = fmaf(wi, a.x, acc[0]);
+        acc[1] = fmaf(wi, a.y, acc[1]);
+        acc[2] = fmaf(wi, a.z, acc[2]);
+        acc[3] = fmaf(wi, a.w, acc[3]);
+        acc[4] = fmaf(wi, b.x, acc[4]);
+        acc[5] = fmaf(wi, b.y, acc[5]);
+        acc[6] = fmaf(wi, b.z, acc[6]);
+        acc[7] = fmaf(wi, b.w, acc[7]);
+      }
+      const long long to = out_row(row);
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      *reinterpret_cast<uint4*>(out + to * 128 + 8 * l16) =
+          make_uint4(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv),
+                     pack_bf16x2(acc[4] * inv, acc[5] * inv), pack_bf16x2(acc[6] * inv, acc[7] * inv));
+      if (p.a.lse && l16 == 0) p.a.lse[to] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+    }
+    return;
+  }
+  for (int row = cta; row < rows; row += ctas) {
     float top = -INFINITY;
-    for (int i = threadIdx.x; i < parts; i += 32 * MERGE_WARPS) top = fmaxf(top, p.part_ml[place(i) * 2]);
-    top = pa::warp_max(top);
-    if (lane == 0) s_w[warp] = top;
+    for (int i = threadIdx.x; i < parts; i += 32 * MERGE_WARPS) top = fmaxf(top, p.part_ml[part_row(i, row) * 2]);
+#pragma unroll
+    for (int by = 16; by; by >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, by));
+    if (lane == 0) s_top[warp] = top;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < MERGE_WARPS; ++w) top = fmaxf(top, s_w[w]);
-    float acc = 0.f, l = 0.f;
+    for (int w = 0; w < MERGE_WARPS; ++w) top = fmaxf(top, s_top[w]);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
 #pragma unroll 8
     for (int i = warp; i < parts; i += MERGE_WARPS) {
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + place(i) * 2);
-      const float o = p.part_o[place(i) * 128 + d];
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + part_row(i, row) * 2);
+      const float4 o = reinterpret_cast<const float4*>(p.part_o + part_row(i, row) * 128)[lane];
       const float w = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - top);
-      acc = fmaf(w, o, acc);
+      acc.x = fmaf(w, o.x, acc.x);
+      acc.y = fmaf(w, o.y, acc.y);
+      acc.z = fmaf(w, o.z, acc.z);
+      acc.w = fmaf(w, o.w, acc.w);
       l = fmaf(w, ml.y, l);
     }
     s_acc[warp][lane] = acc;
     if (lane == 0) s_l[warp] = l;
     __syncthreads();
     if (warp == 0) {
-      acc = l = 0.f;
 #pragma unroll
-      for (int w = 0; w < MERGE_WARPS; ++w) {
-        acc += s_acc[w][lane];
+      for (int w = 1; w < MERGE_WARPS; ++w) {
+        const float4 o = s_acc[w][lane];
+        acc.x += o.x;
+        acc.y += o.y;
+        acc.z += o.z;
+        acc.w += o.w;
         l += s_l[w];
       }
-      const int tok = row / p.group;
-      const long long to = (static_cast<long long>(token0) + tok) * p.a.hq + head * p.group + (row - tok * p.group);
-      static_cast<__nv_bfloat16*>(p.a.out)[to * 128 + d] = __float2bfloat16(l == 0.f ? 0.f : acc / l);
-      if (p.a.lse && d == 0) p.a.lse[to] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+      const long long to = out_row(row);
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      reinterpret_cast<uint2*>(out + to * 128)[lane] = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+      if (p.a.lse && lane == 0) p.a.lse[to] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
     }
     __syncthreads();
   }
@@ -951,7 +994,7 @@ static int launch(const PagedAttentionArgs& a, int pack, DeviceCtx* ctx, int slo
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.ctas - 1);
+  cfg.gridDim = dim3(p.ctas - 1, R / 16);
   cfg.blockDim = dim3(32 * MERGE_WARPS);
   cfg.stream = stream;
   cfg.attrs = attr;
