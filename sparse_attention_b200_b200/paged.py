@@ -11,7 +11,9 @@ A page holds 128 tokens, a head has 128 features. Rows of new tokens are packed 
 captured in a CUDA graph after one eager call. No counterpart in the reference, whose ragged scorer
 (indexers/fp4/vendor_minimax_msa/fp4_indexer_interface.py:745-811) reads a paged key cache that nothing else there uses."""
 import collections
+import contextlib
 import ctypes
+import functools
 
 import torch
 
@@ -19,7 +21,31 @@ from . import _lib
 from .indexers import fp4_block_scores_varlen
 
 PAGE = 128
-_i64 = ctypes.c_int64
+
+# Arguments of the entry points: p a device pointer, q a 64-bit and i a 32-bit whole number, f an fp32, s the stream. With the
+# types known to ctypes a call converts plain numbers, which is most of what a short call costs on the host.
+_KINDS = dict(p=ctypes.c_void_p, q=ctypes.c_int64, i=ctypes.c_int, f=ctypes.c_float, s=ctypes.c_void_p)
+_ENTRIES = dict(extend_pages="pqi" + "ppp" + "i" + "p" + "pppppppp" + "iii" + "s",
+                append_tokens="pqq" + "pqq" + "pp" + "pppppp" + "iiiq" + "s",
+                select_pages="pppp" + "iiiiiiiiii" + "s",
+                paged_attention="pqq" + "pppp" + "pqi" + "ppp" + "ppp" + "q" + "iiii" + "q" + "iiii" + "f" + "s")
+
+
+@functools.lru_cache(maxsize=None)
+def _entry(name):
+    fn = getattr(_lib.lib(), "sparse_b200_" + name)
+    fn.argtypes = [_KINDS[k] for k in _ENTRIES[name]]
+    fn.restype = ctypes.c_int
+    return fn
+
+
+def _on(device):
+    """The device of a call made current, where it is not."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _stream(device):
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 PageBatch = collections.namedtuple(
     "PageBatch", "seq_lens cu_seqlens_q cu_seqlens_k cu_page_offsets kv_indices slots free_count status")
@@ -31,13 +57,13 @@ def _bad(message):
 
 
 def _dense(name, t, dtype, shape, device):
-    if not (t.is_cuda and t.device == device and t.dtype == dtype and tuple(t.shape) == tuple(shape) and t.is_contiguous()):
+    if t.dtype is not dtype or t.device != device or t.shape != shape or not t.is_contiguous():
         _bad(f"{name} must be a contiguous {dtype} tensor {list(shape)} on {device}")
 
 
 def _rows(name, t, heads, device=None, total=None):
     """Packed bf16 rows [T, H, 128]: any token and head stride that keeps rows on 16 bytes."""
-    if not (t.is_cuda and t.dtype == torch.bfloat16 and t.dim() == 3 and t.shape[2] == 128):
+    if t.dtype is not torch.bfloat16 or t.dim() != 3 or t.shape[2] != 128 or not t.is_cuda:
         _bad(f"{name} must be a bfloat16 CUDA tensor [T,H,128]")
     if device is not None and t.device != device:
         _bad(f"{name} must be on {device}")
@@ -45,17 +71,20 @@ def _rows(name, t, heads, device=None, total=None):
         _bad(f"{name} must have shape [{total if total is not None else 'T'},{heads},128]")
     if t.requires_grad:
         _bad("the paged path is forward-only")
-    s = t.stride()
-    if s[2] != 1 or s[0] % 8 or s[1] % 8 or t.data_ptr() % 16:
+    s, at = t.stride(), t.data_ptr()
+    if s[2] != 1 or (s[0] | s[1]) % 8 or at % 16:
         _bad(f"{name}: rows must be dense, 16-byte aligned and at strides that are multiples of 8 elements")
+    return at, s[0], s[1]
 
 
 def _table(block_table, batch, device):
-    if not (block_table.is_cuda and block_table.device == device and block_table.dtype == torch.int32
-            and block_table.dim() == 2 and block_table.shape[0] == batch and block_table.shape[1] > 0
-            and block_table.stride(1) == 1 and (batch == 1 or block_table.stride(0) >= block_table.shape[1])):
+    """Its address, row stride and width."""
+    if block_table.dtype is not torch.int32 or block_table.device != device or block_table.dim() != 2 \
+            or block_table.shape[0] != batch or block_table.shape[1] == 0 or block_table.stride(1) != 1 \
+            or batch > 1 and block_table.stride(0) < block_table.shape[1]:
         _bad("block_table must be int32 [B, pages per request] with dense rows on the same device")
-    return max(int(block_table.stride(0)), int(block_table.shape[1]))
+    width = block_table.shape[1]
+    return block_table.data_ptr(), max(block_table.stride(0), width), width
 
 
 class PagedCache:
@@ -97,6 +126,7 @@ class PagedCache:
             _dense("k_index_scale", k_index_scale, torch.float8_e4m3fn, (*lead, PAGE, 8), k.device)
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.k_index, self.k_index_scale = k_index, k_index_scale
+        self.addresses = tuple(0 if x is None else x.data_ptr() for x in (k, v, k_scale, v_scale, k_index, k_index_scale))
 
 
 def extend_pages(block_table, seq_lens, new_lens, free_pages, free_count, *, total_q, total_pages):
@@ -106,47 +136,45 @@ def extend_pages(block_table, seq_lens, new_lens, free_pages, free_count, *, tot
     [total_q] int64, free_count [1], status [1] (STATUS_* bits; 0: all is well). total_q and total_pages are the sizes of the
     tables; what is behind the last token or page is -1. A request that gets no pages is refused: its length stays, its slots
     are -1."""
-    batch, dev = int(seq_lens.numel()), seq_lens.device
+    batch, dev = seq_lens.numel(), seq_lens.device
     if not seq_lens.is_cuda or batch == 0:
         _bad("seq_lens must be a CUDA tensor of at least one request")
     _dense("seq_lens", seq_lens, torch.int32, (batch,), dev)
     _dense("new_lens", new_lens, torch.int32, (batch,), dev)
     _dense("free_pages", free_pages, torch.int32, (free_pages.numel(),), dev)
     _dense("free_count", free_count, torch.int32, (1,), dev)
-    stride = _table(block_table, batch, dev)
-    total_q, total_pages = int(total_q), int(total_pages)
+    table, stride, width = _table(block_table, batch, dev)
     if total_q < 0 or total_pages < 0:
         _bad("table sizes must not be negative")
-    with torch.cuda.device(dev):
-        out = torch.empty(4 * batch + 5 + total_pages, dtype=torch.int32, device=dev)
-        slots = torch.empty(total_q, dtype=torch.int64, device=dev)
-        seq, cu_q, cu_k, cu_pages, count, status, kv = out.split(
-            [batch, batch + 1, batch + 1, batch + 1, 1, 1, total_pages])
-        _lib.check(_lib.lib().sparse_b200_extend_pages(
-            _lib.ptr(block_table), _i64(stride), int(block_table.shape[1]), _lib.ptr(seq_lens), _lib.ptr(new_lens),
-            _lib.ptr(free_pages), int(free_pages.numel()), _lib.ptr(free_count), _lib.ptr(seq), _lib.ptr(cu_q),
-            _lib.ptr(cu_k), _lib.ptr(cu_pages), _lib.ptr(kv), _lib.ptr(slots), _lib.ptr(count), _lib.ptr(status), batch,
-            total_q, total_pages, _lib.current_stream()))
-    return PageBatch(seq, cu_q, cu_k, cu_pages, kv, slots, count, status)
+    with _on(dev):
+        # one buffer: slots (int64), then the int32 tables
+        buffer = torch.empty(2 * total_q + 4 * batch + 5 + total_pages, dtype=torch.int32, device=dev)
+        slots, seq, cu_q, cu_k, cu_pages, count, status, kv = torch.split_with_sizes(
+            buffer, (2 * total_q, batch, batch + 1, batch + 1, batch + 1, 1, 1, total_pages))
+        at = buffer.data_ptr()
+        at_seq = at + 8 * total_q
+        at_q = at_seq + 4 * batch
+        step = 4 * batch + 4
+        at_count = at_q + 3 * step
+        _lib.check(_entry("extend_pages")(
+            table, stride, width, seq_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(), free_pages.numel(),
+            free_count.data_ptr(), at_seq, at_q, at_q + step, at_q + 2 * step, at_count + 8, at, at_count, at_count + 4, batch,
+            total_q, total_pages, _stream(dev)))
+    return PageBatch(seq, cu_q, cu_k, cu_pages, kv, slots.view(torch.int64), count, status)
 
 
 def append_tokens(cache, k, v, cu_seqlens_q, slots):
     """k, v [T,Hkv,128] bf16 -> the rows of the cache that slots [T] (extend_pages) names: the tokens of a request lie in
     order from its first slot, page after page. A page's scale is the smallest power of two that holds its rows; the rows
     before the new ones are rescaled where it grows. Index vectors are written where the cache has them."""
-    total, dev = int(slots.numel()), cache.device
-    _rows("k", k, cache.kv_heads, dev, total)
-    _rows("v", v, cache.kv_heads, dev, total)
-    batch = int(cu_seqlens_q.numel()) - 1
+    total, dev = slots.numel(), cache.device
+    rows = (*_rows("k", k, cache.kv_heads, dev, total), *_rows("v", v, cache.kv_heads, dev, total))
+    batch = cu_seqlens_q.numel() - 1
     _dense("cu_seqlens_q", cu_seqlens_q, torch.int32, (batch + 1,), dev)
     _dense("slots", slots, torch.int64, (total,), dev)
-    ks, vs = k.stride(), v.stride()
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().sparse_b200_append_tokens(
-            _lib.ptr(k), _i64(ks[0]), _i64(ks[1]), _lib.ptr(v), _i64(vs[0]), _i64(vs[1]), _lib.ptr(cu_seqlens_q),
-            _lib.ptr(slots), _lib.ptr(cache.k), _lib.ptr(cache.v), _lib.ptr(cache.k_scale), _lib.ptr(cache.v_scale),
-            _lib.ptr(cache.k_index), _lib.ptr(cache.k_index_scale), batch, cache.kv_heads, total, _i64(cache.pages),
-            _lib.current_stream()))
+    with _on(dev):
+        _lib.check(_entry("append_tokens")(*rows, cu_seqlens_q.data_ptr(), slots.data_ptr(), *cache.addresses, batch,
+                                           cache.kv_heads, total, cache.pages, _stream(dev)))
 
 
 def list_rows(total_q, batch, tile):
@@ -158,26 +186,35 @@ def select_pages(scores, cu_seqlens_q, seq_lens, *, kv_heads, topk, tile=1, sink
     """scores [Hidx, pages, T] fp32 (fp4_block_scores_varlen) -> ids [kv_heads, list_rows(T, B, tile), topk] int32: for every
     `tile` consecutive tokens of a request the best pages by (score descending, page ascending), written ascending with -1
     behind them. The first `sink` and the last `recent` pages that the tile's last token sees are always among them."""
-    if not (scores.is_cuda and scores.dtype == torch.float32 and scores.is_contiguous() and scores.dim() == 3):
+    if not scores.is_cuda or scores.dtype is not torch.float32 or scores.dim() != 3 or not scores.is_contiguous():
         _bad("scores must be contiguous float32 [Hidx,pages,T] on CUDA")
-    hidx, pages, total = (int(n) for n in scores.shape)
-    dev, batch = scores.device, int(seq_lens.numel())
+    hidx, pages, total = scores.shape
+    dev, batch = scores.device, seq_lens.numel()
     _dense("seq_lens", seq_lens, torch.int32, (batch,), dev)
     _dense("cu_seqlens_q", cu_seqlens_q, torch.int32, (batch + 1,), dev)
-    if tile < 1 or tile & (tile - 1):
-        _bad("tile must be a power of two from 1 to 128")
+    if tile < 1 or tile & (tile - 1) or kv_heads < 1 or topk < 1:
+        _bad("tile must be a power of two from 1 to 128, KV heads and topk positive")
     shape = (kv_heads, list_rows(total, batch, tile), topk)
-    if kv_heads < 1 or topk < 1:
-        _bad("KV heads and topk must be positive")
-    if ids is None:
-        ids = torch.empty(shape, dtype=torch.int32, device=dev)
-    else:
-        _dense("ids", ids, torch.int32, shape, dev)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().sparse_b200_select_pages(
-            _lib.ptr(scores), _lib.ptr(cu_seqlens_q), _lib.ptr(seq_lens), _lib.ptr(ids), batch, hidx, kv_heads, pages, total,
-            topk, tile, sink, recent, int(bool(causal)), _lib.current_stream()))
+    with _on(dev):
+        if ids is None:
+            ids = torch.empty(shape, dtype=torch.int32, device=dev)
+        else:
+            _dense("ids", ids, torch.int32, shape, dev)
+        _lib.check(_entry("select_pages")(
+            scores.data_ptr(), cu_seqlens_q.data_ptr(), seq_lens.data_ptr(), ids.data_ptr(), batch, hidx, kv_heads, pages, total,
+            topk, tile, sink, recent, bool(causal), _stream(dev)))
     return ids
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(device, hq, hkv, tile, max_q, listed):
+    fn = _lib.lib().sparse_b200_paged_attention_workspace_bytes
+    fn.restype = ctypes.c_int64
+    with torch.cuda.device(device):
+        n = fn(hq, hkv, tile, max_q, listed)
+    if n < 0:
+        _lib.check(n)
+    return n
 
 
 def paged_attention(q, cache, block_table, seq_lens, cu_seqlens_q, ids=None, *, tile=1, max_seqlen_q=None, causal=True,
@@ -187,45 +224,40 @@ def paged_attention(q, cache, block_table, seq_lens, cu_seqlens_q, ids=None, *, 
     keys j <= i + seq_len - n. Returns out [T,Hq,128] bf16, with return_lse also the natural-log LSE [T,Hq] fp32; rows behind
     the last token of out and lse are left as they were. max_seqlen_q: the largest number of new tokens, for how many of them
     share a pass over a page (default: T). scale: default 128^-0.5."""
-    _rows("q", q, None, cache.device)
-    total, hq = int(q.shape[0]), int(q.shape[1])
-    hkv, dev, batch = cache.kv_heads, cache.device, int(seq_lens.numel())
+    hkv, dev, batch = cache.kv_heads, cache.device, seq_lens.numel()
+    rows = _rows("q", q, None, dev)
+    total, hq = q.shape[:2]
     if hq < hkv or hq % hkv or hq // hkv > 64:
         _bad("Hq must be a multiple of Hkv, at most 64 query heads to a KV head")
     _dense("seq_lens", seq_lens, torch.int32, (batch,), dev)
     _dense("cu_seqlens_q", cu_seqlens_q, torch.int32, (batch + 1,), dev)
-    stride = _table(block_table, batch, dev)
+    table = _table(block_table, batch, dev)
     topk = 0
     if ids is not None:
         if ids.dim() != 3 or ids.shape[2] < 1 or tile < 1 or tile > 128 or tile & (tile - 1):
             _bad("ids must be [Hkv, list rows, topk] for a tile that is a power of two from 1 to 128")
-        topk = int(ids.shape[2])
+        topk = ids.shape[2]
         _dense("ids", ids, torch.int32, (hkv, list_rows(total, batch, tile), topk), dev)
-    if out is None:
-        out = torch.empty((total, hq, 128), dtype=torch.bfloat16, device=dev)
-    else:
-        _dense("out", out, torch.bfloat16, (total, hq, 128), dev)
-        for t in (q, cache.k, cache.v):
-            if out.untyped_storage().data_ptr() == t.untyped_storage().data_ptr():
-                _bad("output must not alias inputs")
-    if lse is not None:
-        _dense("lse", lse, torch.float32, (total, hq), dev)
-    elif return_lse:
-        lse = torch.empty((total, hq), dtype=torch.float32, device=dev)
     max_q = total if max_seqlen_q is None else int(max_seqlen_q)
-    lib = _lib.lib()
-    lib.sparse_b200_paged_attention_workspace_bytes.restype = ctypes.c_int64
-    with torch.cuda.device(dev):
-        need = lib.sparse_b200_paged_attention_workspace_bytes(hq, hkv, tile, max_q, int(ids is not None))
-        if need < 0:
-            _lib.check(need)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        _lib.check(lib.sparse_b200_paged_attention(
-            _lib.ptr(q), _i64(q.stride(0)), _i64(q.stride(1)), _lib.ptr(cache.k), _lib.ptr(cache.v), _lib.ptr(cache.k_scale),
-            _lib.ptr(cache.v_scale), _lib.ptr(block_table), _i64(stride), int(block_table.shape[1]), _lib.ptr(seq_lens),
-            _lib.ptr(cu_seqlens_q), _lib.ptr(ids), _lib.ptr(out), _lib.ptr(lse), _lib.ptr(ws), _i64(need), batch, hq, hkv,
-            total, _i64(cache.pages), topk, tile, max_q, int(bool(causal)),
-            ctypes.c_float(128 ** -0.5 if scale is None else scale), _lib.current_stream()))
+    with _on(dev):
+        if out is None:
+            out = torch.empty((total, hq, 128), dtype=torch.bfloat16, device=dev)
+        else:
+            _dense("out", out, torch.bfloat16, (total, hq, 128), dev)
+            for t in (q, cache.k, cache.v):
+                if out.untyped_storage().data_ptr() == t.untyped_storage().data_ptr():
+                    _bad("output must not alias inputs")
+        if lse is not None:
+            _dense("lse", lse, torch.float32, (total, hq), dev)
+        elif return_lse:
+            lse = torch.empty((total, hq), dtype=torch.float32, device=dev)
+        # scratch of this call alone, from torch's caching allocator (inside torch.cuda.graph it belongs to the graph)
+        need = _workspace_bytes(dev.index, hq, hkv, tile, max_q, topk > 0)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        _lib.check(_entry("paged_attention")(
+            *rows, *cache.addresses[:4], *table, seq_lens.data_ptr(), cu_seqlens_q.data_ptr(),
+            0 if ids is None else ids.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), ws.data_ptr(), need, batch,
+            hq, hkv, total, cache.pages, topk, tile, max_q, bool(causal), 128 ** -0.5 if scale is None else scale, _stream(dev)))
     return (out, lse) if return_lse else out
 
 
@@ -255,13 +287,13 @@ def quantize_rows(q, hidx):
     """Packed rows q [T,Hq,128] bf16 (contiguous) -> NVFP4 query index vectors (codes [T,hidx,64], scales [T,hidx,8]): the
     mean over the Hq/hidx heads of a group, as indexers.quantize_queries for whole sequences."""
     _rows("q", q, None)
-    total, hq = int(q.shape[0]), int(q.shape[1])
+    total, hq = q.shape[:2]
     if hq % hidx or not q.is_contiguous():
         _bad("q must be contiguous and Hq a multiple of the index head count")
-    codes = torch.empty((total, hidx, 64), dtype=torch.uint8, device=q.device)
-    scales = torch.empty((total, hidx, 8), dtype=torch.float8_e4m3fn, device=q.device)
-    if total:
-        with torch.cuda.device(q.device):      # T batches of one token: their heads are T rows apart by Hq, as the kernel wants
+    with _on(q.device):
+        codes = torch.empty((total, hidx, 64), dtype=torch.uint8, device=q.device)
+        scales = torch.empty((total, hidx, 8), dtype=torch.float8_e4m3fn, device=q.device)
+        if total:      # T batches of one token
             _lib.check(_lib.lib().sparse_b200_nvfp4_quantize(_lib.ptr(q), _lib.ptr(codes), _lib.ptr(scales), total, hidx,
-                                                             hq // hidx, 1, 0, _lib.current_stream()))
+                                                             hq // hidx, 1, 0, ctypes.c_void_p(_stream(q.device))))
     return codes, scales
