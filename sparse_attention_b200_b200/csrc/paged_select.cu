@@ -7,18 +7,20 @@
 // Pages that no token of the list sees, or whose scores are all -inf or NaN, are not listed. A list belongs to `tile`
 // consecutive tokens of one request (first_list_row in paged.cuh).
 //
-// What bounds it: one pass over the scores (4 bytes per index head, page and token). They lie with the tokens innermost, so a
-// CTA takes neighbouring lists, whose tokens fill the 32-byte sectors that it reads, and leaves the maxima as ordered 32-bit
-// keys in shared memory, a row for each list. A warp then finds a list's k-th largest key bit by bit (counting keys at or
-// above a trial value; it stops as soon as exactly k are) and writes the pages above it in page order, by ballots: no sort,
-// and the lists come out as they lie in the sequence.
+// What bounds it: the latency of one pass over the scores (4 bytes per index head, page and token) in a decode step, the
+// searches in a prompt. The scores lie with the tokens innermost, so a CTA takes neighbouring lists, whose tokens fill (or half
+// fill) the 32-byte sectors that it reads, and leaves the maxima as ordered 32-bit keys in shared memory, a row for each list.
+// A warp then takes a list's keys into registers (up to 16 a lane) and finds a border with exactly k keys at or above it, or
+// the k-th key and how many of its equals are taken: it halves the interval of values (not of bits: scores of one sign and
+// size agree in their leading bits) between the smallest and the largest key, about ten counts of a few instructions and a
+// redux each; after 16 of them the interval of keys, which ends whatever the values. The pages above the border are written in
+// page order by ballots: no sort, and a list lies as the sequence does.
 #include "internal.h"
 #include "paged.cuh"
 
 namespace sb {
 namespace {
 
-constexpr int THREADS = 256, WARPS = THREADS / 32;
 constexpr int SMEM_MOST = 200 * 1024;
 
 struct SelectArgs {
@@ -35,15 +37,111 @@ __device__ __forceinline__ uint32_t ordered(float x) {
   if (!(x > -INFINITY)) return 0;
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float value_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 
-template <int ROWS>
+constexpr uint32_t FORCED = 0xffffffffu;
+
+// Writes the list of the n keys k[0..n) (shared memory). KEYS > 0: at most 32 KEYS of them, held in registers.
+template <int KEYS>
+__device__ __forceinline__ void write_list(const uint32_t* k, int n, int topk, int32_t* out) {
+  const int lane = threadIdx.x & 31;
+  uint32_t mine[KEYS ? KEYS : 1];
+  uint32_t top = 0, low = FORCED;
+  int some = 0, forced = 0;
+  const auto look = [&](uint32_t x) {
+    some += x != 0;
+    forced += x == FORCED;
+    if (x != 0 && x != FORCED) {
+      top = max(top, x);
+      low = min(low, x);
+    }
+  };
+  if constexpr (KEYS > 0) {
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) {
+      const int j = 32 * i + lane;
+      mine[i] = j < n ? k[j] : 0;
+      look(mine[i]);
+    }
+  } else {
+    for (int j = lane; j < n; j += 32) look(k[j]);
+  }
+  const auto at_least = [&](uint32_t x) {
+    int c = 0;
+    if constexpr (KEYS > 0) {
+#pragma unroll
+      for (int i = 0; i < KEYS; ++i) c += mine[i] >= x;
+    } else {
+      for (int j = lane; j < n; j += 32) c += k[j] >= x;
+    }
+    return static_cast<int>(__reduce_add_sync(FORCED, c));
+  };
+  some = __reduce_add_sync(FORCED, some);
+  forced = __reduce_add_sync(FORCED, forced);
+  uint32_t border = 1;                     // taken: keys above it, and the first `equals` of those equal to it
+  int equals = topk;
+  if (some > topk && forced < topk) {
+    top = __reduce_max_sync(FORCED, top);
+    low = __reduce_min_sync(FORCED, low);
+    // more than topk keys are at or above low, fewer than topk above top
+    border = low;
+    uint32_t over = top + 1;
+    int above = forced;                    // keys at or above `over`
+    equals = 0;
+    for (int step = 0; over - border > 1; ++step) {
+      uint32_t trial = border + ((over - border) >> 1);
+      if (step < 16) {
+        const float middle = 0.5f * value_of(border) + 0.5f * value_of(over);
+        const uint32_t x = ordered(middle);
+        if (x > border && x < over) trial = x;
+      }
+      const int c = at_least(trial);
+      if (c == topk) {
+        border = trial;
+        equals = topk;
+        break;
+      }
+      if (c > topk) {
+        border = trial;
+      } else {
+        over = trial;
+        above = c;
+      }
+    }
+    if (equals == 0) equals = topk - above;
+  } else if (some > topk) {
+    border = FORCED;                       // the forced pages fill the list
+  }
+  int written = 0;
+  const auto emit = [&](uint32_t key, int j) {
+    const uint32_t equal = __ballot_sync(FORCED, key == border);
+    const bool in = key > border || (key == border && __popc(equal & ((1u << lane) - 1)) < equals);
+    const uint32_t taken = __ballot_sync(FORCED, in);
+    if (in) out[written + __popc(taken & ((1u << lane) - 1))] = j;
+    written += __popc(taken);
+    equals -= min(equals, __popc(equal));
+  };
+  if constexpr (KEYS > 0) {
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i)
+      if (32 * i < n) emit(mine[i], 32 * i + lane);
+  } else {
+    for (int base = 0; base < n && written < topk; base += 32) emit(base + lane < n ? k[base + lane] : 0, base + lane);
+  }
+  for (int j = written + lane; j < topk; j += 32) out[j] = -1;
+}
+
+// SINGLE: a list has one token and one index head
+template <int ROWS, int THREADS, int KEYS, bool SINGLE>
 __global__ void __launch_bounds__(THREADS) select_pages_kernel(SelectArgs a) {
+  constexpr int WARPS = THREADS / 32;
   extern __shared__ uint32_t keys[];
   __shared__ int s_first[ROWS], s_count[ROWS], s_seen[ROWS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int head = blockIdx.y;
   const int row0 = blockIdx.x * ROWS;
   // the tokens of each list and the pages that its last token sees
+#pragma unroll 1
   for (int i = warp; i < ROWS; i += WARPS) {
     const int row = row0 + i;
     int first = 0, count = 0, seen = 0;
@@ -57,7 +155,7 @@ __global__ void __launch_bounds__(THREADS) select_pages_kernel(SelectArgs a) {
         count = min(a.tile, end - first);
         const int k = max(__ldg(a.seq + r), 0);
         const int keys_seen = a.causal ? k - (end - (first + count)) : k;
-        seen = min(max((keys_seen + 127) >> 7, 0), a.pages);
+        seen = min(max((keys_seen >> 7) + ((keys_seen & 127) != 0), 0), a.pages);
       }
     }
     if (lane == 0) {
@@ -70,85 +168,60 @@ __global__ void __launch_bounds__(THREADS) select_pages_kernel(SelectArgs a) {
   const float* scores = a.scores + static_cast<long long>(head) * a.group * a.pages * a.total_q;
   const long long head_stride = static_cast<long long>(a.pages) * a.total_q;
   constexpr int STEP = THREADS / ROWS;
-  const int mine = tid % ROWS;
+  const int mine = tid % ROWS, page0 = tid / ROWS;
   const int seen = s_seen[mine], count = s_count[mine];
   const float* from = scores + s_first[mine];
-#pragma unroll 2
-  for (int page = tid / ROWS; page < a.pages; page += STEP) {
-    uint32_t key = 0;
-    if (page < seen) {
-      if (page < a.sink || page >= seen - a.recent) {
-        key = 0xffffffffu;
-      } else {
+  uint32_t* row = keys + mine * a.pitch;
+  const auto always = [&](int page) { return page < a.sink || page >= seen - a.recent; };
+  if constexpr (SINGLE) {
+    constexpr int AHEAD = 8;               // loads in flight
+    for (int page = page0; page < seen; page += AHEAD * STEP) {
+      float x[AHEAD];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+        if (page + i * STEP < seen) x[i] = __ldg(from + static_cast<long long>(page + i * STEP) * a.total_q);
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i)
+        if (page + i * STEP < seen) row[page + i * STEP] = always(page + i * STEP) ? FORCED : ordered(x[i]);
+    }
+  } else {
+    for (int page = page0; page < seen; page += STEP) {
+      uint32_t key = FORCED;
+      if (!always(page)) {
         const float* p = from + static_cast<long long>(page) * a.total_q;
         float best = -INFINITY;
         for (int t = 0; t < count; ++t) {
-#pragma unroll 8
+#pragma unroll 16
           for (int h = 0; h < a.group; ++h) best = fmaxf(best, __ldg(p + h * head_stride + t));
         }
         key = ordered(best);
       }
+      row[page] = key;
     }
-    keys[mine * a.pitch + page] = key;
   }
   __syncthreads();
+#pragma unroll 1
   for (int i = warp; i < ROWS; i += WARPS) {
     if (row0 + i >= a.lists) break;
-    const uint32_t* k = keys + i * a.pitch;
-    const int n = s_seen[i];
-    int32_t* out = a.ids + (static_cast<long long>(head) * a.lists + row0 + i) * a.topk;
-    const auto at_least = [&](uint32_t x) {
-      int c = 0;
-      for (int j = lane; j < n; j += 32) c += k[j] >= x;
-      return __reduce_add_sync(0xffffffffu, c);
-    };
-    // the largest `least` with at least topk keys at or above it; 1 where there are not that many
-    uint32_t least = 1;
-    int above = at_least(1);
-    bool exact = above <= a.topk;
-    if (!exact) {
-      least = 0;
-      for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t trial = least | (1u << bit);
-        const int c = at_least(trial);
-        if (c >= a.topk) {
-          least = trial;
-          above = c;
-          if (c == a.topk) {
-            exact = true;
-            break;
-          }
-        }
-      }
-    }
-    // keys above `least`, and of those equal to it the first few
-    int equal_room = a.topk;
-    if (!exact) equal_room = a.topk - (least == 0xffffffffu ? 0 : at_least(least + 1));
-    int written = 0;
-    for (int base = 0; base < n && written < a.topk; base += 32) {
-      const int j = base + lane;
-      const uint32_t key = j < n ? k[j] : 0;
-      const uint32_t equal = __ballot_sync(0xffffffffu, !exact && key == least);
-      const int rank = __popc(equal & ((1u << lane) - 1));
-      const bool in = exact ? key >= least : key > least || (key == least && rank < equal_room);
-      const uint32_t taken = __ballot_sync(0xffffffffu, in);
-      if (in) out[written + __popc(taken & ((1u << lane) - 1))] = j;
-      written += __popc(taken);
-      equal_room -= min(equal_room, __popc(equal));
-    }
-    for (int j = written + lane; j < a.topk; j += 32) out[j] = -1;
+    write_list<KEYS>(keys + i * a.pitch, s_seen[i], a.topk, a.ids + (static_cast<long long>(head) * a.lists + row0 + i) * a.topk);
   }
 }
 
-template <int ROWS>
-int launch(const SelectArgs& a, DeviceCtx* ctx, int slot, cudaStream_t stream) {
-  if (!ctx->paged_attr[slot]) {
-    if (cudaFuncSetAttribute(select_pages_kernel<ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MOST) != cudaSuccess)
-      return set_error(SB_ERR_CUDA, "shared memory of the page selection");
-    ctx->paged_attr[slot] = 1;
-  }
-  select_pages_kernel<ROWS><<<dim3((a.lists + ROWS - 1) / ROWS, a.heads), THREADS, ROWS * a.pitch * 4, stream>>>(a);
+template <int ROWS, int THREADS, int KEYS, bool SINGLE>
+int launch(const SelectArgs& a, cudaStream_t stream) {
+  const auto kernel = select_pages_kernel<ROWS, THREADS, KEYS, SINGLE>;
+  const int smem = ROWS * a.pitch * 4;
+  if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MOST) != cudaSuccess)
+    return set_error(SB_ERR_CUDA, "shared memory of the page selection");
+  kernel<<<dim3((a.lists + ROWS - 1) / ROWS, a.heads), THREADS, smem, stream>>>(a);
   return check_kernel_launch();
+}
+
+template <int ROWS, int THREADS, bool SINGLE>
+int launch(const SelectArgs& a, cudaStream_t stream) {
+  return a.pages <= 128   ? launch<ROWS, THREADS, 4, SINGLE>(a, stream)
+         : a.pages <= 512 ? launch<ROWS, THREADS, 16, SINGLE>(a, stream)
+                          : launch<ROWS, THREADS, 0, SINGLE>(a, stream);
 }
 
 }  // namespace
@@ -163,9 +236,11 @@ int launch_select_pages(const float* scores, const int32_t* cu_q, const int32_t*
                static_cast<int>(lists), heads, pages | 1};      // odd pitch: neighbouring lists' keys of a page meet no bank twice
   const auto fits = [&](int rows) { return rows * a.pitch * 4 <= SMEM_MOST; };
   if (!fits(1)) return set_error(SB_ERR_INVALID, "too many pages for the page selection");
-  if (fits(32) && lists * heads >= 32LL * ctx->sm_count) return launch<32>(a, ctx, 1, stream);
-  if (fits(8)) return launch<8>(a, ctx, 2, stream);
-  return launch<1>(a, ctx, 3, stream);
+  const bool single = tile == 1 && a.group == 1;
+  // 32 lists to a CTA read whole 128-byte lines; where that leaves SMs idle, four, with the loads spread over 512 threads
+  if (fits(32) && lists * heads >= 32LL * ctx->sm_count) return single ? launch<32, 256, true>(a, stream) : launch<32, 256, false>(a, stream);
+  if (fits(4)) return single ? launch<4, 512, true>(a, stream) : launch<4, 512, false>(a, stream);
+  return launch<1, 512, 0, false>(a, stream);
 }
 
 }  // namespace sb
