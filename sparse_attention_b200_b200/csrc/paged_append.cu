@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(THREADS) append_tokens_kernel(AppendArgs a) {
         v[2 * i + 1] = f.y;
       }
       uint32_t lo, hi;
-      const uint8_t bits = quantize_nvfp4_group(v, lo, hi);
+      const uint8_t bits = quantize_nvfp4_group_bf16(v, lo, hi);
       const long long vector = page_head * 128 + offset + row;
       *reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.k_index) + vector * 64 + group * 8) = make_uint2(lo, hi);
       static_cast<uint8_t*>(a.k_index_scale)[vector * 8 + group] = bits;

@@ -175,8 +175,24 @@ def test_append_tokens_special_values(sp):
     x[9] = 3e38
     x[10:16] = torch.tensor([448.0, 449, 450, 464, 447, 896]).view(6, 1, 1).to(torch.bfloat16)
     table = torch.arange(5).view(5, 1)
-    c = _cache(gen, 5, 1, index=False)
-    _check_append(sp, c, x, x, _cu(lens), _slots(table, [0, 0, 0, 7, 0], lens))
+    _check_append(sp, _cache(gen, 5, 1, index=False), x, x, _cu(lens), _slots(table, [0, 0, 0, 7, 0], lens))
+    x[2, 0, 7] = math.inf                                              # (index vectors of NaN are not specified)
+    _check_append(sp, _cache(gen, 5, 1), x, x, _cu(lens), _slots(table, [0, 0, 0, 7, 0], lens))
+
+
+@pytest.mark.parametrize("top", [1e-38, 1e-3, 0.0117, 0.3, 1.0, 2.7, 6.25, 2688.0, 2700.0, 1e30])
+def test_append_index_vectors_of_all_values(sp, top):
+    """The conversion without a division against the rule with one: every bf16 value below `top` beside it in a group."""
+    x = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(torch.bfloat16)
+    x = x[torch.isfinite(x.float()) & (x.float().abs() <= top) & (x.float().abs() >= top * 1e-5)]
+    x = torch.cat([x[torch.randperm(x.numel(), generator=torch.Generator().manual_seed(1))], torch.zeros(-x.numel() % 120, dtype=x.dtype)])
+    rows = torch.cat([torch.full((x.numel() // 15, 1), top).to(x.dtype), x.view(-1, 15)], 1).view(-1, 1, 128)
+    n = rows.shape[0]
+    cache = sp.PagedCache(-(-n // PAGE), 1)
+    sp.append_tokens(cache, rows.cuda(), rows.cuda(), _i32([0, n]).cuda(), torch.arange(n).cuda())
+    want, scales = oracle.quantize_nvfp4(rows)
+    assert torch.equal(cache.k_index.view(-1, 64)[:n].cpu(), want[:, 0])
+    assert torch.equal(_bits(cache.k_index_scale).view(-1, 8)[:n], scales.view(torch.uint8)[:, 0])
 
 
 def test_append_tokens_without_a_slot_and_behind_the_last_token(sp):
