@@ -36,7 +36,6 @@ namespace pa {
 constexpr int TILE_BYTES = 128 * 128;
 constexpr int INFO = 16;                          // entries in flight
 constexpr int START = 1, PAGE = 2, END = 3, EMPTY = 4, STOP = 5;
-constexpr int MIN_SHARE = 4;                      // pages of a CTA at least
 
 struct Params {
   PagedAttentionArgs a;
@@ -52,27 +51,27 @@ struct Config {
   static constexpr int SOFTMAX_WARPS = 4 * GROUPS;
   static constexpr int LOADER = SOFTMAX_WARPS, MMA = LOADER + 1, QWARP = MMA + 1, WARPS = QWARP + 2;
   static constexpr int THREADS = 32 * WARPS;
-  static constexpr int CTAS = R == 64 ? 1 : 2;    // per SM
-  static constexpr int SLOTS = R == 16 ? 5 : R == 32 ? 4 : 8;
+  static constexpr int CTAS = R == 16 ? 2 : 1;    // per SM
+  static constexpr int SLOTS = R == 16 ? 5 : 9;
   static constexpr int OFF_RING = 0;
   static constexpr int OFF_Q = OFF_RING + SLOTS * TILE_BYTES;       // two buffers of N rows of 128 bytes
-  static constexpr int OFF_P = OFF_Q + 2 * N * 128;                 // two buffers of 128 keys x N columns
-  static constexpr int OFF_FACTOR = OFF_P + 2 * N * 128;            // float [softmax warp][3][16]
-  static constexpr int OFF_OUT = OFF_FACTOR + SOFTMAX_WARPS * 192;  // float [2][softmax warp][2][16]
-  static constexpr int OFF_MAX = OFF_OUT + 2 * SOFTMAX_WARPS * 128; // float [2][softmax warp][16]
-  static constexpr int OFF_SUM = OFF_MAX + 2 * SOFTMAX_WARPS * 64;  // float [2][softmax warp][16]
-  static constexpr int OFF_QF = OFF_SUM + 2 * SOFTMAX_WARPS * 64;   // float [2][R]: what a row's scores are multiplied by
+  static constexpr int OFF_P = OFF_Q + 2 * N * 128;                 // 128 keys x N columns
+  static constexpr int OFF_FACTOR = OFF_P + N * 128;                // float [softmax warp][4][16]
+  static constexpr int OFF_MAX = OFF_FACTOR + SOFTMAX_WARPS * 256;  // bf16 [2][softmax warp][16]
+  static constexpr int OFF_SUM = OFF_MAX + 2 * SOFTMAX_WARPS * 32;  // float [2][softmax warp][16]
+  static constexpr int OFF_EXACT = OFF_SUM + 2 * SOFTMAX_WARPS * 64; // float [softmax warp][16]
+  static constexpr int OFF_QF = OFF_EXACT + SOFTMAX_WARPS * 64;    // float [2][R]: what a row's scores are multiplied by
   static constexpr int OFF_ROW = OFF_QF + 2 * R * 4;                // int [R]: token << 16 | head of a row
   static constexpr int OFF_ROW_OUT = OFF_ROW + R * 4;               // int [R]: offset of a row in the output, from the item's first
   static constexpr int OFF_INFO = OFF_ROW_OUT + R * 4;                  // int [INFO][8]
   static constexpr int OFF_BAR = OFF_INFO + INFO * 32;
   static constexpr int B_INFO_FULL = 0, B_INFO_EMPTY = INFO, B_FULL = 2 * INFO, B_EMPTY = B_FULL + SLOTS;
-  static constexpr int B_S_FULL = B_EMPTY + SLOTS, B_P_FULL = B_S_FULL + 2, B_O_FULL = B_P_FULL + 2, B_Q_FULL = B_O_FULL + 2,
-                       B_Q_EMPTY = B_Q_FULL + 2, B_MAX = B_Q_EMPTY + 2, B_SUM = B_MAX + 2 * GROUPS, B_DONE = B_SUM + 2 * GROUPS, BARS = B_DONE + 1;
+  static constexpr int B_S_FULL = B_EMPTY + SLOTS, B_P_FULL = B_S_FULL + 2, B_O_FULL = B_P_FULL + 1, B_Q_FULL = B_O_FULL + 1,
+                       B_Q_EMPTY = B_Q_FULL + 2, B_MAX = B_Q_EMPTY + 2, B_SUM = B_MAX + 2 * GROUPS, B_EXACT = B_SUM + 2 * GROUPS, B_DONE = B_EXACT + GROUPS, BARS = B_DONE + 1;
   static constexpr int OFF_FLAG = OFF_BAR + BARS * 8;               // int [SLOTS]: for the MMA warp, with a page's K tile
   static constexpr int OFF_MISC = (OFF_FLAG + SLOTS * 4 + 15) / 16 * 16;
   static constexpr int SMEM = OFF_MISC + 64 + 1024;                 // 1024: alignment of the tiles
-  static constexpr int TMEM = 4 * N < 32 ? 32 : 4 * N;              // S0, S1, O0, O1
+  static constexpr int TMEM = 4 * N;                                // S0, S1, O; a power of two
 };
 
 // kind::f8f6f4 instruction descriptor: e4m3 x e4m3 -> fp32, M = 128.
@@ -99,25 +98,65 @@ __device__ __forceinline__ void mma_e4m3(uint32_t d, uint32_t a, uint32_t b, uin
       "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(HI_128), "n"(HI_B)
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 d;
   f32x2_unpack(f32x2_mul(f32x2_pack(a.x, a.y), f32x2_pack(b.x, b.y)), d.x, d.y);
   return d;
 }
-// A sum or maximum over the warp for each of 16 values: lane l gets that of value l % 16. Every step halves the values that a
-// lane holds: 16 shuffles in all. (redux.sync on fp32 took 40 cycles a value.)
-template <typename F>
-__device__ __forceinline__ float halved(const float (&s)[16], int lane, F op) {
+// Sums over the warp of 16 values: lane l gets that of value l % 16. Every step halves the values that a lane holds: 16
+// shuffles in all.
+__device__ __forceinline__ float row_sums(const float (&s)[16], int lane) {
   float a[8], b[4], c[2];
   const bool h8 = lane & 8, h4 = lane & 4, h2 = lane & 2, h1 = lane & 1;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) a[j] = op(h8 ? s[j + 8] : s[j], __shfl_xor_sync(0xffffffffu, h8 ? s[j] : s[j + 8], 8));
+  for (int j = 0; j < 8; ++j) a[j] = (h8 ? s[j + 8] : s[j]) + __shfl_xor_sync(0xffffffffu, h8 ? s[j] : s[j + 8], 8);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) b[j] = op(h4 ? a[j + 4] : a[j], __shfl_xor_sync(0xffffffffu, h4 ? a[j] : a[j + 4], 4));
+  for (int j = 0; j < 4; ++j) b[j] = (h4 ? a[j + 4] : a[j]) + __shfl_xor_sync(0xffffffffu, h4 ? a[j] : a[j + 4], 4);
 #pragma unroll
-  for (int j = 0; j < 2; ++j) c[j] = op(h2 ? b[j + 2] : b[j], __shfl_xor_sync(0xffffffffu, h2 ? b[j] : b[j + 2], 2));
-  const float d = op(h1 ? c[1] : c[0], __shfl_xor_sync(0xffffffffu, h1 ? c[0] : c[1], 1));
-  return op(d, __shfl_xor_sync(0xffffffffu, d, 16));
+  for (int j = 0; j < 2; ++j) c[j] = (h2 ? b[j + 2] : b[j]) + __shfl_xor_sync(0xffffffffu, h2 ? b[j] : b[j + 2], 2);
+  const float d = (h1 ? c[1] : c[0]) + __shfl_xor_sync(0xffffffffu, h1 ? c[0] : c[1], 1);
+  return d + __shfl_xor_sync(0xffffffffu, d, 16);
+}
+// The same for maxima, out of line.
+__device__ __noinline__ float row_maxima_of(float s0, float s1, float s2, float s3, float s4, float s5, float s6, float s7, float s8, float s9,
+                                             float s10, float s11, float s12, float s13, float s14, float s15, int lane) {
+  const float s[16] = {s0, s1, s2, s3, s4, s5, s6, s7, s8, s9, s10, s11, s12, s13, s14, s15};
+  float a[8], b[4], c[2];
+  const bool h8 = lane & 8, h4 = lane & 4, h2 = lane & 2, h1 = lane & 1;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) a[j] = fmaxf(h8 ? s[j + 8] : s[j], __shfl_xor_sync(0xffffffffu, h8 ? s[j] : s[j + 8], 8));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) b[j] = fmaxf(h4 ? a[j + 4] : a[j], __shfl_xor_sync(0xffffffffu, h4 ? a[j] : a[j + 4], 4));
+#pragma unroll
+  for (int j = 0; j < 2; ++j) c[j] = fmaxf(h2 ? b[j + 2] : b[j], __shfl_xor_sync(0xffffffffu, h2 ? b[j] : b[j + 2], 2));
+  const float d = fmaxf(h1 ? c[1] : c[0], __shfl_xor_sync(0xffffffffu, h1 ? c[0] : c[1], 1));
+  return fmaxf(d, __shfl_xor_sync(0xffffffffu, d, 16));
+}
+__device__ __forceinline__ float row_maxima(const float (&s)[16], int lane) {
+  return row_maxima_of(s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], s[9], s[10], s[11], s[12], s[13], s[14], s[15], lane);
+}
+// Maxima over the warp of 16 values in 8 pairs of bf16: lane l gets those of pair l % 8.
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ uint32_t pair_maxima(const uint32_t (&s)[8], int lane) {
+  uint32_t b[4], c[2];
+  const bool h4 = lane & 4, h2 = lane & 2, h1 = lane & 1;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) b[j] = max_bf16x2(h4 ? s[j + 4] : s[j], __shfl_xor_sync(0xffffffffu, h4 ? s[j] : s[j + 4], 4));
+#pragma unroll
+  for (int j = 0; j < 2; ++j) c[j] = max_bf16x2(h2 ? b[j + 2] : b[j], __shfl_xor_sync(0xffffffffu, h2 ? b[j] : b[j + 2], 2));
+  uint32_t d = max_bf16x2(h1 ? c[1] : c[0], __shfl_xor_sync(0xffffffffu, h1 ? c[0] : c[1], 1));
+  d = max_bf16x2(d, __shfl_xor_sync(0xffffffffu, d, 8));
+  return max_bf16x2(d, __shfl_xor_sync(0xffffffffu, d, 16));
 }
 // A wait by a whole converged warp whose slow part is not in line: a role's loop has to fit the instruction caches beside the
 // others' (the first build of this kernel had 164 KB of code and ran at a fifth of its speed).
@@ -163,6 +202,25 @@ __device__ __forceinline__ float2 from_e4m3x2(uint32_t codes) {
 }
 __device__ __forceinline__ float from_e4m3(uint32_t code) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(code), __NV_E4M3)));
+}
+
+// hi + lo / 16 of 16 rows from tensor memory, eight at a time (registers)
+template <int R>
+__device__ __forceinline__ void load_sums(uint32_t at, float (&x)[16]) {
+#pragma unroll
+  for (int i = 0; i < 16; i += 8) {
+    uint32_t h[8], w[8];
+    tmem_ld8(at + i, h);
+    tmem_ld8(at + R + i, w);
+    tc_wait_ld();
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      const float2 y = fma2(make_float2(__uint_as_float(w[j]), __uint_as_float(w[j + 1])), make_float2(0.0625f, 0.0625f),
+                            make_float2(__uint_as_float(h[j]), __uint_as_float(h[j + 1])));
+      x[i + j] = y.x;
+      x[i + j + 1] = y.y;
+    }
+  }
 }
 
 // o[j] where it is NaN: the sum of p v over the keys of a page that row row0 + j sees, from the probabilities in shared memory
@@ -251,12 +309,12 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(C::B_S_FULL + i), 1);
-      mbar_init(bar(C::B_P_FULL + i), C::SOFTMAX_WARPS);
-      mbar_init(bar(C::B_O_FULL + i), 1);
       mbar_init(bar(C::B_Q_FULL + i), 2);
       mbar_init(bar(C::B_Q_EMPTY + i), C::SOFTMAX_WARPS);
     }
-    for (int i = 0; i < 4 * C::GROUPS; ++i) mbar_init(bar(C::B_MAX + i), 4);
+    mbar_init(bar(C::B_P_FULL), C::SOFTMAX_WARPS);
+    mbar_init(bar(C::B_O_FULL), 1);
+    for (int i = 0; i < 5 * C::GROUPS; ++i) mbar_init(bar(C::B_MAX + i), 4);
     mbar_init(bar(C::B_DONE), 1);
     fence_mbar_init();
     p.part_meta[16 * blockIdx.x] = 0;             // no part yet in either of this CTA's places
@@ -299,7 +357,7 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
     per_head += s_scan[w];
   }
   const long long total = per_head * p.a.hkv;
-  const long long share = max((total + p.ctas - 1) / p.ctas, static_cast<long long>(MIN_SHARE));
+  const long long share = max((total + p.ctas - 1) / p.ctas, 1LL);
   const long long unit0 = blockIdx.x * share, unit1 = min(unit0 + share, total);
   const int head0 = unit0 < total ? static_cast<int>(unit0 / per_head) : 0;
   if (unit0 < total) {
@@ -440,9 +498,9 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   } else if (warp == C::MMA) {
     // --------------------------------------------------------------- MMA issuer
-    // Waits by the whole warp, issue by its elected lane. That S and O of a page may be overwritten by the page after the
-    // next needs no barrier: the softmax warps store the probabilities of a page after they have read its S and the O of the
-    // page before the last.
+    // Waits by the whole warp, issue by its elected lane. That S may be overwritten by the page after the next, and O by the
+    // next, needs no barrier: the softmax warps store the probabilities of a page after they have read its S and the O of the
+    // page before.
     constexpr uint32_t ID_QK = idesc_e4m3(N, false), ID_PV = idesc_e4m3(N, true);
     bool ok = true, stopped = false;
     int first = 0, second = 0, item = -1;          // pages whose first / second product has been issued
@@ -487,20 +545,19 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
         if (stopped || !ok) break;
         continue;
       }
-      const int b = second & 1;
-      if (!stopped && first - second < 2 && !__all_sync(0xffffffffu, mbar_test_wait(bar(C::B_P_FULL + b), (second >> 1) & 1))) {
+      if (!stopped && first - second < 2 && !__all_sync(0xffffffffu, mbar_test_wait(bar(C::B_P_FULL), second & 1))) {
         const bool late = clock64() - t0 > WAIT_LIMIT_CYCLES || *guard.abort_flag;
         if (!__any_sync(0xffffffffu, late)) continue;
       }
-      ok = wait_warp(bar(C::B_P_FULL + b), (second >> 1) & 1, guard, 0xc12) && wait_warp(bar(C::B_FULL + v_slot), v_phase, guard, 0xc13);
+      ok = wait_warp(bar(C::B_P_FULL), second & 1, guard, 0xc12) && wait_warp(bar(C::B_FULL + v_slot), v_phase, guard, 0xc13);
       if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
         const uint32_t v = ((base + C::OFF_RING + v_slot * TILE_BYTES) >> 4) | LO_MN128;
-        const uint32_t pr = ((base + C::OFF_P + b * N * 128) >> 4) | LO_MN32;
+        const uint32_t pr = ((base + C::OFF_P) >> 4) | LO_MN32;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mma_e4m3<HI_MN32>(tmem + (2 + b) * N, v + k * 256, pr + k * 64, ID_PV, k > 0);
-        tc_commit(bar(C::B_O_FULL + b));
+        for (int k = 0; k < 4; ++k) mma_e4m3<HI_MN32>(tmem + 2 * N, v + k * 256, pr + k * 64, ID_PV, k > 0);
+        tc_commit(bar(C::B_O_FULL));
         tc_commit(bar(C::B_EMPTY + v_slot));
       }
       __syncwarp();
@@ -582,16 +639,14 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
     // --------------------------------------------------------------- softmax: lane = key, then lane = feature
     const int wg = warp >> 2, quarter = warp & 3, key = quarter * 32 + lane, row0 = wg * 16, r16 = lane & 15;
     const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
-    // of the warp's 16 rows: score factor, exponent offset, weight of the page's sum; and, for each of two pages, what the
-    // sums so far and the page's output are multiplied by
-    float* factors = reinterpret_cast<float*>(gbase + C::OFF_FACTOR) + warp * 48;
-    float* outs = reinterpret_cast<float*>(gbase + C::OFF_OUT) + warp * 32;             // + parity * SOFTMAX_WARPS * 32
-    float* maxima = reinterpret_cast<float*>(gbase + C::OFF_MAX) + wg * 64;             // [4][16]
+    // of the warp's 16 rows: score factor, exponent offset, weight of the page's sum, weight of its output
+    float* factors = reinterpret_cast<float*>(gbase + C::OFF_FACTOR) + warp * 64;
+    __nv_bfloat16* maxima = reinterpret_cast<__nv_bfloat16*>(gbase + C::OFF_MAX) + wg * 64;   // [4][16]
     float* sums = reinterpret_cast<float*>(gbase + C::OFF_SUM) + wg * 64;
     const float* qf = reinterpret_cast<const float*>(gbase + C::OFF_QF);
-    float acc[16], l[16], m = -INFINITY, scale_row = 0.f;
+    float acc[16], l[16], s[16], m = -INFINITY, scale_row = 0.f;      // m: what the sums of row r16 are relative to
     uint32_t entries = 0;
-    int items = 0, ends = 0, pages = 0, pending = -1, masked = 0;
+    int items = 0, ends = 0, exacts = 0, pages = 0, pending = -1, masked = 0;
     int token0 = 0, tokens = 0, head = 0, place = -1, x0 = 0, x1 = 0;
     // of the pending page, for rows that do not see all of its keys
     int p_row = 0, p_limit = 0, p_valid = 0;
@@ -601,26 +656,13 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
 
     // adds the output of page `pending` to acc
     const auto add_output = [&]() {
-      const int b = pending & 1;
-      ok = ok && wait_warp(bar(C::B_O_FULL + b), (pending >> 1) & 1, guard, 0xc30);
-      const int i = pending;
+      ok = ok && wait_warp(bar(C::B_O_FULL), pending & 1, guard, 0xc30);
       pending = -1;
       if (!ok) return;
       tc_fence_after();
-      uint32_t h[16], w[16];
-      tmem_ld16(tmem + lane_base + 2 * N + b * N + row0, h);
-      tmem_ld16(tmem + lane_base + 2 * N + b * N + R + row0, w);
-      tc_wait_ld();
-      tc_fence_before();
-      const float* f = outs + b * C::SOFTMAX_WARPS * 32;
       float o[16];
-#pragma unroll
-      for (int j = 0; j < 16; j += 2) {
-        const float2 x = fma2(make_float2(__uint_as_float(w[j]), __uint_as_float(w[j + 1])), make_float2(0.0625f, 0.0625f),
-                              make_float2(__uint_as_float(h[j]), __uint_as_float(h[j + 1])));
-        o[j] = x.x;
-        o[j + 1] = x.y;
-      }
+      load_sums<R>(tmem + lane_base + 2 * N + row0, o);
+      tc_fence_before();
       if (masked) {
         // A key that is hidden from a row has probability 0 there, and 0 times a NaN of its value is not 0: such a sum is
         // done again over the keys that the row sees.
@@ -631,7 +673,7 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
           float sums[16];
 #pragma unroll
           for (int j = 0; j < 16; ++j) sums[j] = o[j];
-          visible_sums<R>(sums, gbase + C::OFF_P + (i & 1) * N * 128,
+          visible_sums<R>(sums, gbase + C::OFF_P,
                           static_cast<const uint8_t*>(p.a.v) + static_cast<long long>(p_row) * TILE_BYTES + key, row_of, row0,
                           p_limit, p_valid);
 #pragma unroll
@@ -640,15 +682,13 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
       }
 #pragma unroll
       for (int j = 0; j < 16; j += 4) {
-        const float4 c1 = *reinterpret_cast<const float4*>(f + j), c2 = *reinterpret_cast<const float4*>(f + 16 + j);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = j + 2 * i;
-          const float2 x = mul2(make_float2(o[r], o[r + 1]), i ? make_float2(c2.z, c2.w) : make_float2(c2.x, c2.y));
-          const float2 y = fma2(make_float2(acc[r], acc[r + 1]), i ? make_float2(c1.z, c1.w) : make_float2(c1.x, c1.y), x);
-          acc[r] = y.x;
-          acc[r + 1] = y.y;
-        }
+        const float4 c = *reinterpret_cast<const float4*>(factors + 48 + j);
+        const float2 x = fma2(make_float2(o[j], o[j + 1]), make_float2(c.x, c.y), make_float2(acc[j], acc[j + 1]));
+        const float2 y = fma2(make_float2(o[j + 2], o[j + 3]), make_float2(c.z, c.w), make_float2(acc[j + 2], acc[j + 3]));
+        acc[j] = x.x;
+        acc[j + 1] = x.y;
+        acc[j + 2] = y.x;
+        acc[j + 3] = y.y;
       }
     };
 
@@ -676,8 +716,7 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
       }
       if (x.x == START) continue;
       if (x.x == PAGE) {
-        const int b = pages & 1, row = x.y, valid = x.z, limit = x.w;
-        const float ks = __int_as_float(y.x), vs = __int_as_float(y.y);
+        const int b = pages & 1, valid = x.z, limit = x.w;
         if (fresh) {
           ok = wait_warp(bar(C::B_Q_FULL + (items & 1)), (items >> 1) & 1, guard, 0xc32);
           if (!ok) break;
@@ -687,20 +726,9 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
         ok = wait_warp(bar(C::B_S_FULL + b), (pages >> 1) & 1, guard, 0xc33);
         if (!ok) break;
         tc_fence_after();
-        uint32_t h[16], w[16];
-        tmem_ld16(tmem + lane_base + b * N + row0, h);
-        tmem_ld16(tmem + lane_base + b * N + R + row0, w);
-        tc_wait_ld();
+        load_sums<R>(tmem + lane_base + b * N + row0, s);
         tc_fence_before();
-        float s[16];
         const bool partial = valid < 128 || limit < 128;
-#pragma unroll
-        for (int j = 0; j < 16; j += 2) {
-          const float2 x = fma2(make_float2(__uint_as_float(w[j]), __uint_as_float(w[j + 1])), make_float2(0.0625f, 0.0625f),
-                                make_float2(__uint_as_float(h[j]), __uint_as_float(h[j + 1])));
-          s[j] = x.x;
-          s[j + 1] = x.y;
-        }
         if (partial) {
           // Rows are in token order: those that do not see this key are the first ones.
           const int first = p.a.causal ? (key - limit + 1) * p.group - row0 : key >= limit ? 16 : 0;
@@ -709,31 +737,65 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
           for (int j = 0; j < 16; ++j)
             if (j < unseen) s[j] = -INFINITY;
         }
-        float top = halved(s, lane, [](float a, float b) { return fmaxf(a, b); });
-        float* mx = maxima + b * C::SOFTMAX_WARPS * 16;
-        if (lane < 16) mx[quarter * 16 + lane] = top;
+        // Maxima in bf16: a reference, not a result. Rounded up by what the conversion may have lost they bound every score.
+        uint32_t pairs[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pairs[j] = pack_bf16x2(s[2 * j], s[2 * j + 1]);
+        const uint32_t top = pair_maxima(pairs, lane);
+        if (lane < 8) reinterpret_cast<uint32_t*>(maxima + b * C::SOFTMAX_WARPS * 16 + quarter * 16)[lane] = top;
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(C::B_MAX + 2 * wg + b));
+      }
+      // under the other warps' maxima: the output of the page before
+      if (pending >= 0) {
+        add_output();
+        if (!ok) break;
+      }
+      int type = x.x;
+      asm volatile("" : "+r"(type));               // one copy of add_output for all kinds of entries
+      if (type == PAGE) {
+        const int b = pages & 1, valid = x.z;
         ok = wait_warp(bar(C::B_MAX + 2 * wg + b), (pages >> 1) & 1, guard, 0xc36);
         if (!ok) break;
-        top = fmaxf(fmaxf(mx[r16], mx[16 + r16]), fmaxf(mx[32 + r16], mx[48 + r16]));
-        {
-          float f = scale_row * ks;
-          if (f == 0.f) f = 1e-37f;                 // hidden keys stay hidden with a scale of 0
-          const bool none = top == -INFINITY;
-          const float mu = none ? -INFINITY : top * f;
-          const float next = fmaxf(m, mu);
-          const float c1 = m == -INFINITY ? 0.f : ex2_approx(m - next);
-          const float c2 = none ? 0.f : ex2_approx(mu - next);
-          m = next;
-          if (lane < 16) {
-            factors[lane] = f;
-            factors[16 + lane] = none ? 0.f : 8.f - mu;
-            factors[32 + lane] = c2;
-            float* out = outs + b * C::SOFTMAX_WARPS * 32;
-            out[lane] = c1;
-            out[16 + lane] = c2 * vs * 0.00390625f;
+        const __nv_bfloat16* mx = maxima + b * C::SOFTMAX_WARPS * 16 + r16;
+        float top = fmaxf(fmaxf(__bfloat162float(mx[0]), __bfloat162float(mx[16])),
+                          fmaxf(__bfloat162float(mx[32]), __bfloat162float(mx[48])));
+        float f = scale_row * __int_as_float(y.x);
+        if (f == 0.f) f = 1e-37f;                  // hidden keys stay hidden with a scale of 0
+        const bool none = top == -INFINITY;
+        top = fmaf(fabsf(top), 0.00394f, top);     // 2^-8 and a little
+        if (__any_sync(0xffffffffu, fabsf(top * f) > 100.f)) {
+          // Scores so large that this is more than a factor of 1.5: the maxima in fp32. (All four warps of the group are here.)
+          float* exact = reinterpret_cast<float*>(gbase + C::OFF_EXACT) + wg * 64;
+          top = row_maxima(s, lane);
+          if (lane < 16) exact[quarter * 16 + lane] = top;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(C::B_EXACT + wg));
+          ok = wait_warp(bar(C::B_EXACT + wg), exacts++ & 1, guard, 0xc37);
+          if (!ok) break;
+          top = fmaxf(fmaxf(exact[r16], exact[16 + r16]), fmaxf(exact[32 + r16], exact[48 + r16]));
+        }
+        const float mu = none ? -INFINITY : top * f;
+        if (m == -INFINITY) m = mu;
+        // The sums stay relative to the item's first page: fp32 has room for 2^40 above it, and what lies below loses nothing.
+        const bool jump = mu - m > 40.f;
+        if (__any_sync(0xffffffffu, jump)) {
+          if (lane < 16) factors[lane] = jump ? ex2_approx(m - mu) : 1.f;
+          if (jump) m = mu;
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            acc[j] *= factors[j];
+            l[j] *= factors[j];
           }
+          __syncwarp();
+        }
+        if (lane < 16) {
+          const float w = none ? 0.f : ex2_approx(mu - m);
+          factors[lane] = f;
+          factors[16 + lane] = none ? 0.f : 8.f - mu;
+          factors[32 + lane] = w;
+          factors[48 + lane] = w * __int_as_float(y.y) * 0.00390625f;
         }
         __syncwarp();
         uint32_t ph[4], pl[4];
@@ -742,8 +804,7 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
           const float4 f4 = *reinterpret_cast<const float4*>(factors + 4 * j4);
           const float4 b4 = *reinterpret_cast<const float4*>(factors + 16 + 4 * j4);
           const float4 w4 = *reinterpret_cast<const float4*>(factors + 32 + 4 * j4);
-          const float4 k4 = *reinterpret_cast<const float4*>(outs + b * C::SOFTMAX_WARPS * 32 + 4 * j4);
-          ph[j4] = pl[j4] = 0;
+          uint32_t hi[2], lo[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int j = 4 * j4 + 2 * i;
@@ -751,18 +812,19 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
                             i ? make_float2(b4.z, b4.w) : make_float2(b4.x, b4.y));
             v.x = ex2_approx(v.x);
             v.y = ex2_approx(v.y);
-            const float2 n = fma2(make_float2(l[j], l[j + 1]), i ? make_float2(k4.z, k4.w) : make_float2(k4.x, k4.y),
-                                  mul2(v, i ? make_float2(w4.z, w4.w) : make_float2(w4.x, w4.y)));
+            const float2 n = fma2(v, i ? make_float2(w4.z, w4.w) : make_float2(w4.x, w4.y), make_float2(l[j], l[j + 1]));
             l[j] = n.x;
             l[j + 1] = n.y;
             const float2 cut = make_float2(__uint_as_float(__float_as_uint(v.x) & 0xfff00000u),     // four significant bits
                                            __uint_as_float(__float_as_uint(v.y) & 0xfff00000u));
             const float2 rest = fma2(v, make_float2(16.f, 16.f), mul2(cut, make_float2(-16.f, -16.f)));
-            ph[j4] |= e4m3x2(cut.x, cut.y) << (16 * i);
-            pl[j4] |= e4m3x2(rest.x, rest.y) << (16 * i);
+            hi[i] = e4m3x2(cut.x, cut.y);
+            lo[i] = e4m3x2(rest.x, rest.y);
           }
+          ph[j4] = __byte_perm(hi[0], hi[1], 0x5410);
+          pl[j4] = __byte_perm(lo[0], lo[1], 0x5410);
         }
-        unsigned char* to = gbase + C::OFF_P + b * N * 128 + key * 32;
+        unsigned char* to = gbase + C::OFF_P + key * 32;
         const auto column = [&](int c) { return to + (c >> 5) * 4096 + ((((c >> 4) ^ (key >> 2)) & 1) << 4); };
         *reinterpret_cast<uint4*>(column(row0)) = make_uint4(ph[0], ph[1], ph[2], ph[3]);
         *reinterpret_cast<uint4*>(column(R + row0)) = make_uint4(pl[0], pl[1], pl[2], pl[3]);
@@ -779,15 +841,7 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
         }
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(C::B_P_FULL + b));
-      }
-      if (pending >= 0) {
-        add_output();
-        if (!ok) break;
-      }
-      int type = x.x;
-      asm volatile("" : "+r"(type));               // one copy of add_output for both kinds of entry
-      if (type == PAGE) {
+        if (lane == 0) mbar_arrive(bar(C::B_P_FULL));
         pending = pages++;
         masked = x.w < x.z;
         p_row = x.y;
@@ -802,7 +856,7 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
         ++items;
       }
       float* sm = sums + (ends & 1) * C::SOFTMAX_WARPS * 16;
-      const float sum = halved(l, lane, [](float a, float b) { return a + b; });
+      const float sum = row_sums(l, lane);
       if (lane < 16) sm[quarter * 16 + lane] = sum;
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(C::B_SUM + 2 * wg + (ends & 1)));
@@ -852,15 +906,15 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
 // Adds the parts of the items that lie in several shares, in order:
 //   M = max_i m_i, w_i = exp2(m_i - M), out = sum w_i acc_i / sum w_i l_i, lse = ln 2 (M + log2 sum w_i l_i)
 // blockIdx.x stands for the border of shares x and x + 1; the (n - 1) gridDim.y CTAs of the borders inside an item of n parts
-// divide its rows: a row to a half warp (16 lanes, 8 features each) where the parts are few, to a whole CTA (a warp takes
-// every eighth part, 4 features a lane) where they are many. Either way a thread makes two dependent round trips to memory or
+// divide its rows: a row to a half warp (16 lanes, 8 features each) where the parts are few, 32 features of a row to a whole
+// CTA (a warp takes every eighth part) where they are many. Either way a thread makes two dependent round trips to memory or
 // a few more, which is the kernel's time. (Rows one after another by the CTA of the border: 130 us of the 217 of a batch of
 // speculated tokens, 75 of the 293 of a decode batch over 1.4 GB.)
 constexpr int MERGE_WARPS = 8, FEW = 16;
 template <int R>
 __global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const Params p) {
   __shared__ float s_top[MERGE_WARPS], s_l[MERGE_WARPS];
-  __shared__ float4 s_acc[MERGE_WARPS][32];
+  __shared__ float s_acc[MERGE_WARPS][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int x = blockIdx.x + 1;
@@ -910,45 +964,48 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const Par
     }
     return;
   }
-  for (int row = cta; row < rows; row += ctas) {
-    float top = -INFINITY;
-    for (int i = threadIdx.x; i < parts; i += 32 * MERGE_WARPS) top = fmaxf(top, p.part_ml[part_row(i, row) * 2]);
+  for (int piece = cta; piece < 4 * rows; piece += ctas) {
+    const int row = piece >> 2, d = (piece & 3) * 32 + lane;
+    float top = -INFINITY, acc = 0.f, l = 0.f;
+    for (int c = 0; warp + MERGE_WARPS * c < parts; c += 32) {
+      const int mine = warp + MERGE_WARPS * (c + lane), count = min(32, (parts - warp + MERGE_WARPS - 1) / MERGE_WARPS - c);
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (mine < parts) ml = *reinterpret_cast<const float2*>(p.part_ml + part_row(mine, row) * 2);
+      float now = fmaxf(top, ml.x);
 #pragma unroll
-    for (int by = 16; by; by >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, by));
-    if (lane == 0) s_top[warp] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < MERGE_WARPS; ++w) top = fmaxf(top, s_top[w]);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float l = 0.f;
+      for (int by = 16; by; by >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, by));
+      const float keep = top == -INFINITY ? 0.f : ex2_approx(top - now), w = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - now);
+      top = now;
+      acc *= keep;
+      l *= keep;
 #pragma unroll 8
-    for (int i = warp; i < parts; i += MERGE_WARPS) {
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + part_row(i, row) * 2);
-      const float4 o = reinterpret_cast<const float4*>(p.part_o + part_row(i, row) * 128)[lane];
-      const float w = ml.x == -INFINITY ? 0.f : ex2_approx(ml.x - top);
-      acc.x = fmaf(w, o.x, acc.x);
-      acc.y = fmaf(w, o.y, acc.y);
-      acc.z = fmaf(w, o.z, acc.z);
-      acc.w = fmaf(w, o.w, acc.w);
-      l = fmaf(w, ml.y, l);
+      for (int i = 0; i < count; ++i) {
+        const float o = p.part_o[part_row(warp + MERGE_WARPS * (c + i), row) * 128 + d];
+        const float wi = __shfl_sync(0xffffffffu, w, i), li = __shfl_sync(0xffffffffu, ml.y, i);
+        acc = fmaf(wi, o, acc);
+        l = fmaf(wi, li, l);
+      }
     }
     s_acc[warp][lane] = acc;
-    if (lane == 0) s_l[warp] = l;
+    if (lane == 0) {
+      s_top[warp] = top;
+      s_l[warp] = l;
+    }
     __syncthreads();
     if (warp == 0) {
+      top = -INFINITY;
+      acc = l = 0.f;
 #pragma unroll
-      for (int w = 1; w < MERGE_WARPS; ++w) {
-        const float4 o = s_acc[w][lane];
-        acc.x += o.x;
-        acc.y += o.y;
-        acc.z += o.z;
-        acc.w += o.w;
-        l += s_l[w];
+      for (int w = 0; w < MERGE_WARPS; ++w) top = fmaxf(top, s_top[w]);
+#pragma unroll
+      for (int w = 0; w < MERGE_WARPS; ++w) {
+        const float keep = s_top[w] == -INFINITY ? 0.f : ex2_approx(s_top[w] - top);
+        acc = fmaf(keep, s_acc[w][lane], acc);
+        l = fmaf(keep, s_l[w], l);
       }
       const long long to = out_row(row);
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      reinterpret_cast<uint2*>(out + to * 128)[lane] = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-      if (p.a.lse && lane == 0) p.a.lse[to] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
+      out[to * 128 + d] = __float2bfloat16(l == 0.f ? 0.f : acc / l);
+      if (p.a.lse && d == 0) p.a.lse[to] = l == 0.f ? -INFINITY : (top + log2f(l)) * 0.6931471805599453f;
     }
     __syncthreads();
   }
@@ -1007,7 +1064,7 @@ static int launch(const PagedAttentionArgs& a, int pack, DeviceCtx* ctx, int slo
 
 long long paged_attention_workspace_bytes(int hq, int hkv, int tile, int max_q, bool listed, int sm_count) {
   const int rows = pa::rows_of(hq / hkv, pa::pack_of(hq / hkv, tile, max_q, listed));
-  const long long ctas = static_cast<long long>(sm_count) * (rows == 64 ? pa::Config<64>::CTAS : pa::Config<32>::CTAS);
+  const long long ctas = static_cast<long long>(sm_count) * (rows == 16 ? pa::Config<16>::CTAS : pa::Config<64>::CTAS);
   return 2 * ctas * (rows * 130 * 4LL + 32);
 }
 
