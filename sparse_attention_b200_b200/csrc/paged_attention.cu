@@ -34,8 +34,11 @@ namespace sb {
 namespace pa {
 
 constexpr int TILE_BYTES = 128 * 128;
-constexpr int INFO = 16;                          // entries in flight
-constexpr int START = 1, PAGE = 2, END = 3, EMPTY = 4, STOP = 5;
+// What the loader tells the other warps: batches of up to 32 pages of an item. Header (two int4): flags, pages, first token,
+// tokens; KV head, place of the part (-1: the item lies in this share alone), first and last share of the item. Pages (int4
+// each): row of the page in the cache (page * Hkv + head), keys it holds | keys its first token sees << 16, the two scales.
+constexpr int BATCHES = 4, BATCH_BYTES = 32 + 32 * 16;
+constexpr int FIRST = 1, LAST = 2, STOP = 4;      // first batch of an item, last one; there are no more
 
 struct Params {
   PagedAttentionArgs a;
@@ -52,26 +55,27 @@ struct Config {
   static constexpr int LOADER = SOFTMAX_WARPS, MMA = LOADER + 1, QWARP = MMA + 1, WARPS = QWARP + 2;
   static constexpr int THREADS = 32 * WARPS;
   static constexpr int CTAS = R == 16 ? 2 : 1;    // per SM
-  static constexpr int SLOTS = R == 16 ? 5 : 9;
+  static constexpr int SLOTS = R == 16 ? 5 : R == 32 ? 11 : 9;
   static constexpr int OFF_RING = 0;
   static constexpr int OFF_Q = OFF_RING + SLOTS * TILE_BYTES;       // two buffers of N rows of 128 bytes
   static constexpr int OFF_P = OFF_Q + 2 * N * 128;                 // 128 keys x N columns
-  static constexpr int OFF_FACTOR = OFF_P + N * 128;                // float [softmax warp][4][16]
+  static constexpr int OFF_FACTOR = OFF_P + N * 128;               // float [softmax warp][4][16]
   static constexpr int OFF_MAX = OFF_FACTOR + SOFTMAX_WARPS * 256;  // bf16 [2][softmax warp][16]
   static constexpr int OFF_SUM = OFF_MAX + 2 * SOFTMAX_WARPS * 32;  // float [2][softmax warp][16]
   static constexpr int OFF_EXACT = OFF_SUM + 2 * SOFTMAX_WARPS * 64; // float [softmax warp][16]
-  static constexpr int OFF_QF = OFF_EXACT + SOFTMAX_WARPS * 64;    // float [2][R]: what a row's scores are multiplied by
+  static constexpr int OFF_QF = OFF_EXACT + SOFTMAX_WARPS * 64;     // float [2][R]: what a row's scores are multiplied by
   static constexpr int OFF_ROW = OFF_QF + 2 * R * 4;                // int [R]: token << 16 | head of a row
   static constexpr int OFF_ROW_OUT = OFF_ROW + R * 4;               // int [R]: offset of a row in the output, from the item's first
-  static constexpr int OFF_INFO = OFF_ROW_OUT + R * 4;                  // int [INFO][8]
-  static constexpr int OFF_BAR = OFF_INFO + INFO * 32;
-  static constexpr int B_INFO_FULL = 0, B_INFO_EMPTY = INFO, B_FULL = 2 * INFO, B_EMPTY = B_FULL + SLOTS;
+  static constexpr int OFF_INFO = OFF_ROW_OUT + R * 4;
+  static constexpr int OFF_BAR = OFF_INFO + BATCHES * BATCH_BYTES;
+  static constexpr int B_INFO_FULL = 0, B_INFO_EMPTY = BATCHES, B_FULL = 2 * BATCHES, B_EMPTY = B_FULL + SLOTS;
   static constexpr int B_S_FULL = B_EMPTY + SLOTS, B_P_FULL = B_S_FULL + 2, B_O_FULL = B_P_FULL + 1, B_Q_FULL = B_O_FULL + 1,
-                       B_Q_EMPTY = B_Q_FULL + 2, B_MAX = B_Q_EMPTY + 2, B_SUM = B_MAX + 2 * GROUPS, B_EXACT = B_SUM + 2 * GROUPS, B_DONE = B_EXACT + GROUPS, BARS = B_DONE + 1;
+                       B_Q_EMPTY = B_Q_FULL + 2, B_MAX = B_Q_EMPTY + 2, B_SUM = B_MAX + 2 * GROUPS, B_EXACT = B_SUM + 2 * GROUPS,
+                       B_DONE = B_EXACT + GROUPS, BARS = B_DONE + 1;
   static constexpr int OFF_FLAG = OFF_BAR + BARS * 8;               // int [SLOTS]: for the MMA warp, with a page's K tile
   static constexpr int OFF_MISC = (OFF_FLAG + SLOTS * 4 + 15) / 16 * 16;
   static constexpr int SMEM = OFF_MISC + 64 + 1024;                 // 1024: alignment of the tiles
-  static constexpr int TMEM = 4 * N;                                // S0, S1, O; a power of two
+  static constexpr int TMEM = R == 16 ? 128 : 512;                  // S of two pages and O: a power of two
 };
 
 // kind::f8f6f4 instruction descriptor: e4m3 x e4m3 -> fp32, M = 128.
@@ -167,23 +171,12 @@ __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, const G
   if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
   return wait_longer(bar, parity, g.abort_flag, g.status, code);
 }
-__device__ __noinline__ bool post_entry(uint32_t full, uint32_t empty, uint32_t parity, unsigned char* to, int4 a, int4 b,
-                                        volatile int* abort_flag, int* status) {
-  if (!mbar_wait_warp(empty, parity, Guard{abort_flag, status}, 0xc00)) return false;
-  if ((threadIdx.x & 31) == 0) {
-    reinterpret_cast<int4*>(to)[0] = a;
-    reinterpret_cast<int4*>(to)[1] = b;
-    mbar_arrive(full);
-  }
-  __syncwarp();
-  return true;
-}
 __device__ __noinline__ bool load_tile(uint32_t full, uint32_t empty, uint32_t parity, uint32_t to, const CUtensorMap* map, int row,
                                        volatile int* flag_at, int flag, volatile int* abort_flag, int* status) {
   if (!mbar_wait_warp(empty, parity, Guard{abort_flag, status}, 0xc01)) return false;
   if (elect_one()) {
     *flag_at = flag;
-    if (flag < 0) {
+    if (flag == 2) {
       mbar_arrive(full);
     } else {
       mbar_expect_tx(full, TILE_BYTES);
@@ -299,7 +292,7 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
 
   if (tid == 0) {
     misc[1] = 0;
-    for (int i = 0; i < INFO; ++i) {
+    for (int i = 0; i < BATCHES; ++i) {
       mbar_init(bar(C::B_INFO_FULL + i), 1);
       mbar_init(bar(C::B_INFO_EMPTY + i), C::SOFTMAX_WARPS + 2);
     }
@@ -314,7 +307,7 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
     }
     mbar_init(bar(C::B_P_FULL), C::SOFTMAX_WARPS);
     mbar_init(bar(C::B_O_FULL), 1);
-    for (int i = 0; i < 5 * C::GROUPS; ++i) mbar_init(bar(C::B_MAX + i), 4);
+    for (int i = C::B_MAX; i < C::B_DONE; ++i) mbar_init(bar(i), 4);
     mbar_init(bar(C::B_DONE), 1);
     fence_mbar_init();
     p.part_meta[16 * blockIdx.x] = 0;             // no part yet in either of this CTA's places
@@ -381,16 +374,10 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
 
   if (warp == C::LOADER) {
     // --------------------------------------------------------------- loader
-    uint32_t entries = 0;
-    int items = -1, slot = 0, phase = 0;
+    uint32_t batches = 0;
+    int slot = 0, phase = 0;
     bool ok = true;
-    const auto post = [&](int type, int x0, int x1, int x2, int x3, int x4, int x5) {
-      const uint32_t e = entries % INFO;
-      if (ok) ok = post_entry(bar(C::B_INFO_FULL + e), bar(C::B_INFO_EMPTY + e), ((entries / INFO) & 1) ^ 1, gbase + C::OFF_INFO + 32 * e,
-                              make_int4(type, x0, x1, x2), make_int4(x3, x4, x5, 0), guard.abort_flag, status);
-      ++entries;
-    };
-    // flag: what the MMA warp has to know of a K tile: the number of its item, -1 = there are no more tiles
+    // flag: what the MMA warp has to know of a K tile: 1 = the first of an item, 2 = there are no more tiles
     const auto load = [&](const CUtensorMap* map, int row, int flag) {
       if (ok) ok = load_tile(bar(C::B_FULL + slot), bar(C::B_EMPTY + slot), phase ^ 1, base + C::OFF_RING + slot * TILE_BYTES, map, row,
                              reinterpret_cast<volatile int*>(gbase + C::OFF_FLAG + 4 * slot), flag, guard.abort_flag, status);
@@ -399,6 +386,21 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
         slot = 0;
         phase ^= 1;
       }
+    };
+    // waits for a free batch
+    const auto batch = [&]() {
+      const uint32_t e = batches % BATCHES;
+      ok = ok && wait_warp(bar(C::B_INFO_EMPTY + e), ((batches / BATCHES) & 1) ^ 1, guard, 0xc00);
+      return reinterpret_cast<int4*>(gbase + C::OFF_INFO + e * BATCH_BYTES);
+    };
+    const auto post = [&](int4* to, int flags, int pages, int token0, int tokens, int4 item) {
+      if (lane == 0 && ok) {
+        to[0] = make_int4(flags, pages, token0, tokens);
+        to[1] = item;
+      }
+      __syncwarp();
+      if (lane == 0 && ok) mbar_arrive(bar(C::B_INFO_FULL + batches % BATCHES));
+      ++batches;
     };
     if (unit0 < total) {
       long long left = unit1 - unit0;
@@ -431,7 +433,7 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
         const int from = static_cast<int>(off), to = static_cast<int>(min(static_cast<long long>(count), off + left));
         const int x0 = static_cast<int>(start / share), x1 = static_cast<int>((start + count - 1) / share);
         const int place = x0 == x1 ? -1 : 2 * static_cast<int>(blockIdx.x) + (x0 == static_cast<int>(blockIdx.x));
-        bool started = false;
+        bool posted = false, started = false;
         const int32_t* list = nullptr;
         if (p.a.ids) {
           const int s = p.tile_shift;
@@ -446,38 +448,41 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
           if (live && list) j = __ldg(list + j);
           live = live && j >= 0 && j < q.held && j * 128LL < seen;
           int row = 0;
-          float ks = 0.f, vs = 0.f;
           if (live) {
             const int page = __ldg(table + j);
             live = page >= 0 && page < p.a.pages;
-            if (live) {
-              row = page * p.a.hkv + head;
-              ks = __ldg(p.a.k_scale + row);
-              vs = __ldg(p.a.v_scale + row);
-            }
+            row = live ? page * p.a.hkv + head : 0;
           }
-          uint32_t todo = __ballot_sync(0xffffffffu, live);
-#pragma unroll 1
-          while (ok && todo) {
-            const int l = __ffs(todo) - 1;
+          const uint32_t pages = __ballot_sync(0xffffffffu, live);
+          const bool last = at + 32 >= to;
+          if (!pages && !last) continue;
+          uint32_t todo = pages;
+          const auto load_next = [&]() {
+            const int next = __shfl_sync(0xffffffffu, row, __ffs(todo) - 1) * 128;
             todo &= todo - 1;
-            const int pj = __shfl_sync(0xffffffffu, j, l), prow = __shfl_sync(0xffffffffu, row, l);
-            const int pks = __shfl_sync(0xffffffffu, __float_as_int(ks), l), pvs = __shfl_sync(0xffffffffu, __float_as_int(vs), l);
-            const int valid = static_cast<int>(min(128LL, q.k_len - pj * 128LL));
-            // keys of the page that the first token sees; the others one more each. Not causal: all see the same.
-            const int limit = static_cast<int>(max(-128LL, min(128LL, seen0 - pj * 128LL)));
-            if (!started) {
-              started = true;
-              ++items;
-              post(START, q.begin + token0, tokens, head, place, x0, x1);
+            load(&k_map, next, started ? 0 : 1);
+            load(&v_map, next, 0);
+            started = true;
+          };
+          int4* to_batch = nullptr;
+#pragma unroll 1
+          for (bool told = false; ok && (todo || !told);) {
+            if (todo) load_next();
+            if (told) continue;
+            // behind the first page's tiles: the scales have to be fetched
+            told = true;
+            to_batch = batch();
+            if (live && ok) {
+              const int valid = static_cast<int>(min(128LL, q.k_len - j * 128LL));
+              // keys of the page that the first token sees; the others one more each. Not causal: all see the same.
+              const int limit = static_cast<int>(max(-128LL, min(128LL, seen0 - j * 128LL)));
+              to_batch[2 + __popc(pages & ((1u << lane) - 1))] =
+                  make_int4(row, valid | (limit << 16), __float_as_int(__ldg(p.a.k_scale + row)), __float_as_int(__ldg(p.a.v_scale + row)));
             }
-            post(PAGE, prow, valid, limit, pks, pvs, 0);
-            load(&k_map, prow * 128, items);
-            load(&v_map, prow * 128, 0);
+            post(to_batch, (posted ? 0 : FIRST) | (last ? LAST : 0), __popc(pages), q.begin + token0, tokens, make_int4(head, place, x0, x1));
+            posted = true;
           }
         }
-        if (started) post(END, 0, 0, 0, 0, 0, 0);
-        else post(EMPTY, q.begin + token0, tokens, head, place, x0, x1);      // no page of it is taken: its rows are 0
         left -= to - from;
         start += count;
         off = 0;
@@ -493,14 +498,17 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
         }
       }
     }
-    post(STOP, 0, 0, 0, 0, 0, 0);
-    load(&k_map, 0, -1);
+    post(batch(), STOP, 0, 0, 0, make_int4(0, 0, 0, 0));
+    load(&k_map, 0, 2);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   } else if (warp == C::MMA) {
     // --------------------------------------------------------------- MMA issuer
     // Waits by the whole warp, issue by its elected lane. That S may be overwritten by the page after the next, and O by the
-    // next, needs no barrier: the softmax warps store the probabilities of a page after they have read its S and the O of the
-    // page before.
+    // next, needs no barrier: the softmax warps store the probabilities of a page after they have read its S and the O
+    // of the page before.
+    // Everything that the issue depends on is uniform for the compiler to see (counters, votes, no call in the way): the
+    // operands of tcgen05 instructions come from uniform registers, and what is not known to be uniform is moved there
+    // one by one, which took 500 cycles for the four instructions and two commits of a product.
     constexpr uint32_t ID_QK = idesc_e4m3(N, false), ID_PV = idesc_e4m3(N, true);
     bool ok = true, stopped = false;
     int first = 0, second = 0, item = -1;          // pages whose first / second product has been issued
@@ -512,21 +520,37 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
         f ^= 1;
       }
     };
+    const auto ready = [&](int which, int parity) { return __all_sync(0xffffffffu, mbar_test_wait(bar(which), parity)) != 0; };
     long long t0 = clock64();
     while (ok) {
       // One page ahead of the second products; where its K tile is not there yet and the probabilities of the page before
       // are, these go first.
-      if (!stopped && first - second < 2 &&
-          (first == second ? ok = wait_warp(bar(C::B_FULL + slot), phase, guard, 0xc10)
-                           : __all_sync(0xffffffffu, mbar_test_wait(bar(C::B_FULL + slot), phase)))) {
+      bool tile = false;
+      if (!stopped && first - second < 2) {
+        tile = ready(C::B_FULL + slot, phase);
+        if (!tile && first == second) {
+          ok = mbar_wait_warp(bar(C::B_FULL + slot), phase, guard, 0xc10);
+          if (!ok) break;
+          tile = true;
+        }
+      }
+      if (tile) {
         const int flag = *reinterpret_cast<volatile int*>(gbase + C::OFF_FLAG + 4 * slot);
-        stopped = flag < 0;
-        if (!stopped) {
-          if (flag != item) {
-            item = flag;
-            ok = wait_warp(bar(C::B_Q_FULL + (item & 1)), (item >> 1) & 1, guard, 0xc11);
+        stopped = __any_sync(0xffffffffu, flag & 2);
+        const int of = item + (__any_sync(0xffffffffu, flag & 1) ? 1 : 0);
+        bool queries = of == item;
+        if (!stopped && !queries) {
+          // A new item's queries are not waited for while second products are owed: their buffer may be that of an item whose
+          // end needs those.
+          queries = ready(C::B_Q_FULL + (of & 1), (of >> 1) & 1);
+          if (!queries && first == second) {
+            ok = mbar_wait_warp(bar(C::B_Q_FULL + (of & 1)), (of >> 1) & 1, guard, 0xc11);
             if (!ok) break;
+            queries = true;
           }
+        }
+        if (!stopped && queries) {
+          item = of;
           tc_fence_after();
           if (elect_one()) {
             const uint32_t kt = (base + C::OFF_RING + slot * TILE_BYTES) >> 4, qt = (base + C::OFF_Q + (item & 1) * N * 128) >> 4;
@@ -541,15 +565,17 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
           t0 = clock64();
         }
       }
-      if (!ok || first == second) {
-        if (stopped || !ok) break;
+      if (first == second) {
+        if (stopped) break;
         continue;
       }
-      if (!stopped && first - second < 2 && !__all_sync(0xffffffffu, mbar_test_wait(bar(C::B_P_FULL), second & 1))) {
+      if (!ready(C::B_P_FULL, second & 1)) {
         const bool late = clock64() - t0 > WAIT_LIMIT_CYCLES || *guard.abort_flag;
-        if (!__any_sync(0xffffffffu, late)) continue;
+        if (!stopped && first - second < 2 && !__any_sync(0xffffffffu, late)) continue;
+        ok = mbar_wait_warp(bar(C::B_P_FULL), second & 1, guard, 0xc12);
+        if (!ok) break;
       }
-      ok = wait_warp(bar(C::B_P_FULL), second & 1, guard, 0xc12) && wait_warp(bar(C::B_FULL + v_slot), v_phase, guard, 0xc13);
+      ok = mbar_wait_warp(bar(C::B_FULL + v_slot), v_phase, guard, 0xc13);
       if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
@@ -573,27 +599,28 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
     // --------------------------------------------------------------- queries of the next item
     const int half = warp - C::QWARP;
     bool ok = true;
-    uint32_t entries = 0;
+    uint32_t batches = 0;
     int items = 0;
     const float sign = p.a.scale < 0.f ? -1.f : 1.f, factor = fabsf(p.a.scale) * 1.4426950408889634f;
     while (ok) {
-      const uint32_t e = entries % INFO;
-      ok = wait_warp(bar(C::B_INFO_FULL + e), (entries / INFO) & 1, guard, 0xc20);
+      const uint32_t e = batches % BATCHES;
+      ok = wait_warp(bar(C::B_INFO_FULL + e), (batches / BATCHES) & 1, guard, 0xc20);
       if (!ok) break;
-      const int4 x = *reinterpret_cast<const int4*>(gbase + C::OFF_INFO + 32 * e);
+      const int4 x = *reinterpret_cast<const int4*>(gbase + C::OFF_INFO + e * BATCH_BYTES);
+      const int head = *reinterpret_cast<const int*>(gbase + C::OFF_INFO + e * BATCH_BYTES + 16);
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(C::B_INFO_EMPTY + e));
-      ++entries;
-      if (x.x == STOP) break;
-      if (x.x != START) continue;
+      ++batches;
+      if (x.x & STOP) break;
+      if (!(x.x & FIRST) || x.y == 0) continue;
       const int buf = items & 1;
       ok = wait_warp(bar(C::B_Q_EMPTY + buf), ((items >> 1) & 1) ^ 1, guard, 0xc21);
       if (!ok) break;
-      const int rows = x.z * p.group;              // tokens x heads of the KV head
+      const int rows = x.w * p.group;              // tokens x heads of the KV head
       unsigned char* q8 = gbase + C::OFF_Q + buf * N * 128;
       float* qf = reinterpret_cast<float*>(gbase + C::OFF_QF) + buf * R;
-      const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.a.q) + x.y * p.a.q_token +
-                                 static_cast<long long>(x.w) * p.group * p.a.q_head + lane * 4;
+      const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.a.q) + x.z * p.a.q_token +
+                                 static_cast<long long>(head) * p.group * p.a.q_head + lane * 4;
 #pragma unroll 1
       for (int r0 = half * (R / 2); r0 < (half + 1) * (R / 2); r0 += 4) {
         uint2 w[4];
@@ -645,9 +672,9 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
     float* sums = reinterpret_cast<float*>(gbase + C::OFF_SUM) + wg * 64;
     const float* qf = reinterpret_cast<const float*>(gbase + C::OFF_QF);
     float acc[16], l[16], s[16], m = -INFINITY, scale_row = 0.f;      // m: what the sums of row r16 are relative to
-    uint32_t entries = 0;
+    uint32_t batches = 0;
     int items = 0, ends = 0, exacts = 0, pages = 0, pending = -1, masked = 0;
-    int token0 = 0, tokens = 0, head = 0, place = -1, x0 = 0, x1 = 0;
+    int item_pages = 0;
     // of the pending page, for rows that do not see all of its keys
     int p_row = 0, p_limit = 0, p_valid = 0;
     bool ok = true, fresh = false;
@@ -693,203 +720,207 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
     };
 
     while (ok) {
-      const uint32_t e = entries % INFO;
-      ok = wait_warp(bar(C::B_INFO_FULL + e), (entries / INFO) & 1, guard, 0xc31);
+      const uint32_t e = batches % BATCHES;
+      ok = wait_warp(bar(C::B_INFO_FULL + e), (batches / BATCHES) & 1, guard, 0xc31);
       if (!ok) break;
-      const int4 x = *reinterpret_cast<const int4*>(gbase + C::OFF_INFO + 32 * e);
-      const int4 y = *reinterpret_cast<const int4*>(gbase + C::OFF_INFO + 32 * e + 16);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(C::B_INFO_EMPTY + e));
-      ++entries;
-      if (x.x == STOP) break;
-      if (x.x == START || x.x == EMPTY) {
-        token0 = x.y;
-        tokens = x.z;
-        head = x.w;
-        place = y.x;
-        x0 = y.y;
-        x1 = y.z;
+      const int4* info = reinterpret_cast<const int4*>(gbase + C::OFF_INFO + e * BATCH_BYTES);
+      const int flags = info[0].x, count = info[0].y;
+      if (flags & STOP) break;
+      if (flags & FIRST) {
         m = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[i] = l[i] = 0.f;
         fresh = true;
+        item_pages = 0;
       }
-      if (x.x == START) continue;
-      if (x.x == PAGE) {
-        const int b = pages & 1, valid = x.z, limit = x.w;
-        if (fresh) {
-          ok = wait_warp(bar(C::B_Q_FULL + (items & 1)), (items >> 1) & 1, guard, 0xc32);
+      item_pages += count;
+      // the pages of the batch, then the item's end
+      const int steps = count + (flags & LAST ? 1 : 0);
+#pragma unroll 1
+      for (int step = 0; ok && step < steps; ++step) {
+        const bool page = step < count;
+        const volatile int* x = reinterpret_cast<const volatile int*>(info + 2 + min(step, 31));     // read where it is needed: registers
+        const int seen = x[1], valid = seen & 0xffff, limit = seen >> 16;
+        if (page) {
+          const int b = pages & 1;
+          if (fresh) {
+            ok = wait_warp(bar(C::B_Q_FULL + (items & 1)), (items >> 1) & 1, guard, 0xc32);
+            if (!ok) break;
+            scale_row = qf[(items & 1) * R + row0 + r16];
+            fresh = false;
+          }
+          ok = wait_warp(bar(C::B_S_FULL + b), (pages >> 1) & 1, guard, 0xc33);
           if (!ok) break;
-          scale_row = qf[(items & 1) * R + row0 + r16];
-          fresh = false;
+          tc_fence_after();
+          load_sums<R>(tmem + lane_base + b * N + row0, s);
+          tc_fence_before();
+          const bool partial = valid < 128 || limit < 128;
+          if (partial) {
+            // Rows are in token order: those that do not see this key are the first ones.
+            const int first = p.a.causal ? (key - limit + 1) * p.group - row0 : key >= limit ? 16 : 0;
+            const int unseen = key >= valid ? 16 : first;
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (j < unseen) s[j] = -INFINITY;
+          }
+          // Maxima in bf16: a reference, not a result. Rounded up by what the conversion may have lost they bound every score.
+          uint32_t pairs[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) pairs[j] = pack_bf16x2(s[2 * j], s[2 * j + 1]);
+          const uint32_t top = pair_maxima(pairs, lane);
+          if (lane < 8) reinterpret_cast<uint32_t*>(maxima + b * C::SOFTMAX_WARPS * 16 + quarter * 16)[lane] = top;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(C::B_MAX + 2 * wg + b));
         }
-        ok = wait_warp(bar(C::B_S_FULL + b), (pages >> 1) & 1, guard, 0xc33);
+        // under the other warps' maxima: the output of the page before
+        if (pending >= 0) {
+          add_output();
+          if (!ok) break;
+        }
+        int again = page;
+        asm volatile("" : "+r"(again));              // one copy of add_output for pages and ends
+        if (again) {
+          const int b = pages & 1;
+          ok = wait_warp(bar(C::B_MAX + 2 * wg + b), (pages >> 1) & 1, guard, 0xc36);
+          if (!ok) break;
+          const __nv_bfloat16* mx = maxima + b * C::SOFTMAX_WARPS * 16 + r16;
+          float top = fmaxf(fmaxf(__bfloat162float(mx[0]), __bfloat162float(mx[16])),
+                            fmaxf(__bfloat162float(mx[32]), __bfloat162float(mx[48])));
+          float f = scale_row * __int_as_float(x[2]);
+          if (f == 0.f) f = 1e-37f;                  // hidden keys stay hidden with a scale of 0
+          const bool none = top == -INFINITY;
+          top = fmaf(fabsf(top), 0.00394f, top);     // 2^-8 and a little
+          if (__any_sync(0xffffffffu, fabsf(top * f) > 100.f)) {
+            // Scores so large that this is more than a factor of 1.5: the maxima in fp32. (All four warps of the group are here.)
+            float* exact = reinterpret_cast<float*>(gbase + C::OFF_EXACT) + wg * 64;
+            top = row_maxima(s, lane);
+            if (lane < 16) exact[quarter * 16 + lane] = top;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(C::B_EXACT + wg));
+            ok = wait_warp(bar(C::B_EXACT + wg), exacts++ & 1, guard, 0xc37);
+            if (!ok) break;
+            top = fmaxf(fmaxf(exact[r16], exact[16 + r16]), fmaxf(exact[32 + r16], exact[48 + r16]));
+          }
+          const float mu = none ? -INFINITY : top * f;
+          if (m == -INFINITY) m = mu;
+          // The sums stay relative to the item's first page: fp32 has room for 2^40 above it, and what lies below loses nothing.
+          const bool jump = mu - m > 40.f;
+          if (__any_sync(0xffffffffu, jump)) {
+            if (lane < 16) factors[lane] = jump ? ex2_approx(m - mu) : 1.f;
+            if (jump) m = mu;
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              acc[j] *= factors[j];
+              l[j] *= factors[j];
+            }
+            __syncwarp();
+          }
+          if (lane < 16) {
+            const float w = none ? 0.f : ex2_approx(mu - m);
+            factors[lane] = f;
+            factors[16 + lane] = none ? 0.f : 8.f - mu;
+            factors[32 + lane] = w;
+            factors[48 + lane] = w * __int_as_float(x[3]) * 0.00390625f;
+          }
+          __syncwarp();
+          uint32_t ph[4], pl[4];
+#pragma unroll
+          for (int j4 = 0; j4 < 4; ++j4) {
+            const float4 f4 = *reinterpret_cast<const float4*>(factors + 4 * j4);
+            const float4 b4 = *reinterpret_cast<const float4*>(factors + 16 + 4 * j4);
+            const float4 w4 = *reinterpret_cast<const float4*>(factors + 32 + 4 * j4);
+            uint32_t hi[2], lo[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int j = 4 * j4 + 2 * i;
+              float2 v = fma2(make_float2(s[j], s[j + 1]), i ? make_float2(f4.z, f4.w) : make_float2(f4.x, f4.y),
+                              i ? make_float2(b4.z, b4.w) : make_float2(b4.x, b4.y));
+              v.x = ex2_approx(v.x);
+              v.y = ex2_approx(v.y);
+              const float2 n = fma2(v, i ? make_float2(w4.z, w4.w) : make_float2(w4.x, w4.y), make_float2(l[j], l[j + 1]));
+              l[j] = n.x;
+              l[j + 1] = n.y;
+              const float2 cut = make_float2(__uint_as_float(__float_as_uint(v.x) & 0xfff00000u),     // four significant bits
+                                             __uint_as_float(__float_as_uint(v.y) & 0xfff00000u));
+              const float2 rest = fma2(v, make_float2(16.f, 16.f), mul2(cut, make_float2(-16.f, -16.f)));
+              hi[i] = e4m3x2(cut.x, cut.y);
+              lo[i] = e4m3x2(rest.x, rest.y);
+            }
+            ph[j4] = __byte_perm(hi[0], hi[1], 0x5410);
+            pl[j4] = __byte_perm(lo[0], lo[1], 0x5410);
+          }
+          unsigned char* to = gbase + C::OFF_P + key * 32;
+          const auto column = [&](int c) { return to + (c >> 5) * 4096 + ((((c >> 4) ^ (key >> 2)) & 1) << 4); };
+          *reinterpret_cast<uint4*>(column(row0)) = make_uint4(ph[0], ph[1], ph[2], ph[3]);
+          *reinterpret_cast<uint4*>(column(R + row0)) = make_uint4(pl[0], pl[1], pl[2], pl[3]);
+          if (valid < 128 && row0 == 0) {
+            // rows behind the sequence may hold anything: they become zeros before the second product reads them
+            const int n = 2 * pages + 1, vslot = n % SLOTS;
+            ok = wait_warp(bar(C::B_FULL + vslot), (n / SLOTS) & 1, guard, 0xc34);
+            if (!ok) break;
+            if (key >= valid) {
+              uint4* v = reinterpret_cast<uint4*>(gbase + C::OFF_RING + vslot * TILE_BYTES + key * 128);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[i] = make_uint4(0, 0, 0, 0);
+            }
+          }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(C::B_P_FULL));
+          pending = pages++;
+          masked = limit < valid;
+          p_row = x[0];
+          p_limit = limit;
+          p_valid = valid;
+          continue;
+        }
+        // the item's end
+        if (item_pages) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(C::B_Q_EMPTY + (items & 1)));
+          ++items;
+        }
+        float* sm = sums + (ends & 1) * C::SOFTMAX_WARPS * 16;
+        const float sum = row_sums(l, lane);
+        if (lane < 16) sm[quarter * 16 + lane] = sum;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(C::B_SUM + 2 * wg + (ends & 1)));
+        ok = wait_warp(bar(C::B_SUM + 2 * wg + (ends & 1)), (ends >> 1) & 1, guard, 0xc35);
+        ++ends;
         if (!ok) break;
-        tc_fence_after();
-        load_sums<R>(tmem + lane_base + b * N + row0, s);
-        tc_fence_before();
-        const bool partial = valid < 128 || limit < 128;
-        if (partial) {
-          // Rows are in token order: those that do not see this key are the first ones.
-          const int first = p.a.causal ? (key - limit + 1) * p.group - row0 : key >= limit ? 16 : 0;
-          const int unseen = key >= valid ? 16 : first;
+        const int token0 = info[0].z, rows = info[0].w * p.group, head = info[1].x, place = info[1].y;
+        // lane r: sum of row r
+        const float sum_row = ((sm[r16] + sm[16 + r16]) + (sm[32 + r16] + sm[48 + r16])) * 0.00390625f;
+        if (place < 0) {
+          const long long first = static_cast<long long>(token0) * p.a.hq + head * p.group;
+          if (lane < 16) factors[lane] = sum_row == 0.f ? 0.f : 1.f / sum_row;
+          __syncwarp();
+          __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.a.out) + first * 128 + key;
+          const int* at = row_out + row0;
 #pragma unroll
           for (int j = 0; j < 16; ++j)
-            if (j < unseen) s[j] = -INFINITY;
-        }
-        // Maxima in bf16: a reference, not a result. Rounded up by what the conversion may have lost they bound every score.
-        uint32_t pairs[8];
+            if (row0 + j < rows) out[at[j]] = __float2bfloat16(acc[j] * factors[j]);
+          if (p.a.lse && quarter == 0 && lane < 16 && row0 + lane < rows)
+            p.a.lse[first + (at[lane] >> 7)] = sum_row == 0.f ? -INFINITY : (m + log2f(sum_row)) * 0.6931471805599453f;
+        } else {
+          float* part = p.part_o + (static_cast<long long>(place) * R + row0) * 128 + key;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) pairs[j] = pack_bf16x2(s[2 * j], s[2 * j + 1]);
-        const uint32_t top = pair_maxima(pairs, lane);
-        if (lane < 8) reinterpret_cast<uint32_t*>(maxima + b * C::SOFTMAX_WARPS * 16 + quarter * 16)[lane] = top;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(C::B_MAX + 2 * wg + b));
-      }
-      // under the other warps' maxima: the output of the page before
-      if (pending >= 0) {
-        add_output();
-        if (!ok) break;
-      }
-      int type = x.x;
-      asm volatile("" : "+r"(type));               // one copy of add_output for all kinds of entries
-      if (type == PAGE) {
-        const int b = pages & 1, valid = x.z;
-        ok = wait_warp(bar(C::B_MAX + 2 * wg + b), (pages >> 1) & 1, guard, 0xc36);
-        if (!ok) break;
-        const __nv_bfloat16* mx = maxima + b * C::SOFTMAX_WARPS * 16 + r16;
-        float top = fmaxf(fmaxf(__bfloat162float(mx[0]), __bfloat162float(mx[16])),
-                          fmaxf(__bfloat162float(mx[32]), __bfloat162float(mx[48])));
-        float f = scale_row * __int_as_float(y.x);
-        if (f == 0.f) f = 1e-37f;                  // hidden keys stay hidden with a scale of 0
-        const bool none = top == -INFINITY;
-        top = fmaf(fabsf(top), 0.00394f, top);     // 2^-8 and a little
-        if (__any_sync(0xffffffffu, fabsf(top * f) > 100.f)) {
-          // Scores so large that this is more than a factor of 1.5: the maxima in fp32. (All four warps of the group are here.)
-          float* exact = reinterpret_cast<float*>(gbase + C::OFF_EXACT) + wg * 64;
-          top = row_maxima(s, lane);
-          if (lane < 16) exact[quarter * 16 + lane] = top;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(C::B_EXACT + wg));
-          ok = wait_warp(bar(C::B_EXACT + wg), exacts++ & 1, guard, 0xc37);
-          if (!ok) break;
-          top = fmaxf(fmaxf(exact[r16], exact[16 + r16]), fmaxf(exact[32 + r16], exact[48 + r16]));
-        }
-        const float mu = none ? -INFINITY : top * f;
-        if (m == -INFINITY) m = mu;
-        // The sums stay relative to the item's first page: fp32 has room for 2^40 above it, and what lies below loses nothing.
-        const bool jump = mu - m > 40.f;
-        if (__any_sync(0xffffffffu, jump)) {
-          if (lane < 16) factors[lane] = jump ? ex2_approx(m - mu) : 1.f;
-          if (jump) m = mu;
-          __syncwarp();
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            acc[j] *= factors[j];
-            l[j] *= factors[j];
-          }
-          __syncwarp();
-        }
-        if (lane < 16) {
-          const float w = none ? 0.f : ex2_approx(mu - m);
-          factors[lane] = f;
-          factors[16 + lane] = none ? 0.f : 8.f - mu;
-          factors[32 + lane] = w;
-          factors[48 + lane] = w * __int_as_float(y.y) * 0.00390625f;
-        }
-        __syncwarp();
-        uint32_t ph[4], pl[4];
-#pragma unroll
-        for (int j4 = 0; j4 < 4; ++j4) {
-          const float4 f4 = *reinterpret_cast<const float4*>(factors + 4 * j4);
-          const float4 b4 = *reinterpret_cast<const float4*>(factors + 16 + 4 * j4);
-          const float4 w4 = *reinterpret_cast<const float4*>(factors + 32 + 4 * j4);
-          uint32_t hi[2], lo[2];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int j = 4 * j4 + 2 * i;
-            float2 v = fma2(make_float2(s[j], s[j + 1]), i ? make_float2(f4.z, f4.w) : make_float2(f4.x, f4.y),
-                            i ? make_float2(b4.z, b4.w) : make_float2(b4.x, b4.y));
-            v.x = ex2_approx(v.x);
-            v.y = ex2_approx(v.y);
-            const float2 n = fma2(v, i ? make_float2(w4.z, w4.w) : make_float2(w4.x, w4.y), make_float2(l[j], l[j + 1]));
-            l[j] = n.x;
-            l[j + 1] = n.y;
-            const float2 cut = make_float2(__uint_as_float(__float_as_uint(v.x) & 0xfff00000u),     // four significant bits
-                                           __uint_as_float(__float_as_uint(v.y) & 0xfff00000u));
-            const float2 rest = fma2(v, make_float2(16.f, 16.f), mul2(cut, make_float2(-16.f, -16.f)));
-            hi[i] = e4m3x2(cut.x, cut.y);
-            lo[i] = e4m3x2(rest.x, rest.y);
-          }
-          ph[j4] = __byte_perm(hi[0], hi[1], 0x5410);
-          pl[j4] = __byte_perm(lo[0], lo[1], 0x5410);
-        }
-        unsigned char* to = gbase + C::OFF_P + key * 32;
-        const auto column = [&](int c) { return to + (c >> 5) * 4096 + ((((c >> 4) ^ (key >> 2)) & 1) << 4); };
-        *reinterpret_cast<uint4*>(column(row0)) = make_uint4(ph[0], ph[1], ph[2], ph[3]);
-        *reinterpret_cast<uint4*>(column(R + row0)) = make_uint4(pl[0], pl[1], pl[2], pl[3]);
-        if (valid < 128 && wg == 0) {
-          // rows behind the sequence may hold anything: they become zeros before the second product reads them
-          const int n = 2 * pages + 1, vslot = n % SLOTS;
-          ok = wait_warp(bar(C::B_FULL + vslot), (n / SLOTS) & 1, guard, 0xc34);
-          if (!ok) break;
-          if (key >= valid) {
-            uint4* v = reinterpret_cast<uint4*>(gbase + C::OFF_RING + vslot * TILE_BYTES + key * 128);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = make_uint4(0, 0, 0, 0);
+          for (int j = 0; j < 16; ++j)
+            if (row0 + j < rows) part[j * 128] = acc[j];
+          if (quarter == 0 && lane < 16)
+            *reinterpret_cast<float2*>(p.part_ml + (static_cast<long long>(place) * R + row0 + lane) * 2) = make_float2(m, sum_row);
+          if (warp == 0 && lane == 0) {
+            int* meta = p.part_meta + 8 * place;
+            *reinterpret_cast<int4*>(meta) = make_int4(1, info[1].z, info[1].w, token0);
+            *reinterpret_cast<int2*>(meta + 4) = make_int2(info[0].w, head);
           }
         }
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(C::B_P_FULL));
-        pending = pages++;
-        masked = x.w < x.z;
-        p_row = x.y;
-        p_limit = x.w;
-        p_valid = x.z;
-        continue;
+        break;
       }
-      // END or EMPTY
-      if (x.x == END) {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(C::B_Q_EMPTY + (items & 1)));
-        ++items;
-      }
-      float* sm = sums + (ends & 1) * C::SOFTMAX_WARPS * 16;
-      const float sum = row_sums(l, lane);
-      if (lane < 16) sm[quarter * 16 + lane] = sum;
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar(C::B_SUM + 2 * wg + (ends & 1)));
-      ok = wait_warp(bar(C::B_SUM + 2 * wg + (ends & 1)), (ends >> 1) & 1, guard, 0xc35);
-      ++ends;
-      if (!ok) break;
-      const int rows = tokens * p.group;
-      // lane r: sum of row r
-      const float sum_row = ((sm[r16] + sm[16 + r16]) + (sm[32 + r16] + sm[48 + r16])) * 0.00390625f;
-      if (place < 0) {
-        const long long first = static_cast<long long>(token0) * p.a.hq + head * p.group;
-        if (lane < 16) factors[lane] = sum_row == 0.f ? 0.f : 1.f / sum_row;
-        __syncwarp();
-        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.a.out) + first * 128 + key;
-        const int* at = row_out + row0;
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (row0 + j < rows) out[at[j]] = __float2bfloat16(acc[j] * factors[j]);
-        if (p.a.lse && quarter == 0 && lane < 16 && row0 + lane < rows)
-          p.a.lse[first + (at[lane] >> 7)] = sum_row == 0.f ? -INFINITY : (m + log2f(sum_row)) * 0.6931471805599453f;
-      } else {
-        float* part = p.part_o + (static_cast<long long>(place) * R + row0) * 128 + key;
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (row0 + j < rows) part[j * 128] = acc[j];
-        if (quarter == 0 && lane < 16)
-          *reinterpret_cast<float2*>(p.part_ml + (static_cast<long long>(place) * R + row0 + lane) * 2) = make_float2(m, sum_row);
-        if (warp == 0 && lane == 0) {
-          int* meta = p.part_meta + 8 * place;
-          *reinterpret_cast<int4*>(meta) = make_int4(1, x0, x1, token0);
-          *reinterpret_cast<int2*>(meta + 4) = make_int2(tokens, head);
-        }
-      }
+      if (lane == 0) mbar_arrive(bar(C::B_INFO_EMPTY + e));
+      ++batches;
     }
   }
   tc_fence_before();
