@@ -788,10 +788,12 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
                             fmaxf(__bfloat162float(mx[32]), __bfloat162float(mx[48])));
           float f = scale_row * __int_as_float(x[2]);
           if (f == 0.f) f = 1e-37f;                  // hidden keys stay hidden with a scale of 0
-          const bool none = top == -INFINITY;
-          top = fmaf(fabsf(top), 0.00394f, top);     // 2^-8 and a little
-          if (__any_sync(0xffffffffu, fabsf(top * f) > 100.f)) {
-            // Scores so large that this is more than a factor of 1.5: the maxima in fp32. (All four warps of the group are here.)
+          const bool none = top == -INFINITY, unset = m == -INFINITY;
+          float mu = none ? -INFINITY : fmaf(fabsf(top), 0.00394f, top) * f;       // 2^-8 and a little
+          // The sums stay relative to the item's first page: fp32 has room for 2^40 above it, and what lies below loses nothing.
+          if (__any_sync(0xffffffffu, !none && (fabsf(mu) > 100.f || (!unset && mu - m > 40.f)))) {
+            // Rare: scores above that, or so large that the rounding up is more than a factor of 1.5. The maxima in fp32; all
+            // four warps of the group are here.
             float* exact = reinterpret_cast<float*>(gbase + C::OFF_EXACT) + wg * 64;
             top = row_maxima(s, lane);
             if (lane < 16) exact[quarter * 16 + lane] = top;
@@ -800,12 +802,8 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
             ok = wait_warp(bar(C::B_EXACT + wg), exacts++ & 1, guard, 0xc37);
             if (!ok) break;
             top = fmaxf(fmaxf(exact[r16], exact[16 + r16]), fmaxf(exact[32 + r16], exact[48 + r16]));
-          }
-          const float mu = none ? -INFINITY : top * f;
-          if (m == -INFINITY) m = mu;
-          // The sums stay relative to the item's first page: fp32 has room for 2^40 above it, and what lies below loses nothing.
-          const bool jump = mu - m > 40.f;
-          if (__any_sync(0xffffffffu, jump)) {
+            if (!none) mu = top * f;
+            const bool jump = !unset && mu - m > 40.f;
             if (lane < 16) factors[lane] = jump ? ex2_approx(m - mu) : 1.f;
             if (jump) m = mu;
             __syncwarp();
@@ -816,6 +814,7 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
             }
             __syncwarp();
           }
+          if (unset) m = mu;
           if (lane < 16) {
             const float w = none ? 0.f : ex2_approx(mu - m);
             factors[lane] = f;
