@@ -24,29 +24,10 @@
 //
 // CTA: R / 16 softmax warpgroups, a loader warp (TMA, one 16 KB tile of K or V to a slot of a ring), an MMA warp, two warps
 // that bring and split the queries of the next item. Entries (start of an item, page, end) go through a ring of their own.
-#include <cuda_bf16.h>
-#include <cuda_fp8.h>
-#include "internal.h"
-#include "paged.cuh"
-#include "ptx.cuh"
+#include "paged_attention.cuh"
 
 namespace sb {
 namespace pa {
-
-constexpr int TILE_BYTES = 128 * 128;
-// What the loader tells the other warps: batches of up to 32 pages of an item. Header (two int4): flags, pages, first token,
-// tokens; KV head, place of the part (-1: the item lies in this share alone), first and last share of the item. Pages (int4
-// each): row of the page in the cache (page * Hkv + head), keys it holds | keys its first token sees << 16, the two scales.
-constexpr int BATCHES = 4, BATCH_BYTES = 32 + 32 * 16;
-constexpr int FIRST = 1, LAST = 2, STOP = 4;      // first batch of an item, last one; there are no more
-
-struct Params {
-  PagedAttentionArgs a;
-  int group, pack, pack_shift, tile_shift, ctas;
-  float* part_o;                                  // [2 ctas, R, 128]
-  float* part_ml;                                 // [2 ctas, R, 2]
-  int* part_meta;                                 // [2 ctas, 8]
-};
 
 template <int R_>
 struct Config {
@@ -55,7 +36,7 @@ struct Config {
   static constexpr int LOADER = SOFTMAX_WARPS, MMA = LOADER + 1, QWARP = MMA + 1, WARPS = QWARP + 2;
   static constexpr int THREADS = 32 * WARPS;
   static constexpr int CTAS = R == 16 ? 2 : 1;    // per SM
-  static constexpr int SLOTS = R == 16 ? 5 : R == 32 ? 11 : 9;
+  static constexpr int SLOTS = R == 16 ? 5 : 11;
   static constexpr int OFF_RING = 0;
   static constexpr int OFF_Q = OFF_RING + SLOTS * TILE_BYTES;       // two buffers of N rows of 128 bytes
   static constexpr int OFF_P = OFF_Q + 2 * N * 128;                 // 128 keys x N columns
@@ -108,11 +89,6 @@ __device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
                : "r"(taddr)
                : "memory");
 }
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 d;
-  f32x2_unpack(f32x2_mul(f32x2_pack(a.x, a.y), f32x2_pack(b.x, b.y)), d.x, d.y);
-  return d;
-}
 // Sums over the warp of 16 values: lane l gets that of value l % 16. Every step halves the values that a lane holds: 16
 // shuffles in all.
 __device__ __forceinline__ float row_sums(const float (&s)[16], int lane) {
@@ -162,15 +138,6 @@ __device__ __forceinline__ uint32_t pair_maxima(const uint32_t (&s)[8], int lane
   d = max_bf16x2(d, __shfl_xor_sync(0xffffffffu, d, 8));
   return max_bf16x2(d, __shfl_xor_sync(0xffffffffu, d, 16));
 }
-// A wait by a whole converged warp whose slow part is not in line: a role's loop has to fit the instruction caches beside the
-// others' (the first build of this kernel had 164 KB of code and ran at a fifth of its speed).
-__device__ __noinline__ bool wait_longer(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
-  return mbar_wait_warp(bar, parity, Guard{abort_flag, status}, code);
-}
-__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, const Guard& g, int code) {
-  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-  return wait_longer(bar, parity, g.abort_flag, g.status, code);
-}
 __device__ __noinline__ bool load_tile(uint32_t full, uint32_t empty, uint32_t parity, uint32_t to, const CUtensorMap* map, int row,
                                        volatile int* flag_at, int flag, volatile int* abort_flag, int* status) {
   if (!mbar_wait_warp(empty, parity, Guard{abort_flag, status}, 0xc01)) return false;
@@ -186,17 +153,9 @@ __device__ __noinline__ bool load_tile(uint32_t full, uint32_t empty, uint32_t p
   __syncwarp();
   return true;
 }
-__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
-__device__ __forceinline__ float2 from_e4m3x2(uint32_t codes) {
-  return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(codes), __NV_E4M3)));
-}
-__device__ __forceinline__ float from_e4m3(uint32_t code) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(code), __NV_E4M3)));
-}
-
 // hi + lo / 16 of 16 rows from tensor memory, eight at a time (registers)
 template <int R>
 __device__ __forceinline__ void load_sums(uint32_t at, float (&x)[16]) {
@@ -235,44 +194,6 @@ __device__ __noinline__ void visible_sums(float* o, const unsigned char* pr, con
   }
 }
 
-// ------------------------------------------------------------------ the work of a request
-struct Request {
-  int begin, n, k_len, held, tiles;
-  __device__ __forceinline__ void set(const Params& p, int cu0, int cu1, int seq) {
-    begin = min(max(cu0, 0), p.a.total_q);
-    n = max(min(max(cu1, 0), p.a.total_q) - begin, 0);
-    k_len = max(seq, 0);
-    held = min((k_len >> 7) + ((k_len & 127) != 0), p.a.width);
-    tiles = static_cast<int>((static_cast<long long>(n) + p.pack - 1) >> p.pack_shift);
-  }
-};
-// Pages of the first `tiles` tiles of a request: a list's length each, or the pages that a tile's last token sees (one at
-// least, so that every item has a place): min(held, ceil((k - n + (i + 1) pack) / 128)) summed over i. With pack = 128 / m the
-// ceiling is floor((first + i) / m), whose sums have a closed form.
-__device__ __noinline__ long long pages_before(int topk, int causal, int shift, int k_len, int n, int held, int tiles) {
-  if (topk) return static_cast<long long>(tiles) * topk;
-  const long long most = max(held, 1);
-  if (!causal) return tiles * most;
-  const int mshift = 7 - shift, m = 1 << mshift;
-  const long long first = ((static_cast<long long>(k_len) - n + 127) >> shift) + 1;
-  const auto clamp = [&](long long x) { return x < 0 ? 0 : x > tiles ? tiles : x; };
-  const long long ones = clamp(m - first), full = max(clamp(most * m - first), ones);
-  const auto sum = [&](long long x) {             // sum of floor(t / m) over 0 <= t < x
-    const long long q = x >> mshift, rest = x & (m - 1);
-    return m * (q * (q - 1) / 2) + rest * q;
-  };
-  const long long middle = full > ones ? sum(first + full) - sum(first + ones) : 0;
-  return ones + middle + (tiles - full) * most;
-}
-__device__ __forceinline__ long long pages_before(const Params& p, const Request& r, int tiles) {
-  return pages_before(p.a.topk, p.a.causal, p.pack_shift, r.k_len, r.n, r.held, tiles);
-}
-__device__ __forceinline__ long long pages_of_request(const Params& p, int r) {
-  Request q;
-  q.set(p, __ldg(p.a.cu_q + r), __ldg(p.a.cu_q + r + 1), __ldg(p.a.seq + r));
-  return pages_before(p, q, q.tiles);
-}
-
 // ------------------------------------------------------------------ kernel
 template <int R_>
 __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
@@ -287,8 +208,6 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Guard guard{misc + 1, status};
   const auto bar = [&](int i) { return base + C::OFF_BAR + 8 * i; };
-  __shared__ long long s_scan[C::WARPS];
-  __shared__ long long s_place[2];                // unit within the request, request
 
   if (tid == 0) {
     misc[1] = 0;
@@ -328,47 +247,9 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
     prefetch_tmap(&k_map);
     prefetch_tmap(&v_map);
   }
-  // The share of this CTA: a scan over the requests' pages.
-  const int each = (p.a.batch + C::THREADS - 1) / C::THREADS;
-  const int lo = min(tid * each, p.a.batch), hi = min(lo + each, p.a.batch);
-  long long mine = 0;
-#pragma unroll 1
-  for (int r = lo; r < hi; ++r) mine += pages_of_request(p, r);
-  long long upto = mine;
-  for (int by = 1; by < 32; by <<= 1) {
-    const long long x = __shfl_up_sync(0xffffffffu, upto, by);
-    if (lane >= by) upto += x;
-  }
-  if (lane == 31) s_scan[warp] = upto;
   tc_fence_before();
-  __syncthreads();
+  const Share share = find_share<C::WARPS>(p);     // (two barriers of the CTA)
   tc_fence_after();
-  long long per_head = 0;
-  upto -= mine;
-  for (int w = 0; w < C::WARPS; ++w) {
-    if (w < warp) upto += s_scan[w];
-    per_head += s_scan[w];
-  }
-  const long long total = per_head * p.a.hkv;
-  const long long share = max((total + p.ctas - 1) / p.ctas, 1LL);
-  const long long unit0 = blockIdx.x * share, unit1 = min(unit0 + share, total);
-  const int head0 = unit0 < total ? static_cast<int>(unit0 / per_head) : 0;
-  if (unit0 < total) {
-    long long at = unit0 - head0 * per_head - upto;
-    if (at >= 0 && at < mine) {
-#pragma unroll 1
-      for (int r = lo; r < hi; ++r) {
-        const long long w = pages_of_request(p, r);
-        if (at < w) {
-          s_place[0] = at;
-          s_place[1] = r;
-          break;
-        }
-        at -= w;
-      }
-    }
-  }
-  __syncthreads();
   const uint32_t tmem = static_cast<uint32_t>(misc[0]);
   uint32_t fills = 0;
 
@@ -393,112 +274,36 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
       ok = ok && wait_warp(bar(C::B_INFO_EMPTY + e), ((batches / BATCHES) & 1) ^ 1, guard, 0xc00);
       return reinterpret_cast<int4*>(gbase + C::OFF_INFO + e * BATCH_BYTES);
     };
-    const auto post = [&](int4* to, int flags, int pages, int token0, int tokens, int4 item) {
-      if (lane == 0 && ok) {
-        to[0] = make_int4(flags, pages, token0, tokens);
-        to[1] = item;
+    bool started = false;
+    walk_share(p, share, ok, [&](const Item& item, int flags, uint32_t pages, int row, int j) {
+      if (flags & FIRST) started = false;
+      uint32_t todo = pages;
+#pragma unroll 1
+      for (bool told = false; ok && (todo || !told);) {
+        if (todo) {
+          const int next = __shfl_sync(0xffffffffu, row, __ffs(todo) - 1) * 128;
+          todo &= todo - 1;
+          load(&k_map, next, started ? 0 : 1);
+          load(&v_map, next, 0);
+          started = true;
+        }
+        if (told) continue;
+        told = true;                               // behind the first page's tiles: the scales have to be fetched
+        int4* to = batch();
+        if (!ok) break;
+        write_batch(p, to, item, flags, pages, row, j);
+        if (lane == 0) mbar_arrive(bar(C::B_INFO_FULL + batches % BATCHES));
+        ++batches;
+      }
+    });
+    int4* to = batch();
+    if (ok) {
+      if (lane == 0) {
+        to[0] = make_int4(STOP, 0, 0, 0);
+        mbar_arrive(bar(C::B_INFO_FULL + batches % BATCHES));
       }
       __syncwarp();
-      if (lane == 0 && ok) mbar_arrive(bar(C::B_INFO_FULL + batches % BATCHES));
-      ++batches;
-    };
-    if (unit0 < total) {
-      long long left = unit1 - unit0;
-      int head = head0, r = static_cast<int>(s_place[1]), tile;
-      long long off = s_place[0];
-      // requests come 32 at a time, one per lane
-      int block = -1, c0 = 0, c1 = 0, sq = 0;
-      Request q;
-      const auto fetch = [&](int want) {
-        if (want >> 5 != block) {
-          block = want >> 5;
-          const int i = block * 32 + lane;
-          const bool in = i < p.a.batch;
-          c0 = in ? __ldg(p.a.cu_q + i) : 0;
-          c1 = in ? __ldg(p.a.cu_q + i + 1) : 0;
-          sq = in ? __ldg(p.a.seq + i) : 0;
-        }
-        q.set(p, __shfl_sync(0xffffffffu, c0, want & 31), __shfl_sync(0xffffffffu, c1, want & 31),
-              __shfl_sync(0xffffffffu, sq, want & 31));
-      };
-      fetch(r);
-      tile = warp_last_at_most(q.tiles, off, [&](int t) { return pages_before(p, q, t); });
-      off -= pages_before(p, q, tile);
-      long long start = unit0 - off;               // first unit of the item
-      while (ok && left > 0) {
-        const int token0 = tile * p.pack, tokens = min(p.pack, q.n - token0);
-        const long long seen0 = p.a.causal ? static_cast<long long>(q.k_len) - q.n + token0 + 1 : q.k_len;   // keys of token 0
-        const long long seen = p.a.causal ? seen0 + tokens - 1 : q.k_len;
-        const int count = static_cast<int>(pages_before(p, q, tile + 1) - pages_before(p, q, tile));
-        const int from = static_cast<int>(off), to = static_cast<int>(min(static_cast<long long>(count), off + left));
-        const int x0 = static_cast<int>(start / share), x1 = static_cast<int>((start + count - 1) / share);
-        const int place = x0 == x1 ? -1 : 2 * static_cast<int>(blockIdx.x) + (x0 == static_cast<int>(blockIdx.x));
-        bool posted = false, started = false;
-        const int32_t* list = nullptr;
-        if (p.a.ids) {
-          const int s = p.tile_shift;
-          const long long lists = s ? (p.a.total_q >> s) + p.a.batch : p.a.total_q;
-          list = p.a.ids + (head * lists + (q.begin >> s) + (s ? r : 0) + (token0 >> s)) * p.a.topk;
-        }
-        const int32_t* table = p.a.table + r * p.a.table_stride;
-#pragma unroll 1
-        for (int at = from; ok && at < to; at += 32) {
-          int j = at + lane;
-          bool live = j < to;
-          if (live && list) j = __ldg(list + j);
-          live = live && j >= 0 && j < q.held && j * 128LL < seen;
-          int row = 0;
-          if (live) {
-            const int page = __ldg(table + j);
-            live = page >= 0 && page < p.a.pages;
-            row = live ? page * p.a.hkv + head : 0;
-          }
-          const uint32_t pages = __ballot_sync(0xffffffffu, live);
-          const bool last = at + 32 >= to;
-          if (!pages && !last) continue;
-          uint32_t todo = pages;
-          const auto load_next = [&]() {
-            const int next = __shfl_sync(0xffffffffu, row, __ffs(todo) - 1) * 128;
-            todo &= todo - 1;
-            load(&k_map, next, started ? 0 : 1);
-            load(&v_map, next, 0);
-            started = true;
-          };
-          int4* to_batch = nullptr;
-#pragma unroll 1
-          for (bool told = false; ok && (todo || !told);) {
-            if (todo) load_next();
-            if (told) continue;
-            // behind the first page's tiles: the scales have to be fetched
-            told = true;
-            to_batch = batch();
-            if (live && ok) {
-              const int valid = static_cast<int>(min(128LL, q.k_len - j * 128LL));
-              // keys of the page that the first token sees; the others one more each. Not causal: all see the same.
-              const int limit = static_cast<int>(max(-128LL, min(128LL, seen0 - j * 128LL)));
-              to_batch[2 + __popc(pages & ((1u << lane) - 1))] =
-                  make_int4(row, valid | (limit << 16), __float_as_int(__ldg(p.a.k_scale + row)), __float_as_int(__ldg(p.a.v_scale + row)));
-            }
-            post(to_batch, (posted ? 0 : FIRST) | (last ? LAST : 0), __popc(pages), q.begin + token0, tokens, make_int4(head, place, x0, x1));
-            posted = true;
-          }
-        }
-        left -= to - from;
-        start += count;
-        off = 0;
-        if (++tile >= q.tiles && left > 0) {       // the next request that has tokens; behind the last one the next head
-          tile = 0;
-          do {
-            if (++r == p.a.batch) {
-              r = 0;
-              ++head;
-            }
-            fetch(r);
-          } while (q.tiles == 0);
-        }
-      }
     }
-    post(batch(), STOP, 0, 0, 0, make_int4(0, 0, 0, 0));
     load(&k_map, 0, 2);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   } else if (warp == C::MMA) {
@@ -941,7 +746,6 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
 // a few more, which is the kernel's time. (Rows one after another by the CTA of the border: 130 us of the 217 of a batch of
 // speculated tokens, 75 of the 293 of a decode batch over 1.4 GB.)
 constexpr int MERGE_WARPS = 8, FEW = 16;
-template <int R>
 __global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const Params p) {
   __shared__ float s_top[MERGE_WARPS], s_l[MERGE_WARPS];
   __shared__ float s_acc[MERGE_WARPS][32];
@@ -953,7 +757,7 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const Par
   const int2 more = *reinterpret_cast<const int2*>(p.part_meta + 16 * x + 4);
   const int x0 = meta.y, parts = meta.z - x0 + 1, token0 = meta.w, rows = more.x * p.group, head = more.y;
   const int cta = (x - x0 - 1) * gridDim.y + blockIdx.y, ctas = (parts - 1) * gridDim.y;
-  const auto part_row = [&](int i, int row) { return static_cast<long long>(2 * (x0 + i) + (i == 0)) * R + row; };
+  const auto part_row = [&](int i, int row) { return static_cast<long long>(2 * (x0 + i) + (i == 0)) * p.rows + row; };
   const auto out_row = [&](int row) {
     const int token = row / p.group;
     return (static_cast<long long>(token0) + token) * p.a.hq + head * p.group + (row - token * p.group);
@@ -1041,25 +845,23 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const Par
   }
 }
 
-// Tokens that share a pass over the pages: as many as 64 rows hold, a power of two, no more than there are.
+// Tokens that share a pass over the pages: as many as 128 rows hold, a power of two, no more than there are.
 static int pack_of(int group, int tile, int max_q, bool listed) {
   int pack = 1;
-  while (2 * pack * group <= 64 && pack < max_q && (!listed || 2 * pack <= tile)) pack *= 2;
+  while (2 * pack * group <= WIDE_ROWS && pack < max_q && (!listed || 2 * pack <= tile)) pack *= 2;
   return pack;
 }
-static int rows_of(int group, int pack) { return pack * group <= 16 ? 16 : pack * group <= 32 ? 32 : 64; }
+// Rows of an item at most. The kernels for 16 and 32 rows have keys on the M dimension and multiply the codes as they are: what
+// they pay for a page grows with the rows. The wide kernel converts a page to f16 first, always for 128 rows. Measured: 4 heads
+// and up to 8 new tokens, 32 rows (32 requests of up to 8192 keys, 8 KV heads): 77 us here, 130 us there; lists of tiles of 16
+// tokens, 16 heads (4 prompts of 512 to 1024 tokens, 16 pages a list): 181 us as items of 64 rows here, 128 us as 128 rows there.
+static int rows_of(int used) { return used <= 16 ? 16 : used <= 32 ? 32 : WIDE_ROWS; }
+static int ctas_of(int rows, int sm_count) { return sm_count * (rows == 16 ? Config<16>::CTAS : rows == 32 ? Config<32>::CTAS : WIDE_CTAS); }
 
 template <int R>
-static int launch(const PagedAttentionArgs& a, int pack, DeviceCtx* ctx, int slot, cudaStream_t stream) {
+static int launch_narrow(const Params& p, DeviceCtx* ctx, cudaStream_t stream) {
   using C = Config<R>;
-  Params p{a, a.hq / a.hkv, pack, 0, 0, ctx->sm_count * C::CTAS, nullptr, nullptr, nullptr};
-  while ((1 << p.pack_shift) < pack) ++p.pack_shift;
-  while (a.ids && (1 << p.tile_shift) < a.tile) ++p.tile_shift;
-  if (!a.ids) p.a.topk = 0;
-  unsigned char* ws = static_cast<unsigned char*>(a.workspace);
-  p.part_o = reinterpret_cast<float*>(ws);
-  p.part_ml = p.part_o + static_cast<long long>(2) * p.ctas * R * 128;
-  p.part_meta = reinterpret_cast<int*>(p.part_ml + static_cast<long long>(2) * p.ctas * R * 2);
+  const PagedAttentionArgs& a = p.a;
   CUtensorMap km, vm;
   const cuuint64_t dims[2] = {128, static_cast<cuuint64_t>(a.pages) * a.hkv * 128};
   const cuuint64_t strides[1] = {128};
@@ -1068,44 +870,51 @@ static int launch(const PagedAttentionArgs& a, int pack, DeviceCtx* ctx, int slo
     if (encode_tiled(i ? &vm : &km, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(i ? a.v : a.k), dims, strides, box, steps,
                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B))
       return set_error(SB_ERR_CUDA, "tensor map of the cache pages");
-  auto kernel = paged_attention_kernel<R>;
-  if (!ctx->paged_attr[slot]) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
+  constexpr int KERNEL = R == 16 ? 4 : 6;
+  if (!ctx->paged_attr[KERNEL]) {
+    if (cudaFuncSetAttribute(paged_attention_kernel<R>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
       return set_error(SB_ERR_CUDA, "shared memory of the paged attention");
-    ctx->paged_attr[slot] = 1;
+    ctx->paged_attr[KERNEL] = 1;
   }
-  kernel<<<p.ctas, C::THREADS, C::SMEM, stream>>>(km, vm, p, ctx->status);
-  int rc = check_kernel_launch();
-  if (rc) return rc;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.ctas - 1, R / 16);
-  cfg.blockDim = dim3(32 * MERGE_WARPS);
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_merge_kernel<R>, p);
-  return e == cudaSuccess ? SB_OK : set_error(SB_ERR_CUDA, cudaGetErrorString(e));
+  paged_attention_kernel<R><<<p.ctas, C::THREADS, C::SMEM, stream>>>(km, vm, p, ctx->status);
+  return check_kernel_launch();
 }
 
 }  // namespace pa
 
 long long paged_attention_workspace_bytes(int hq, int hkv, int tile, int max_q, bool listed, int sm_count) {
-  const int rows = pa::rows_of(hq / hkv, pa::pack_of(hq / hkv, tile, max_q, listed));
-  const long long ctas = static_cast<long long>(sm_count) * (rows == 16 ? pa::Config<16>::CTAS : pa::Config<64>::CTAS);
-  return 2 * ctas * (rows * 130 * 4LL + 32);
+  const int group = hq / hkv, rows = pa::rows_of(pa::pack_of(group, tile, max_q, listed) * group);
+  return 2LL * pa::ctas_of(rows, sm_count) * (rows * 130 * 4LL + 32);
 }
 
 int launch_paged_attention(const PagedAttentionArgs& a, cudaStream_t stream) {
+  using namespace pa;
   DeviceCtx* ctx = device_ctx();
   if (!ctx) return SB_ERR_CUDA;
-  const int group = a.hq / a.hkv, pack = pa::pack_of(group, a.tile, a.max_q, a.ids != nullptr), rows = pa::rows_of(group, pack);
   if (!a.workspace || a.workspace_bytes < paged_attention_workspace_bytes(a.hq, a.hkv, a.tile, a.max_q, a.ids != nullptr, ctx->sm_count))
     return set_error(SB_ERR_INVALID, "workspace too small (see sparse_b200_paged_attention_workspace_bytes)");
-  return rows == 16 ? pa::launch<16>(a, pack, ctx, 4, stream)
-                    : rows == 32 ? pa::launch<32>(a, pack, ctx, 5, stream) : pa::launch<64>(a, pack, ctx, 6, stream);
+  const int group = a.hq / a.hkv, pack = pack_of(group, a.tile, a.max_q, a.ids != nullptr), rows = rows_of(pack * group);
+  Params p{a, group, pack, 0, 0, ctas_of(rows, ctx->sm_count), rows, nullptr, nullptr, nullptr};
+  while ((1 << p.pack_shift) < pack) ++p.pack_shift;
+  while (a.ids && (1 << p.tile_shift) < a.tile) ++p.tile_shift;
+  if (!a.ids) p.a.topk = 0;
+  p.part_o = static_cast<float*>(a.workspace);
+  p.part_ml = p.part_o + 2LL * p.ctas * rows * 128;
+  p.part_meta = reinterpret_cast<int*>(p.part_ml + 2LL * p.ctas * rows * 2);
+  const int rc = rows == 16 ? launch_narrow<16>(p, ctx, stream)
+                 : rows == 32 ? launch_narrow<32>(p, ctx, stream) : launch_paged_wide(p, ctx->status, ctx, stream);
+  if (rc) return rc;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(p.ctas - 1, rows / 16);
+  cfg.blockDim = dim3(32 * MERGE_WARPS);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_merge_kernel, p);
+  return e == cudaSuccess ? SB_OK : set_error(SB_ERR_CUDA, cudaGetErrorString(e));
 }
 
 }  // namespace sb
