@@ -14,19 +14,20 @@
 // warps. (One thread a row, two passes over S and two CTAs to an SM took 6500 cycles a step; the narrow kernel's threads own
 // keys, and a step of 64 rows took it 3300.)
 //
-// CTA (one to an SM): eight softmax warps; eight that convert a page's codes from a ring in shared memory; an MMA warp, which
-// issues QK of a page ahead of PV of the page before; a warp that walks over the share's pages and brings them (bulk copies, a
-// tile of K or V is 16 KB in a row); two that bring and scale the queries of the next item.
+// CTA (one to an SM): eight softmax warps; eight that scale an item's queries and convert a page's codes
+// from a ring in shared memory; an MMA warp, which
+// issues QK of a page ahead of PV of the page before; a warp that walks over the share's pages and one that brings them (bulk
+// copies, a tile of K or V is 16 KB in a row).
 #include "paged_attention.cuh"
 
 namespace sb {
 namespace pa {
 namespace {
 
-constexpr int CONVERT = 8, MMA = 16, WALK = 17, QUERY = 18, WARPS = 20, THREADS = 32 * WARPS;
+constexpr int CONVERT = 8, MMA = 16, WALK = 17, LOAD = 18, WARPS = 19, THREADS = 32 * WARPS;
 constexpr int HALF_TILE = 128 * 256;              // 128 rows of 128 f16: two panels of 64 features, 128-byte swizzle
-constexpr int SLOTS = 5;
-constexpr int OFF_Q = 0, OFF_K = 2 * HALF_TILE, OFF_V = OFF_K + HALF_TILE, OFF_RING = OFF_V + HALF_TILE;
+constexpr int SLOTS = 7;
+constexpr int OFF_Q = 0, OFF_K = HALF_TILE, OFF_V = OFF_K + HALF_TILE, OFF_RING = OFF_V + HALF_TILE;
 constexpr int OFF_NAN = OFF_RING + SLOTS * TILE_BYTES;             // int [4][128]: by item, first key whose value has a NaN at a feature
 constexpr int OFF_QF = OFF_NAN + 4 * 512;         // float [2][128]: what a row's scores are multiplied by
 constexpr int OFF_MAX = OFF_QF + 2 * 512;         // float [2][2][128]: by page, half and row
@@ -35,7 +36,7 @@ constexpr int OFF_INFO = OFF_SUM + 4 * 512;
 constexpr int OFF_BAR = OFF_INFO + BATCHES * BATCH_BYTES;
 constexpr int B_INFO_FULL = 0, B_INFO_EMPTY = BATCHES, B_FULL = 2 * BATCHES, B_EMPTY = B_FULL + SLOTS, B_K_FULL = B_EMPTY + SLOTS,
               B_K_EMPTY = B_K_FULL + 1, B_V_FULL = B_K_EMPTY + 1, B_V_EMPTY = B_V_FULL + 2, B_S_FULL = B_V_EMPTY + 2,
-              B_P_FULL = B_S_FULL + 2, B_Q_FULL = B_P_FULL + 2, B_Q_EMPTY = B_Q_FULL + 2, B_MAX = B_Q_EMPTY + 2, B_SUM = B_MAX + 8,
+              B_P_FULL = B_S_FULL + 2, B_Q_FULL = B_P_FULL + 2, B_MAX = B_Q_FULL + 2, B_SUM = B_MAX + 8,
               B_DONE = B_SUM + 4, BARS = B_DONE + 1;
 constexpr int OFF_FLAG = OFF_BAR + BARS * 8;      // int [2]: for the MMA warp, with a page's K tile: 1 = the first of an item, 2 = stop
 constexpr int OFF_MISC = (OFF_FLAG + 8 + 15) / 16 * 16;
@@ -105,7 +106,7 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
       for (int i = first; i < first + n; ++i) mbar_init(bar(i), count);
     };
     init(B_INFO_FULL, BATCHES, 1);
-    init(B_INFO_EMPTY, BATCHES, 18);              // softmax, conversion, queries
+    init(B_INFO_EMPTY, BATCHES, 17);              // softmax, conversion, loads
     init(B_FULL, SLOTS, 1);
     init(B_EMPTY, SLOTS, 8);
     init(B_K_FULL, 1, 8);
@@ -114,8 +115,7 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
     init(B_V_EMPTY, 2, 1);
     init(B_S_FULL, 2, 1);
     init(B_P_FULL, 2, 8);                         // by page: a warp may be a page ahead of another
-    init(B_Q_FULL, 2, 2);
-    init(B_Q_EMPTY, 2, 8);
+    init(B_Q_FULL, 2, 8);
     init(B_MAX, 12, 2);
     init(B_DONE, 1, 1);
     fence_mbar_init();
@@ -133,12 +133,35 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
   uint32_t fills = 0;
 
   if (warp == WALK) {
-    // --------------------------------------------------------------- the share's pages
+    // --------------------------------------------------------------- the share's pages, told as far ahead as there is place
+    bool ok = true;
+    uint32_t batches = 0;
+    const auto next = [&]() {
+      const uint32_t e = batches % BATCHES;
+      ok = ok && wait_warp(bar(B_INFO_EMPTY + e), ((batches / BATCHES) & 1) ^ 1, guard, 0xd00);
+      return batch_at(e);
+    };
+    walk_share(p, share, ok, [&](const Item& item, int flags, uint32_t pages, int row, int j) {
+      int4* to = next();
+      if (!ok) return;
+      write_batch(p, to, item, flags, pages, row, j);
+      if (lane == 0) mbar_arrive(bar(B_INFO_FULL + batches % BATCHES));
+      ++batches;
+    });
+    int4* to = next();
+    if (ok && lane == 0) {
+      to[0] = make_int4(STOP, 0, 0, 0);
+      mbar_arrive(bar(B_INFO_FULL + batches % BATCHES));
+    }
+    __syncwarp();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  } else if (warp == LOAD) {
+    // --------------------------------------------------------------- their tiles
     bool ok = true;
     uint32_t batches = 0;
     int slot = 0, phase = 0;
     const auto load = [&](const void* cache, int row) {
-      ok = ok && wait_warp(bar(B_EMPTY + slot), phase ^ 1, guard, 0xd01);
+      ok = ok && wait_warp(bar(B_EMPTY + slot), phase ^ 1, guard, 0xd02);
       if (!ok) return;
       if (elect_one()) {
         mbar_expect_tx(bar(B_FULL + slot), TILE_BYTES);
@@ -152,43 +175,25 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
         phase ^= 1;
       }
     };
-    const auto next = [&]() {
+    int behind = -1;                              // page whose V is still to come: it follows the next page's K, within an item
+    while (ok) {
       const uint32_t e = batches % BATCHES;
-      ok = ok && wait_warp(bar(B_INFO_EMPTY + e), ((batches / BATCHES) & 1) ^ 1, guard, 0xd00);
-      return batch_at(e);
-    };
-    int behind = -1;                              // page whose V is still to come: it follows the next page's K
-    walk_share(p, share, ok, [&](const Item& item, int flags, uint32_t pages, int row, int j) {
-      uint32_t todo = pages;
+      ok = wait_warp(bar(B_INFO_FULL + e), (batches / BATCHES) & 1, guard, 0xd01);
+      if (!ok) break;
+      const int4* info = batch_at(e);
+      const int flags = info[0].x, count = info[0].y;
+      if (flags & STOP) break;
 #pragma unroll 1
-      for (bool told = false; ok;) {
-        const int next_row = todo ? __shfl_sync(0xffffffffu, row, __ffs(todo) - 1) : -1;
-        const bool ends = !todo && (flags & LAST);
-        if (todo) load(p.a.k, next_row);
-        if (behind >= 0 && (todo || ends)) load(p.a.v, behind);
-        if (todo || ends) behind = next_row;
-        const bool more = todo != 0;
-        todo &= todo - 1;
-        if (told) {
-          if (!more) break;
-          continue;
-        }
-        told = true;                              // behind the first page's tiles: the scales have to be fetched
-        int4* to = next();
-        if (!ok) break;
-        write_batch(p, to, item, flags, pages, row, j);
-        if (lane == 0) mbar_arrive(bar(B_INFO_FULL + batches % BATCHES));
-        ++batches;
-        if (!more) break;
+      for (int step = 0; ok && step < count + (flags & LAST ? 1 : 0); ++step) {
+        const int row = step < count ? info[2 + step].x : -1;
+        if (row >= 0) load(p.a.k, row);
+        if (behind >= 0) load(p.a.v, behind);
+        behind = row;
       }
-    });
-    int4* to = next();
-    if (ok && lane == 0) {
-      to[0] = make_int4(STOP, 0, 0, 0);
-      mbar_arrive(bar(B_INFO_FULL + batches % BATCHES));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(B_INFO_EMPTY + e));
+      ++batches;
     }
-    __syncwarp();
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   } else if (warp == MMA) {
     // --------------------------------------------------------------- MMA issuer
     // QK of a page overwrites the S that the PV of the page before the last has read P from: it is issued behind that. The O of
@@ -222,7 +227,7 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
           else fresh0 = fresh;
           tc_fence_after();
           if (elect_one()) {
-            const uint32_t q = (base + OFF_Q + (item & 1) * HALF_TILE) >> 4, k = (base + OFF_K) >> 4;
+            const uint32_t q = (base + OFF_Q) >> 4, k = (base + OFF_K) >> 4;
 #pragma unroll
             for (int kk = 0; kk < 8; ++kk) {
               const uint32_t at = (kk >> 2) * (HALF_TILE / 2 >> 4) + (kk & 3) * 2;
@@ -265,67 +270,11 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
     if (elect_one()) tc_commit(bar(B_DONE));
     __syncwarp();
     mbar_wait_drain(bar(B_DONE), 0);
-  } else if (warp >= QUERY) {
-    // --------------------------------------------------------------- queries of the next item
-    const int group_inverse = (65535 + p.group) / p.group;        // row / group = row * this >> 16 for rows below 128
-    const float sign = p.a.scale < 0.f ? -1.f : 1.f, factor = fabsf(p.a.scale) * 1.4426950408889634f;
-    bool ok = true;
-    uint32_t batches = 0;
-    int item = -1;
-    while (ok) {
-      const uint32_t e = batches % BATCHES;
-      ok = wait_warp(bar(B_INFO_FULL + e), (batches / BATCHES) & 1, guard, 0xd40);
-      if (!ok) break;
-      const int4 what = batch_at(e)[0];
-      const int head = batch_at(e)[1].x;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(B_INFO_EMPTY + e));
-      ++batches;
-      if (what.x & STOP) break;
-      if (!(what.x & FIRST) || what.y == 0) continue;
-      ++item;
-      ok = wait_warp(bar(B_Q_EMPTY + (item & 1)), ((item >> 1) & 1) ^ 1, guard, 0xd41);
-      if (!ok) break;
-      const int rows = what.w * p.group;
-      const int part = lane & 15, second = lane >> 4;             // half a warp to a row, 8 features to a thread
-      unsigned char* tile = gbase + OFF_Q + (item & 1) * HALF_TILE + (part >> 3) * (HALF_TILE / 2);
-      float* qf = reinterpret_cast<float*>(gbase + OFF_QF) + (item & 1) * 128;
-      const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.a.q) + what.z * p.a.q_token +
-                                 static_cast<long long>(head) * p.group * p.a.q_head + part * 8;
-      // A thread's pieces come to the places they keep, all in flight at once, and are scaled there. Short loops: code that runs
-      // once an item is not in the instruction caches (eight rows unrolled took 30000 cycles, an item of 16 pages 55000).
-      const auto piece = [&](int row) { return tile + row * 128 + (((part & 7) ^ (row & 7)) << 4); };
-#pragma unroll 1
-      for (int row = (warp - QUERY) * 2 + second; row < 128; row += 4) {
-        const int token = row * group_inverse >> 16, g = row - token * p.group;
-        const bool in = row < rows;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(piece(row))),
-                     "l"(in ? src + token * p.a.q_token + g * p.a.q_head : src), "r"(in ? 16 : 0)
-                     : "memory");
-      }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-#pragma unroll 2
-      for (int row = (warp - QUERY) * 2 + second; row < 128; row += 4) {
-        const uint4 w = *reinterpret_cast<const uint4*>(piece(row));
-        const uint32_t m = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
-        const uint32_t top = __reduce_max_sync(second ? 0xffff0000u : 0xffffu, max(m & 0xffffu, m >> 16));
-        const bool odd = top >= 0x7f80u;          // infinities and NaN: the row ends as NaN
-        const int ex = top == 0 || odd ? 0 : min(134 - static_cast<int>(top >> 7), 126);
-        const float by = odd ? __int_as_float(0x7fffffff) : power_of_two(ex) * sign;
-        const auto scaled = [&](uint32_t pair) {
-          const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&pair));
-          return pack_half2(x.x * by, x.y * by);
-        };
-        *reinterpret_cast<uint4*>(piece(row)) = make_uint4(scaled(w.x), scaled(w.y), scaled(w.z), scaled(w.w));
-        if (part == 0) qf[row] = factor * power_of_two(-ex);
-      }
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(B_Q_FULL + (item & 1)));
-    }
   } else if (warp >= CONVERT) {
     // --------------------------------------------------------------- pages into f16 tiles
     const int t = tid - 32 * CONVERT;
+    const int group_inverse = (65535 + p.group) / p.group;        // row / group = row * this >> 16 for rows below 128
+    const float sign = p.a.scale < 0.f ? -1.f : 1.f, factor = fabsf(p.a.scale) * 1.4426950408889634f;
     bool ok = true, started = false;
     uint32_t batches = 0;
     int item = -1, pages = 0, values = 0, slot = 0, phase = 0;       // tiles of K and of V done
@@ -361,6 +310,45 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
       if (count && !started) {
         ++item;
         if (t < 128) nan_at[(item & 3) * 128 + t] = 0x7fffffff;    // (read for the last time items ago)
+        // The item's queries: half a warp to a row, 8 features to a thread. A thread's pieces come to the places they keep, all
+        // in flight at once, and are scaled there.
+        ok = wait_warp(bar(B_K_EMPTY), (pages & 1) ^ 1, guard, 0xd27);         // QK of the item before
+        if (!ok) break;
+        const int rows = info[0].w * p.group, part = lane & 15, row0 = 2 * (warp - CONVERT) + (lane >> 4);
+        const auto piece = [&](int row) {
+          return gbase + OFF_Q + (part >> 3) * (HALF_TILE / 2) + row * 128 + (((part & 7) ^ (row & 7)) << 4);
+        };
+        const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.a.q) + info[0].z * p.a.q_token +
+                                   static_cast<long long>(info[1].x) * p.group * p.a.q_head + part * 8;
+#pragma unroll 1
+        for (int row = row0; row < 128; row += 16) {
+          const int token = row * group_inverse >> 16, g = row - token * p.group;
+          const bool in = row < rows;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(piece(row))),
+                       "l"(in ? src + token * p.a.q_token + g * p.a.q_head : src), "r"(in ? 16 : 0)
+                       : "memory");
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll 2
+        for (int row = row0; row < 128; row += 16) {
+          const uint4 w = *reinterpret_cast<const uint4*>(piece(row));
+          uint32_t top = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
+#pragma unroll
+          for (int by = 8; by; by >>= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, by));
+          top = max(top & 0xffffu, top >> 16);
+          const bool odd = top >= 0x7f80u;        // infinities and NaN: the row ends as NaN
+          const int ex = top == 0 || odd ? 0 : min(134 - static_cast<int>(top >> 7), 126);
+          const float by = odd ? __int_as_float(0x7fffffff) : power_of_two(ex) * sign;
+          const auto scaled = [&](uint32_t pair) {
+            const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&pair));
+            return pack_half2(x.x * by, x.y * by);
+          };
+          *reinterpret_cast<uint4*>(piece(row)) = make_uint4(scaled(w.x), scaled(w.y), scaled(w.z), scaled(w.w));
+          if (part == 0) reinterpret_cast<float*>(gbase + OFF_QF)[(item & 1) * 128 + row] = factor * power_of_two(-ex);
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_Q_FULL + (item & 1)));
       }
       nan_at += (item & 3) * 128;
 #pragma unroll 1
@@ -547,8 +535,6 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
       if (flags & LAST) {
         const int token0 = info[0].z, head = info[1].x, place = info[1].y;
         if (!fresh) {
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(B_Q_EMPTY + (items & 1)));
           ok = wait_warp(bar(B_V_EMPTY + ((pages - 1) & 1)), ((pages - 1) >> 1) & 1, guard, 0xd36);         // PV of the last page
           if (!ok) break;
           tc_fence_after();
@@ -622,7 +608,7 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == WALK && misc[1]) {                   // a wait was given up: copies in flight land before the CTA leaves
+  if (warp == LOAD && misc[1]) {                   // a wait was given up: copies in flight land before the CTA leaves
     for (uint32_t f = fills > SLOTS ? fills - SLOTS : 0; f < fills; ++f) mbar_wait_drain(bar(B_FULL + f % SLOTS), (f / SLOTS) & 1);
   }
   if (warp == MMA) {
