@@ -26,16 +26,16 @@ namespace {
 
 constexpr int CONVERT = 8, MMA = 16, WALK = 17, LOAD = 18, WARPS = 19, THREADS = 32 * WARPS;
 constexpr int HALF_TILE = 128 * 256;              // 128 rows of 128 f16: two panels of 64 features, 128-byte swizzle
-constexpr int SLOTS = 7;
-constexpr int OFF_Q = 0, OFF_K = HALF_TILE, OFF_V = OFF_K + HALF_TILE, OFF_RING = OFF_V + HALF_TILE;
-constexpr int OFF_NAN = OFF_RING + SLOTS * TILE_BYTES;             // int [4][128]: by item, first key whose value has a NaN at a feature
-constexpr int OFF_QF = OFF_NAN + 4 * 512;         // float [2][128]: what a row's scores are multiplied by
+constexpr int SLOTS = 5;
+constexpr int OFF_Q = 0, OFF_K = HALF_TILE, OFF_V = OFF_K + HALF_TILE, OFF_RING = OFF_V + 2 * HALF_TILE;
+constexpr int OFF_NAN = OFF_RING + SLOTS * TILE_BYTES;             // int [8][128]: by item, first key whose value has a NaN at a feature
+constexpr int OFF_QF = OFF_NAN + 8 * 512;         // float [2][128]: what a row's scores are multiplied by
 constexpr int OFF_MAX = OFF_QF + 2 * 512;         // float [2][2][128]: by page, half and row
 constexpr int OFF_SUM = OFF_MAX + 4 * 512;        // float [2][2][128]: by item, half and row
 constexpr int OFF_INFO = OFF_SUM + 4 * 512;
 constexpr int OFF_BAR = OFF_INFO + BATCHES * BATCH_BYTES;
 constexpr int B_INFO_FULL = 0, B_INFO_EMPTY = BATCHES, B_FULL = 2 * BATCHES, B_EMPTY = B_FULL + SLOTS, B_K_FULL = B_EMPTY + SLOTS,
-              B_K_EMPTY = B_K_FULL + 1, B_V_FULL = B_K_EMPTY + 1, B_V_EMPTY = B_V_FULL + 2, B_S_FULL = B_V_EMPTY + 2,
+              B_K_EMPTY = B_K_FULL + 1, B_V_FULL = B_K_EMPTY + 2, B_V_EMPTY = B_V_FULL + 2, B_S_FULL = B_V_EMPTY + 2,
               B_P_FULL = B_S_FULL + 2, B_Q_FULL = B_P_FULL + 2, B_MAX = B_Q_FULL + 2, B_SUM = B_MAX + 8,
               B_DONE = B_SUM + 4, BARS = B_DONE + 1;
 constexpr int OFF_FLAG = OFF_BAR + BARS * 8;      // int [2]: for the MMA warp, with a page's K tile: 1 = the first of an item, 2 = stop
@@ -62,10 +62,10 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// A tile of codes (128 rows of 128 bytes, shared memory) into f16, 256 threads: four chunks of 16 codes each. Eight threads of
-// a warp write two rows of a panel: 16-byte pieces that meet no bank twice. rows: the others become zeros.
-__device__ __forceinline__ int chunk_row(int t, int i) { return (t >> 2) + 64 * (i & 1); }
-__device__ __forceinline__ int chunk_part(int t, int i) { return (t & 3) + 4 * (((i >> 1) ^ (t >> 2)) & 1); }
+// A tile of codes (128 rows of 128 bytes, shared memory) into f16 by 128 threads: eight chunks of 16 codes each. Eight threads
+// of a warp read and write two rows, in 16-byte pieces that meet no bank twice.
+__device__ __forceinline__ int chunk_row(int t, int i) { return (t >> 2) + 32 * (i & 3); }
+__device__ __forceinline__ int chunk_part(int t, int i) { return (t & 3) + 4 * (((i >> 2) ^ (t >> 2)) & 1); }
 __device__ __forceinline__ void store_chunk(unsigned char* tile, int row, int part, uint4 x) {
   unsigned char* to = tile + (part >> 2) * (HALF_TILE / 2) + row * 128;
   const int c = (part & 3) * 2;
@@ -90,6 +90,34 @@ __device__ __noinline__ uint4 without_nan(uint4 x, int* nan_at, int key) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// The rare parts of the softmax (out of line they cost 3 us of 108). 64 columns of TMEM:
+// scores from the key `sees` on become -inf; outputs are scaled.
+__device__ __forceinline__ void mask_scores(uint32_t taddr, int sees) {
+#pragma unroll 1
+  for (int c = 0; c < 64; c += 16) {
+    uint32_t s[16];
+    tmem_ld16(taddr + c, s);
+    tc_wait_ld();
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (c + j >= sees) s[j] = 0xff800000u;
+    tmem_st16(taddr + c, s);
+  }
+  tc_wait_st();
+}
+__device__ __forceinline__ void scale_output(uint32_t taddr, float by) {
+  tc_fence_after();
+#pragma unroll 1
+  for (int c = 0; c < 64; c += 16) {
+    uint32_t o[16];
+    tmem_ld16(taddr + c, o);
+    tc_wait_ld();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * by);
+    tmem_st16(taddr + c, o);
+  }
+}
+
 __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Params p, int* status) {
   extern __shared__ unsigned char raw[];
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
@@ -108,13 +136,13 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
     init(B_INFO_FULL, BATCHES, 1);
     init(B_INFO_EMPTY, BATCHES, 17);              // softmax, conversion, loads
     init(B_FULL, SLOTS, 1);
-    init(B_EMPTY, SLOTS, 8);
-    init(B_K_FULL, 1, 8);
-    init(B_K_EMPTY, 1, 1);
-    init(B_V_FULL, 2, 8);                         // by page, as those below: the softmax warps may be a page ahead
+    init(B_EMPTY, SLOTS, 4);
+    init(B_K_FULL, 1, 4);
+    init(B_K_EMPTY, 2, 1);                        // by page, as all below: who waits for it may be a page ahead
+    init(B_V_FULL, 2, 4);
     init(B_V_EMPTY, 2, 1);
     init(B_S_FULL, 2, 1);
-    init(B_P_FULL, 2, 8);                         // by page: a warp may be a page ahead of another
+    init(B_P_FULL, 2, 8);
     init(B_Q_FULL, 2, 8);
     init(B_MAX, 12, 2);
     init(B_DONE, 1, 1);
@@ -126,6 +154,7 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
     tmem_alloc(smem_u32(const_cast<int*>(misc)), TMEM_COLUMNS);
     tmem_relinquish();
   }
+  if (tid < 256) reinterpret_cast<int*>(gbase + OFF_NAN)[tid] = 0x7fffffff;
   tc_fence_before();
   const Share share = find_share<WARPS>(p);       // (two barriers of the CTA)
   tc_fence_after();
@@ -175,7 +204,6 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
         phase ^= 1;
       }
     };
-    int behind = -1;                              // page whose V is still to come: it follows the next page's K, within an item
     while (ok) {
       const uint32_t e = batches % BATCHES;
       ok = wait_warp(bar(B_INFO_FULL + e), (batches / BATCHES) & 1, guard, 0xd01);
@@ -184,12 +212,7 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
       const int flags = info[0].x, count = info[0].y;
       if (flags & STOP) break;
 #pragma unroll 1
-      for (int step = 0; ok && step < count + (flags & LAST ? 1 : 0); ++step) {
-        const int row = step < count ? info[2 + step].x : -1;
-        if (row >= 0) load(p.a.k, row);
-        if (behind >= 0) load(p.a.v, behind);
-        behind = row;
-      }
+      for (int n = 0; ok && n < 2 * count; ++n) load(n & 1 ? p.a.v : p.a.k, info[2 + (n >> 1)].x);
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(B_INFO_EMPTY + e));
       ++batches;
@@ -234,7 +257,7 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
               mma_ss_lo<HI, HI>(tmem + (first & 1) * 128, q + at, k + at, ID_QK, kk > 0);
             }
             tc_commit(bar(B_S_FULL + (first & 1)));
-            tc_commit(bar(B_K_EMPTY));
+            tc_commit(bar(B_K_EMPTY + (first & 1)));
           }
           __syncwarp();
           ++first;
@@ -255,7 +278,7 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
       if (!ok) break;
       tc_fence_after();
       if (elect_one()) {
-        const uint32_t v = ((base + OFF_V) >> 4) | ((HALF_TILE / 2 >> 4) << 16);
+        const uint32_t v = ((base + OFF_V + (second & 1) * HALF_TILE) >> 4) | ((HALF_TILE / 2 >> 4) << 16);
         const bool fresh = second & 1 ? fresh1 : fresh0;
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
@@ -271,25 +294,17 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
     __syncwarp();
     mbar_wait_drain(bar(B_DONE), 0);
   } else if (warp >= CONVERT) {
-    // --------------------------------------------------------------- pages into f16 tiles
-    const int t = tid - 32 * CONVERT;
+    // --------------------------------------------------------------- pages into f16 tiles: four warps K, four V
+    const bool values = warp >= CONVERT + 4;
+    const int t = tid & 127, mine = values ? 1 : 0;
     const int group_inverse = (65535 + p.group) / p.group;        // row / group = row * this >> 16 for rows below 128
     const float sign = p.a.scale < 0.f ? -1.f : 1.f, factor = fabsf(p.a.scale) * 1.4426950408889634f;
     bool ok = true, started = false;
     uint32_t batches = 0;
-    int item = -1, pages = 0, values = 0, slot = 0, phase = 0;       // tiles of K and of V done
-    int behind = 0;                               // keys of the page whose V is still to be done (within an item only) as in a batch
-    const auto tile_full = [&](int code) {
-      ok = wait_warp(bar(B_FULL + slot), phase, guard, code);
-      return gbase + OFF_RING + slot * TILE_BYTES;
-    };
-    const auto tile_read = [&]() {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(B_EMPTY + slot));
-      if (++slot == SLOTS) {
-        slot = 0;
-        phase ^= 1;
-      }
+    int item = -1, pages = 0, slot = mine, phase = 0;
+    const auto qk_done = [&](int page, int code) {
+      ok = wait_warp(bar(B_K_EMPTY + (page & 1)), (page >> 1) & 1, guard, code);
+      return ok;
     };
     while (ok) {
       const uint32_t e = batches % BATCHES;
@@ -298,22 +313,19 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
       const int4* info = batch_at(e);
       const int flags = info[0].x, count = info[0].y;
       if (flags & STOP) {
-        ok = wait_warp(bar(B_K_EMPTY), (pages & 1) ^ 1, guard, 0xd21);
-        if (!ok) break;
+        if (values) break;
+        if (!qk_done(pages - 1, 0xd21)) break;
         if (t == 0) *reinterpret_cast<volatile int*>(gbase + OFF_FLAG + 4 * (pages & 1)) = 2;
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(B_K_FULL));
         break;
       }
       if (flags & FIRST) started = false;
-      int* nan_at = reinterpret_cast<int*>(gbase + OFF_NAN);
       if (count && !started) {
         ++item;
-        if (t < 128) nan_at[(item & 3) * 128 + t] = 0x7fffffff;    // (read for the last time items ago)
         // The item's queries: half a warp to a row, 8 features to a thread. A thread's pieces come to the places they keep, all
         // in flight at once, and are scaled there.
-        ok = wait_warp(bar(B_K_EMPTY), (pages & 1) ^ 1, guard, 0xd27);         // QK of the item before
-        if (!ok) break;
+        if (!qk_done(pages - 1, 0xd27)) break;
         const int rows = info[0].w * p.group, part = lane & 15, row0 = 2 * (warp - CONVERT) + (lane >> 4);
         const auto piece = [&](int row) {
           return gbase + OFF_Q + (part >> 3) * (HALF_TILE / 2) + row * 128 + (((part & 7) ^ (row & 7)) << 4);
@@ -350,37 +362,39 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(B_Q_FULL + (item & 1)));
       }
-      nan_at += (item & 3) * 128;
 #pragma unroll 1
-      for (int step = 0; step < count + (flags & LAST ? 1 : 0); ++step) {
-        const int seen = step < count ? info[2 + step].y : 0;
-        if (step < count) {
-          const unsigned char* from = tile_full(0xd22);
-          ok = ok && wait_warp(bar(B_K_EMPTY), (pages & 1) ^ 1, guard, 0xd23);
-          if (!ok) break;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = chunk_row(t, i), part = chunk_part(t, i);
-            store_chunk(gbase + OFF_K, row, part, *reinterpret_cast<const uint4*>(from + row * 128 + part * 16));
-          }
-          if (t == 0) *reinterpret_cast<volatile int*>(gbase + OFF_FLAG + 4 * (pages & 1)) = started ? 0 : 1;
-          started = true;
-          fence_async_smem();
-          tile_read();
-          if (lane == 0) mbar_arrive(bar(B_K_FULL));
-          ++pages;
+      for (int step = 0; step < count; ++step) {
+        const int seen = info[2 + step].y, valid = values ? seen & 0xffff : 128, limit = values ? seen >> 16 : 128;
+        ok = wait_warp(bar(B_FULL + slot), phase, guard, 0xd22);
+        // the product that read the tile before
+        ok = ok && (values ? wait_warp(bar(B_V_EMPTY + (pages & 1)), ((pages >> 1) & 1) ^ 1, guard, 0xd25) : qk_done(pages - 1, 0xd23));
+        if (!ok) break;
+        if (!started) {
+          // V: the place of the item after the next is cleared here. Its first page comes two pages behind at least, and is
+          // converted when PV of this one is done: all four warps have been here. (The item that had the place has ended.)
+          if (values) reinterpret_cast<int*>(gbase + OFF_NAN)[((item + 2) & 7) * 128 + t] = 0x7fffffff;
         }
-        if (behind) {
-          // V comes behind the next page's K, so that its QK can be issued while the softmax of this page is under way
-          const int valid = behind & 0xffff, limit = behind >> 16;
-          const unsigned char* from = tile_full(0xd24);
-          ok = ok && wait_warp(bar(B_V_EMPTY + ((values - 1) & 1)), ((values - 1) >> 1) & 1, guard, 0xd25);
-          if (ok && limit < valid) ok = wait_warp(bar(B_K_FULL), (pages - 1) & 1, guard, 0xd26);   // all have cleared their nan_at
-          if (!ok) break;
+        if (t == 0 && !values) *reinterpret_cast<volatile int*>(gbase + OFF_FLAG + 4 * (pages & 1)) = started ? 0 : 1;
+        started = true;
+        const unsigned char* from = gbase + OFF_RING + slot * TILE_BYTES;
+        unsigned char* to = gbase + (values ? OFF_V + (pages & 1) * HALF_TILE : OFF_K);
+        const auto piece = [&](int i) {
+          return reinterpret_cast<const uint4*>(from + chunk_row(t, i) * 128 + chunk_part(t, i) * 16);
+        };
+        if (limit == 128 && valid == 128) {       // nothing between the loads: their latencies overlap
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < 8; i += 4) {
+            const uint4 x0 = *piece(i), x1 = *piece(i + 1), x2 = *piece(i + 2), x3 = *piece(i + 3);
+            store_chunk(to, chunk_row(t, i), chunk_part(t, i), x0);
+            store_chunk(to, chunk_row(t, i + 1), chunk_part(t, i + 1), x1);
+            store_chunk(to, chunk_row(t, i + 2), chunk_part(t, i + 2), x2);
+            store_chunk(to, chunk_row(t, i + 3), chunk_part(t, i + 3), x3);
+          }
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < 8; ++i) {
             const int row = chunk_row(t, i), part = chunk_part(t, i);
-            uint4 x = *reinterpret_cast<const uint4*>(from + row * 128 + part * 16);
+            uint4 x = *piece(i);
             if (row >= valid) {
               x = make_uint4(0, 0, 0, 0);         // what lies behind the sequence may hold anything
             } else if (limit < valid) {
@@ -388,16 +402,24 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
               // one at a feature is kept, as a distance from the keys that the first token sees; rows that see it get their NaN
               // in the end.
               const auto any = [](uint32_t w) { return (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0; };
-              if (any(x.x) || any(x.y) || any(x.z) || any(x.w)) x = without_nan(x, nan_at + part * 16, row - limit);
+              if (any(x.x) || any(x.y) || any(x.z) || any(x.w))
+                x = without_nan(x, reinterpret_cast<int*>(gbase + OFF_NAN) + (item & 7) * 128 + part * 16, row - limit);
             }
-            store_chunk(gbase + OFF_V, row, part, x);
+            store_chunk(to, row, part, x);
           }
-          fence_async_smem();
-          tile_read();
-          if (lane == 0) mbar_arrive(bar(B_V_FULL + (values & 1)));
-          ++values;
         }
-        behind = seen;                            // (a page that is taken holds a key at least)
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(bar(B_EMPTY + slot));
+          mbar_arrive(bar(values ? B_V_FULL + (pages & 1) : B_K_FULL));
+        }
+        slot += 2;
+        if (slot >= SLOTS) {
+          slot -= SLOTS;
+          phase ^= 1;
+        }
+        ++pages;
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(B_INFO_EMPTY + e));
@@ -441,16 +463,12 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
         const int seen = info[2 + step].y, valid = seen & 0xffff, limit = seen >> 16;
         if (!idle) {
           tc_fence_after();
+          if (valid < 128 || limit < 128)
+            mask_scores(t_row + 128 * b + 64 * half, min(p.a.causal ? limit + token : limit, valid) - 64 * half);
           uint32_t s[2][32];
           tmem_ld32(t_row + 128 * b + 64 * half, s[0]);
           tmem_ld32(t_row + 128 * b + 64 * half + 32, s[1]);
           tc_wait_ld();
-          if (valid < 128 || limit < 128) {
-            const int sees = min(p.a.causal ? limit + token : limit, valid) - 64 * half;
-#pragma unroll
-            for (int j = 0; j < 64; ++j)
-              if (j >= sees) s[j >> 5][j & 31] = 0xff800000u;
-          }
           float top = -INFINITY, other = -INFINITY;
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
@@ -487,16 +505,7 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
           if (!fresh && __any_sync(0xffffffffu, keep != 1.f)) {
             ok = wait_warp(bar(B_V_EMPTY + (b ^ 1)), ((pages - 1) >> 1) & 1, guard, 0xd34);       // PV of the page before
             if (!ok) break;
-            tc_fence_after();
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              uint32_t o[16];
-              tmem_ld16(t_row + O_COLUMN + 64 * half + 16 * c, o);
-              tc_wait_ld();
-#pragma unroll
-              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
-              tmem_st16(t_row + O_COLUMN + 64 * half + 16 * c, o);
-            }
+            scale_output(t_row + O_COLUMN + 64 * half, keep);
           }
           const float ratio = vs == v_ref ? 1.f : vs == 0.f ? 0.f : __fdividef(vs, v_ref);      // at most 1; NaN stays
           const float offset = LIFT - (m == -INFINITY ? 0.f : m);
@@ -549,7 +558,7 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
           const float total = sum_at[row] + sum_at[128 + row];
           const float by = total == 0.f ? 0.f : place >= 0 ? v_ref : v_ref / total;
           const long long out_row = (static_cast<long long>(token0) + token) * p.a.hq + head * p.group + g;
-          const int* nan_at = reinterpret_cast<const int*>(gbase + OFF_NAN) + (items & 3) * 128 + 64 * half;
+          const int* nan_at = reinterpret_cast<const int*>(gbase + OFF_NAN) + (items & 7) * 128 + 64 * half;
 #pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             uint32_t o[16];
