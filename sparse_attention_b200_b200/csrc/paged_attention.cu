@@ -539,6 +539,8 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
         item_pages = 0;
       }
       item_pages += count;
+      // A second group whose rows are none only keeps the others' count (an item may be shorter than the longest one).
+      const bool idle = R > 16 && row0 >= info[0].w * p.group;
       // the pages of the batch, then the item's end
       const int steps = count + (flags & LAST ? 1 : 0);
 #pragma unroll 1
@@ -546,6 +548,15 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
         const bool page = step < count;
         const volatile int* x = reinterpret_cast<const volatile int*>(info + 2 + min(step, 31));     // read where it is needed: registers
         const int seen = x[1], valid = seen & 0xffff, limit = seen >> 16;
+        if (page && idle) {
+          if (lane == 0) mbar_arrive(bar(C::B_MAX + 2 * wg + (pages & 1)));
+          ok = pending < 0 || wait_warp(bar(C::B_O_FULL), pending & 1, guard, 0xc38);
+          if (!ok) break;
+          if (lane == 0) mbar_arrive(bar(C::B_P_FULL));
+          pending = pages++;
+          masked = 0;
+          continue;
+        }
         if (page) {
           const int b = pages & 1;
           if (fresh) {

@@ -29,18 +29,19 @@ constexpr int HALF_TILE = 128 * 256;              // 128 rows of 128 f16: two pa
 constexpr int SLOTS = 5;
 constexpr int OFF_Q = 0, OFF_K = HALF_TILE, OFF_V = OFF_K + HALF_TILE, OFF_RING = OFF_V + 2 * HALF_TILE;
 constexpr int OFF_NAN = OFF_RING + SLOTS * TILE_BYTES;             // int [8][128]: by item, first key whose value has a NaN at a feature
-constexpr int OFF_QF = OFF_NAN + 8 * 512;         // float [2][128]: what a row's scores are multiplied by
-constexpr int OFF_MAX = OFF_QF + 2 * 512;         // float [2][2][128]: by page, half and row
+constexpr int OFF_QF = OFF_NAN + 8 * 512;         // float [4][128]: by item, what a row's scores are multiplied by
+constexpr int OFF_MAX = OFF_QF + 4 * 512;         // float [2][2][128]: by page, half and row
 constexpr int OFF_SUM = OFF_MAX + 4 * 512;        // float [2][2][128]: by item, half and row
 constexpr int OFF_INFO = OFF_SUM + 4 * 512;
 constexpr int OFF_BAR = OFF_INFO + BATCHES * BATCH_BYTES;
 constexpr int B_INFO_FULL = 0, B_INFO_EMPTY = BATCHES, B_FULL = 2 * BATCHES, B_EMPTY = B_FULL + SLOTS, B_K_FULL = B_EMPTY + SLOTS,
               B_K_EMPTY = B_K_FULL + 1, B_V_FULL = B_K_EMPTY + 2, B_V_EMPTY = B_V_FULL + 2, B_S_FULL = B_V_EMPTY + 2,
-              B_P_FULL = B_S_FULL + 2, B_Q_FULL = B_P_FULL + 2, B_MAX = B_Q_FULL + 2, B_SUM = B_MAX + 8,
+              B_P_FULL = B_S_FULL + 2, B_Q_FULL = B_P_FULL + 2, B_MAX = B_Q_FULL + 4, B_SUM = B_MAX + 8,
               B_DONE = B_SUM + 4, BARS = B_DONE + 1;
 constexpr int OFF_FLAG = OFF_BAR + BARS * 8;      // int [2]: for the MMA warp, with a page's K tile: 1 = the first of an item, 2 = stop
 constexpr int OFF_MISC = (OFF_FLAG + 8 + 15) / 16 * 16;
 constexpr int SMEM = OFF_MISC + 64 + 1024;        // 1024: alignment of the tiles
+static_assert(SMEM <= 227 * 1024 - 512, "shared memory of an SM");
 constexpr int TMEM_COLUMNS = 512;                 // S of two pages (and P over its first half), O
 constexpr int O_COLUMN = 256;
 constexpr float LIFT = 6.f;                       // probabilities are exp2(x - m + 6): up to 2^14 before m follows
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
     init(B_V_EMPTY, 2, 1);
     init(B_S_FULL, 2, 1);
     init(B_P_FULL, 2, 8);
-    init(B_Q_FULL, 2, 8);
+    init(B_Q_FULL, 4, 8);                          // by item: QK may be two items of a page each ahead of the softmax
     init(B_MAX, 12, 2);
     init(B_DONE, 1, 1);
     fence_mbar_init();
@@ -243,7 +244,7 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
           const bool fresh = __any_sync(0xffffffffu, flag & 1);
           if (fresh) {
             ++item;
-            ok = mbar_wait_warp(bar(B_Q_FULL + (item & 1)), (item >> 1) & 1, guard, 0xd11);
+            ok = mbar_wait_warp(bar(B_Q_FULL + (item & 3)), (item >> 2) & 1, guard, 0xd11);
             if (!ok) break;
           }
           if (first & 1) fresh1 = fresh;
@@ -356,11 +357,11 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
             return pack_half2(x.x * by, x.y * by);
           };
           *reinterpret_cast<uint4*>(piece(row)) = make_uint4(scaled(w.x), scaled(w.y), scaled(w.z), scaled(w.w));
-          if (part == 0) reinterpret_cast<float*>(gbase + OFF_QF)[(item & 1) * 128 + row] = factor * power_of_two(-ex);
+          if (part == 0) reinterpret_cast<float*>(gbase + OFF_QF)[(item & 3) * 128 + row] = factor * power_of_two(-ex);
         }
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(B_Q_FULL + (item & 1)));
+        if (lane == 0) mbar_arrive(bar(B_Q_FULL + (item & 3)));
       }
 #pragma unroll 1
       for (int step = 0; step < count; ++step) {
@@ -454,9 +455,9 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
       for (int step = 0; step < count; ++step) {
         const int b = pages & 1;
         if (fresh) {
-          ok = wait_warp(bar(B_Q_FULL + (items & 1)), (items >> 1) & 1, guard, 0xd31);
+          ok = wait_warp(bar(B_Q_FULL + (items & 3)), (items >> 2) & 1, guard, 0xd31);
           if (!ok) break;
-          f_row = reinterpret_cast<const float*>(gbase + OFF_QF)[(items & 1) * 128 + row];
+          f_row = reinterpret_cast<const float*>(gbase + OFF_QF)[(items & 3) * 128 + row];
         }
         ok = wait_warp(bar(B_S_FULL + b), (pages >> 1) & 1, guard, 0xd32);
         if (!ok) break;
