@@ -3,40 +3,42 @@
 //   s_ij = scale * q_i . (k_scale * k_j)          keys j <= i + k_len - q_len of the request (causal) in the pages taken
 //   o_i = sum_j softmax(s_i)_j v_scale v_j        lse_i = ln sum_j exp s_ij;  no key: o = 0, lse = -inf
 //
-// Mathematics. A work item is `pack` tokens of a request and a KV head: R rows (token, query head) that share a pass over the
-// pages. Keys are the M dimension of both products, so that even one token of a few heads fills the instruction:
+// Mathematics. A work item is `pack` tokens of a request and a KV head: R rows (token, query head), 16 here, that share a pass
+// over the pages; paged_attention_wide.cu has the kernel for more. Keys are the M dimension of both products, so that even one
+// token of a few heads fills the instruction:
 //   S^T [128 keys, R] = K [128 keys, 128] Q^T       O^T [128 features, R] = V^T [128 features, 128 keys] P^T
 // The tensor core multiplies e4m3 by e4m3 (kind::f8f6f4), and the codes of a page are its operands as they lie in memory:
 // nothing is dequantised. The other operand is split in two e4m3 terms in columns of their own, x = hi + lo / 16: a bf16 has
 // eight significant bits and an e4m3 code four, so a query (scaled by a power of two to [128, 256) by its row's largest
 // feature) is carried exactly but for features below 2^-22 of the largest; a probability (times 256, against the maximum of
 // its own page, so that no page's weights fall below the format's range) is cut at four bits and the rest rounded to four:
-// within 2^-8 of its value, half a step of bf16. Maxima, sums and outputs are fp32; every page's output is added
-// to registers with the page's own factor exp2(page maximum - running maximum) * v_scale.
+// within 2^-8 of its value, half a step of bf16. Sums and outputs are fp32; every page's output is added to registers with the
+// page's own factor exp2(page maximum - maximum of the item's first page) * v_scale.
 //
-// A softmax thread owns a key (a TMEM lane of S^T) and 16 rows; a row's maximum over the page is a warp reduction
-// (redux.sync on fp32) and an exchange between four warps. In the second product the same thread owns a feature.
+// A softmax thread owns a key (a TMEM lane of S^T) and the 16 rows; a row's maximum over the page is taken in bf16 pairs by
+// shuffles and an exchange between the four warps, in fp32 only where the scores are huge. In the second product the same
+// thread owns a feature.
 //
 // Work split. Pages of all items, in the order (head, request, tile, page), are cut in equal shares, one per CTA: long and
 // short requests balance whatever their lengths, known on the device only. Every CTA finds its share itself, from closed sums
 // over a request's tiles and a scan over the requests. An item that lies in several shares is left as partial sums (fp32, with
 // its maximum and sum) that paged_merge_kernel adds in order: no atomics, the same bits every time.
 //
-// CTA: R / 16 softmax warpgroups, a loader warp (TMA, one 16 KB tile of K or V to a slot of a ring), an MMA warp, two warps
-// that bring and split the queries of the next item. Entries (start of an item, page, end) go through a ring of their own.
+// CTA (two to an SM, so that one's exchanges and waits lie under the other's exponentials): four softmax warps, a loader warp
+// (TMA, one 16 KB tile of K or V to a slot of a ring), an MMA warp, two warps that bring and split the queries of the next item.
+// What the loader tells of items and pages goes through a ring of its own, in batches of 32 pages.
 #include "paged_attention.cuh"
 
 namespace sb {
 namespace pa {
 
-template <int R_>
+constexpr int R = 16, N = 2 * R;                  // rows of an item, columns that carry them: hi and lo
 struct Config {
-  static constexpr int R = R_, N = 2 * R, GROUPS = R / 16;
-  static constexpr int SOFTMAX_WARPS = 4 * GROUPS;
+  static constexpr int SOFTMAX_WARPS = 4;
   static constexpr int LOADER = SOFTMAX_WARPS, MMA = LOADER + 1, QWARP = MMA + 1, WARPS = QWARP + 2;
   static constexpr int THREADS = 32 * WARPS;
-  static constexpr int CTAS = R == 16 ? 2 : 1;    // per SM
-  static constexpr int SLOTS = R == 16 ? 5 : 11;
+  static constexpr int CTAS = 2;                  // per SM
+  static constexpr int SLOTS = 5;
   static constexpr int OFF_RING = 0;
   static constexpr int OFF_Q = OFF_RING + SLOTS * TILE_BYTES;       // two buffers of N rows of 128 bytes
   static constexpr int OFF_P = OFF_Q + 2 * N * 128;                 // 128 keys x N columns
@@ -51,12 +53,12 @@ struct Config {
   static constexpr int OFF_BAR = OFF_INFO + BATCHES * BATCH_BYTES;
   static constexpr int B_INFO_FULL = 0, B_INFO_EMPTY = BATCHES, B_FULL = 2 * BATCHES, B_EMPTY = B_FULL + SLOTS;
   static constexpr int B_S_FULL = B_EMPTY + SLOTS, B_P_FULL = B_S_FULL + 2, B_O_FULL = B_P_FULL + 1, B_Q_FULL = B_O_FULL + 1,
-                       B_Q_EMPTY = B_Q_FULL + 2, B_MAX = B_Q_EMPTY + 2, B_SUM = B_MAX + 2 * GROUPS, B_EXACT = B_SUM + 2 * GROUPS,
-                       B_DONE = B_EXACT + GROUPS, BARS = B_DONE + 1;
+                       B_Q_EMPTY = B_Q_FULL + 2, B_MAX = B_Q_EMPTY + 2, B_SUM = B_MAX + 2, B_EXACT = B_SUM + 2,
+                       B_DONE = B_EXACT + 1, BARS = B_DONE + 1;
   static constexpr int OFF_FLAG = OFF_BAR + BARS * 8;               // int [SLOTS]: for the MMA warp, with a page's K tile
   static constexpr int OFF_MISC = (OFF_FLAG + SLOTS * 4 + 15) / 16 * 16;
   static constexpr int SMEM = OFF_MISC + 64 + 1024;                 // 1024: alignment of the tiles
-  static constexpr int TMEM = R == 16 ? 128 : 512;                  // S of two pages and O: a power of two
+  static constexpr int TMEM = 128;                                  // S of two pages and O: a power of two
 };
 
 // kind::f8f6f4 instruction descriptor: e4m3 x e4m3 -> fp32, M = 128.
@@ -157,7 +159,6 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
 // hi + lo / 16 of 16 rows from tensor memory, eight at a time (registers)
-template <int R>
 __device__ __forceinline__ void load_sums(uint32_t at, float (&x)[16]) {
 #pragma unroll
   for (int i = 0; i < 16; i += 8) {
@@ -175,32 +176,30 @@ __device__ __forceinline__ void load_sums(uint32_t at, float (&x)[16]) {
   }
 }
 
-// o[j] where it is NaN: the sum of p v over the keys of a page that row row0 + j sees, from the probabilities in shared memory
+// o[j] where it is NaN: the sum of p v over the keys of a page that row j sees, from the probabilities in shared memory
 // and a feature's codes
-template <int R>
-__device__ __noinline__ void visible_sums(float* o, const unsigned char* pr, const uint8_t* v, const int* row_of, int row0, int limit,
+__device__ __noinline__ void visible_sums(float* o, const unsigned char* pr, const uint8_t* v, const int* row_of, int limit,
                                           int valid) {
 #pragma unroll 1
   for (int j = 0; j < 16; ++j) {
     if (o[j] == o[j]) continue;
-    const int row = row0 + j, end = min(limit + (row_of[row] >> 16), valid);
+    const int end = min(limit + (row_of[j] >> 16), valid);
     float x = 0.f;
 #pragma unroll 1
     for (int n = 0; n < end; ++n) {
       const auto at = [&](int c) { return from_e4m3(pr[(c >> 5) * 4096 + n * 32 + ((((c >> 4) ^ (n >> 2)) & 1) << 4) + (c & 15)]); };
-      x = fmaf(fmaf(at(R + row), 0.0625f, at(row)), from_e4m3(__ldg(v + n * 128)), x);
+      x = fmaf(fmaf(at(R + j), 0.0625f, at(j)), from_e4m3(__ldg(v + n * 128)), x);
     }
     o[j] = x;
   }
 }
 
 // ------------------------------------------------------------------ kernel
-template <int R_>
-__global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
+__global__ void __launch_bounds__(Config::THREADS, Config::CTAS)
     paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const Params p,
                            int* status) {
-  using C = Config<R_>;
-  constexpr int R = C::R, N = C::N, SLOTS = C::SLOTS;
+  using C = Config;
+  constexpr int SLOTS = C::SLOTS;
   extern __shared__ unsigned char raw[];
   const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
   unsigned char* gbase = raw + (base - smem_u32(raw));
@@ -469,12 +468,12 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
     }
   } else {
     // --------------------------------------------------------------- softmax: lane = key, then lane = feature
-    const int wg = warp >> 2, quarter = warp & 3, key = quarter * 32 + lane, row0 = wg * 16, r16 = lane & 15;
-    const uint32_t lane_base = static_cast<uint32_t>(quarter * 32) << 16;
+    const int key = warp * 32 + lane, r16 = lane & 15;
+    const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
     // of the warp's 16 rows: score factor, exponent offset, weight of the page's sum, weight of its output
     float* factors = reinterpret_cast<float*>(gbase + C::OFF_FACTOR) + warp * 64;
-    __nv_bfloat16* maxima = reinterpret_cast<__nv_bfloat16*>(gbase + C::OFF_MAX) + wg * 64;   // [4][16]
-    float* sums = reinterpret_cast<float*>(gbase + C::OFF_SUM) + wg * 64;
+    __nv_bfloat16* maxima = reinterpret_cast<__nv_bfloat16*>(gbase + C::OFF_MAX);
+    float* sums = reinterpret_cast<float*>(gbase + C::OFF_SUM);
     const float* qf = reinterpret_cast<const float*>(gbase + C::OFF_QF);
     float acc[16], l[16], s[16], m = -INFINITY, scale_row = 0.f;      // m: what the sums of row r16 are relative to
     uint32_t batches = 0;
@@ -493,7 +492,7 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
       if (!ok) return;
       tc_fence_after();
       float o[16];
-      load_sums<R>(tmem + lane_base + 2 * N + row0, o);
+      load_sums(tmem + lane_base + 2 * N, o);
       tc_fence_before();
       if (masked) {
         // A key that is hidden from a row has probability 0 there, and 0 times a NaN of its value is not 0: such a sum is
@@ -505,8 +504,8 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
           float sums[16];
 #pragma unroll
           for (int j = 0; j < 16; ++j) sums[j] = o[j];
-          visible_sums<R>(sums, gbase + C::OFF_P,
-                          static_cast<const uint8_t*>(p.a.v) + static_cast<long long>(p_row) * TILE_BYTES + key, row_of, row0,
+          visible_sums(sums, gbase + C::OFF_P,
+                          static_cast<const uint8_t*>(p.a.v) + static_cast<long long>(p_row) * TILE_BYTES + key, row_of,
                           p_limit, p_valid);
 #pragma unroll
           for (int j = 0; j < 16; ++j) o[j] = sums[j];
@@ -539,8 +538,6 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
         item_pages = 0;
       }
       item_pages += count;
-      // A second group whose rows are none only keeps the others' count (an item may be shorter than the longest one).
-      const bool idle = R > 16 && row0 >= info[0].w * p.group;
       // the pages of the batch, then the item's end
       const int steps = count + (flags & LAST ? 1 : 0);
 #pragma unroll 1
@@ -548,32 +545,23 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
         const bool page = step < count;
         const volatile int* x = reinterpret_cast<const volatile int*>(info + 2 + min(step, 31));     // read where it is needed: registers
         const int seen = x[1], valid = seen & 0xffff, limit = seen >> 16;
-        if (page && idle) {
-          if (lane == 0) mbar_arrive(bar(C::B_MAX + 2 * wg + (pages & 1)));
-          ok = pending < 0 || wait_warp(bar(C::B_O_FULL), pending & 1, guard, 0xc38);
-          if (!ok) break;
-          if (lane == 0) mbar_arrive(bar(C::B_P_FULL));
-          pending = pages++;
-          masked = 0;
-          continue;
-        }
         if (page) {
           const int b = pages & 1;
           if (fresh) {
             ok = wait_warp(bar(C::B_Q_FULL + (items & 1)), (items >> 1) & 1, guard, 0xc32);
             if (!ok) break;
-            scale_row = qf[(items & 1) * R + row0 + r16];
+            scale_row = qf[(items & 1) * R + r16];
             fresh = false;
           }
           ok = wait_warp(bar(C::B_S_FULL + b), (pages >> 1) & 1, guard, 0xc33);
           if (!ok) break;
           tc_fence_after();
-          load_sums<R>(tmem + lane_base + b * N + row0, s);
+          load_sums(tmem + lane_base + b * N, s);
           tc_fence_before();
           const bool partial = valid < 128 || limit < 128;
           if (partial) {
             // Rows are in token order: those that do not see this key are the first ones.
-            const int first = p.a.causal ? (key - limit + 1) * p.group - row0 : key >= limit ? 16 : 0;
+            const int first = p.a.causal ? (key - limit + 1) * p.group : key >= limit ? 16 : 0;
             const int unseen = key >= valid ? 16 : first;
 #pragma unroll
             for (int j = 0; j < 16; ++j)
@@ -584,9 +572,9 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
 #pragma unroll
           for (int j = 0; j < 8; ++j) pairs[j] = pack_bf16x2(s[2 * j], s[2 * j + 1]);
           const uint32_t top = pair_maxima(pairs, lane);
-          if (lane < 8) reinterpret_cast<uint32_t*>(maxima + b * C::SOFTMAX_WARPS * 16 + quarter * 16)[lane] = top;
+          if (lane < 8) reinterpret_cast<uint32_t*>(maxima + b * C::SOFTMAX_WARPS * 16 + warp * 16)[lane] = top;
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar(C::B_MAX + 2 * wg + b));
+          if (lane == 0) mbar_arrive(bar(C::B_MAX + b));
         }
         // under the other warps' maxima: the output of the page before
         if (pending >= 0) {
@@ -597,7 +585,7 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
         asm volatile("" : "+r"(again));              // one copy of add_output for pages and ends
         if (again) {
           const int b = pages & 1;
-          ok = wait_warp(bar(C::B_MAX + 2 * wg + b), (pages >> 1) & 1, guard, 0xc36);
+          ok = wait_warp(bar(C::B_MAX + b), (pages >> 1) & 1, guard, 0xc36);
           if (!ok) break;
           const __nv_bfloat16* mx = maxima + b * C::SOFTMAX_WARPS * 16 + r16;
           float top = fmaxf(fmaxf(__bfloat162float(mx[0]), __bfloat162float(mx[16])),
@@ -610,12 +598,12 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
           if (__any_sync(0xffffffffu, !none && (fabsf(mu) > 100.f || (!unset && mu - m > 40.f)))) {
             // Rare: scores above that, or so large that the rounding up is more than a factor of 1.5. The maxima in fp32; all
             // four warps of the group are here.
-            float* exact = reinterpret_cast<float*>(gbase + C::OFF_EXACT) + wg * 64;
+            float* exact = reinterpret_cast<float*>(gbase + C::OFF_EXACT);
             top = row_maxima(s, lane);
-            if (lane < 16) exact[quarter * 16 + lane] = top;
+            if (lane < 16) exact[warp * 16 + lane] = top;
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar(C::B_EXACT + wg));
-            ok = wait_warp(bar(C::B_EXACT + wg), exacts++ & 1, guard, 0xc37);
+            if (lane == 0) mbar_arrive(bar(C::B_EXACT));
+            ok = wait_warp(bar(C::B_EXACT), exacts++ & 1, guard, 0xc37);
             if (!ok) break;
             top = fmaxf(fmaxf(exact[r16], exact[16 + r16]), fmaxf(exact[32 + r16], exact[48 + r16]));
             if (!none) mu = top * f;
@@ -667,9 +655,9 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
           }
           unsigned char* to = gbase + C::OFF_P + key * 32;
           const auto column = [&](int c) { return to + (c >> 5) * 4096 + ((((c >> 4) ^ (key >> 2)) & 1) << 4); };
-          *reinterpret_cast<uint4*>(column(row0)) = make_uint4(ph[0], ph[1], ph[2], ph[3]);
-          *reinterpret_cast<uint4*>(column(R + row0)) = make_uint4(pl[0], pl[1], pl[2], pl[3]);
-          if (valid < 128 && row0 == 0) {
+          *reinterpret_cast<uint4*>(column(0)) = make_uint4(ph[0], ph[1], ph[2], ph[3]);
+          *reinterpret_cast<uint4*>(column(R)) = make_uint4(pl[0], pl[1], pl[2], pl[3]);
+          if (valid < 128) {
             // rows behind the sequence may hold anything: they become zeros before the second product reads them
             const int n = 2 * pages + 1, vslot = n % SLOTS;
             ok = wait_warp(bar(C::B_FULL + vslot), (n / SLOTS) & 1, guard, 0xc34);
@@ -698,10 +686,10 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
         }
         float* sm = sums + (ends & 1) * C::SOFTMAX_WARPS * 16;
         const float sum = row_sums(l, lane);
-        if (lane < 16) sm[quarter * 16 + lane] = sum;
+        if (lane < 16) sm[warp * 16 + lane] = sum;
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(C::B_SUM + 2 * wg + (ends & 1)));
-        ok = wait_warp(bar(C::B_SUM + 2 * wg + (ends & 1)), (ends >> 1) & 1, guard, 0xc35);
+        if (lane == 0) mbar_arrive(bar(C::B_SUM + (ends & 1)));
+        ok = wait_warp(bar(C::B_SUM + (ends & 1)), (ends >> 1) & 1, guard, 0xc35);
         ++ends;
         if (!ok) break;
         const int token0 = info[0].z, rows = info[0].w * p.group, head = info[1].x, place = info[1].y;
@@ -712,19 +700,18 @@ __global__ void __launch_bounds__(Config<R_>::THREADS, Config<R_>::CTAS)
           if (lane < 16) factors[lane] = sum_row == 0.f ? 0.f : 1.f / sum_row;
           __syncwarp();
           __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.a.out) + first * 128 + key;
-          const int* at = row_out + row0;
 #pragma unroll
           for (int j = 0; j < 16; ++j)
-            if (row0 + j < rows) out[at[j]] = __float2bfloat16(acc[j] * factors[j]);
-          if (p.a.lse && quarter == 0 && lane < 16 && row0 + lane < rows)
-            p.a.lse[first + (at[lane] >> 7)] = sum_row == 0.f ? -INFINITY : (m + log2f(sum_row)) * 0.6931471805599453f;
+            if (j < rows) out[row_out[j]] = __float2bfloat16(acc[j] * factors[j]);
+          if (p.a.lse && warp == 0 && lane < rows)
+            p.a.lse[first + (row_out[lane] >> 7)] = sum_row == 0.f ? -INFINITY : (m + log2f(sum_row)) * 0.6931471805599453f;
         } else {
-          float* part = p.part_o + (static_cast<long long>(place) * R + row0) * 128 + key;
+          float* part = p.part_o + static_cast<long long>(place) * R * 128 + key;
 #pragma unroll
           for (int j = 0; j < 16; ++j)
-            if (row0 + j < rows) part[j * 128] = acc[j];
-          if (quarter == 0 && lane < 16)
-            *reinterpret_cast<float2*>(p.part_ml + (static_cast<long long>(place) * R + row0 + lane) * 2) = make_float2(m, sum_row);
+            if (j < rows) part[j * 128] = acc[j];
+          if (warp == 0 && lane < 16)
+            *reinterpret_cast<float2*>(p.part_ml + (static_cast<long long>(place) * R + lane) * 2) = make_float2(m, sum_row);
           if (warp == 0 && lane == 0) {
             int* meta = p.part_meta + 8 * place;
             *reinterpret_cast<int4*>(meta) = make_int4(1, info[1].z, info[1].w, token0);
@@ -856,22 +843,24 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const Par
   }
 }
 
-// Tokens that share a pass over the pages: as many as 128 rows hold, a power of two, no more than there are.
+// Tokens that share a pass over the pages, a power of two: as many as 128 rows hold, no more than there are. Up to 32 rows
+// items of 16 rows read the pages twice (the second time from the L2 cache): the kernel for 16 rows does so quicker than the wide
+// one goes once over them, which works on 128 rows always, and requests with fewer tokens need one item. Measured, 32
+// requests of up to 8 tokens and 8192 keys, 4 heads to each of 8 KV heads: 67 us as 16 rows, 76 us in a variant for 32, 130 us
+// in the wide one; 16 heads, lists of 16 pages for tiles of 16 tokens (4 prompts of 512 to 1024): 181 us in a variant for 64
+// rows, 108 us in the wide one.
 static int pack_of(int group, int tile, int max_q, bool listed) {
   int pack = 1;
   while (2 * pack * group <= WIDE_ROWS && pack < max_q && (!listed || 2 * pack <= tile)) pack *= 2;
+  if (group <= R && pack * group <= 2 * R)
+    while (pack * group > R) pack /= 2;
   return pack;
 }
-// Rows of an item at most. The kernels for 16 and 32 rows have keys on the M dimension and multiply the codes as they are: what
-// they pay for a page grows with the rows. The wide kernel converts a page to f16 first, always for 128 rows. Measured: 4 heads
-// and up to 8 new tokens, 32 rows (32 requests of up to 8192 keys, 8 KV heads): 77 us here, 130 us there; lists of tiles of 16
-// tokens, 16 heads (4 prompts of 512 to 1024 tokens, 16 pages a list): 181 us as items of 64 rows here, 128 us as 128 rows there.
-static int rows_of(int used) { return used <= 16 ? 16 : used <= 32 ? 32 : WIDE_ROWS; }
-static int ctas_of(int rows, int sm_count) { return sm_count * (rows == 16 ? Config<16>::CTAS : rows == 32 ? Config<32>::CTAS : WIDE_CTAS); }
+static int rows_of(int used) { return used <= R ? R : WIDE_ROWS; }
+static int ctas_of(int rows, int sm_count) { return sm_count * (rows == R ? Config::CTAS : WIDE_CTAS); }
 
-template <int R>
 static int launch_narrow(const Params& p, DeviceCtx* ctx, cudaStream_t stream) {
-  using C = Config<R>;
+  using C = Config;
   const PagedAttentionArgs& a = p.a;
   CUtensorMap km, vm;
   const cuuint64_t dims[2] = {128, static_cast<cuuint64_t>(a.pages) * a.hkv * 128};
@@ -881,13 +870,12 @@ static int launch_narrow(const Params& p, DeviceCtx* ctx, cudaStream_t stream) {
     if (encode_tiled(i ? &vm : &km, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(i ? a.v : a.k), dims, strides, box, steps,
                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B))
       return set_error(SB_ERR_CUDA, "tensor map of the cache pages");
-  constexpr int KERNEL = R == 16 ? 4 : 6;
-  if (!ctx->paged_attr[KERNEL]) {
-    if (cudaFuncSetAttribute(paged_attention_kernel<R>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
+  if (!ctx->paged_attr[4]) {
+    if (cudaFuncSetAttribute(paged_attention_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
       return set_error(SB_ERR_CUDA, "shared memory of the paged attention");
-    ctx->paged_attr[KERNEL] = 1;
+    ctx->paged_attr[4] = 1;
   }
-  paged_attention_kernel<R><<<p.ctas, C::THREADS, C::SMEM, stream>>>(km, vm, p, ctx->status);
+  paged_attention_kernel<<<p.ctas, C::THREADS, C::SMEM, stream>>>(km, vm, p, ctx->status);
   return check_kernel_launch();
 }
 
@@ -912,8 +900,7 @@ int launch_paged_attention(const PagedAttentionArgs& a, cudaStream_t stream) {
   p.part_o = static_cast<float*>(a.workspace);
   p.part_ml = p.part_o + 2LL * p.ctas * rows * 128;
   p.part_meta = reinterpret_cast<int*>(p.part_ml + 2LL * p.ctas * rows * 2);
-  const int rc = rows == 16 ? launch_narrow<16>(p, ctx, stream)
-                 : rows == 32 ? launch_narrow<32>(p, ctx, stream) : launch_paged_wide(p, ctx->status, ctx, stream);
+  const int rc = rows == R ? launch_narrow(p, ctx, stream) : launch_paged_wide(p, ctx->status, ctx, stream);
   if (rc) return rc;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -20,7 +20,7 @@ constexpr int FIRST = 1, LAST = 2, STOP = 4;      // first batch of an item, las
 struct Params {
   PagedAttentionArgs a;
   int group, pack, pack_shift, tile_shift, ctas;
-  int rows;                                       // of an item at most: 16, 32 or 128 (wide kernel)
+  int rows;                                       // of an item at most: 16, or 128 (wide kernel)
   float* part_o;                                  // [2 ctas, rows, 128]
   float* part_ml;                                 // [2 ctas, rows, 2]
   int* part_meta;                                 // [2 ctas, 8]
