@@ -6,9 +6,10 @@
 //
 // Mathematics. The codes of a page become f16, exactly, on their way into shared memory. A query row is scaled by a power of
 // two (largest feature in [128, 256)) and is exact in f16 but for features below 2^-22 of the largest, which lose up to 2^-33
-// of it. The page's key scale joins the row's factor of the softmax; the page's value scale, relative to the largest of the
-// item so far, its probabilities: p = exp2(x - m + 6) v_scale / v_ref, f16 (2^-11, floor 2^-30 of the largest weight). O stays
-// in tensor memory and is rescaled where a row's maximum rises by more than 2^8, or v_ref rises.
+// of it. The page's key scale joins the row's factor of the softmax. Outputs are sums of exp2(x + log2 v_scale - o + 6) and the
+// codes, the weight in f16 (2^-11, floor 2^-31 of the row's largest): a page whose values are huge and whose weights are nothing
+// costs the others no bits. Sums are kept relative to m. m and o are maxima of a row, of x and of x + log2 v_scale, that follow
+// where those rise by more than 8. O stays in tensor memory and is rescaled when o follows.
 //
 // Two threads of the softmax warps own a row, 64 keys each: S is read once, maximum and sum need one exchange between two
 // warps. (One thread a row, two passes over S and two CTAs to an SM took 6500 cycles a step; the narrow kernel's threads own
@@ -436,7 +437,7 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
     bool ok = true, fresh = true, odd_values = false;
     uint32_t batches = 0;
     int items = 0, ends = 0, pages = 0, joint = 0;       // joint: pages of which this warp had rows
-    float m = -INFINITY, l = 0.f, f_row = 0.f, v_ref = 0.f;
+    float m = -INFINITY, o_ref = -INFINITY, l = 0.f, f_row = 0.f;          // what l and O are relative to
     while (ok) {
       const uint32_t e = batches % BATCHES;
       ok = wait_warp(bar(B_INFO_FULL + e), (batches / BATCHES) & 1, guard, 0xd30);
@@ -447,8 +448,8 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
       if (flags & FIRST) {
         fresh = true;
         odd_values = false;
-        m = -INFINITY;
-        l = v_ref = 0.f;
+        m = o_ref = -INFINITY;
+        l = 0.f;
       }
       const bool idle = 32 * quarter >= rows;     // none of this warp's rows is one
 #pragma unroll 1
@@ -490,27 +491,32 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
           top = fmaxf(top, maxima[(2 * turn + (half ^ 1)) * 128 + row]);
           float f = f_row * __int_as_float(info[2 + step].z);
           if (f == 0.f) f = 1e-37f;               // hidden keys stay hidden with a scale of 0
-          const float mu = top == -INFINITY ? -INFINITY : top * f, vs = __int_as_float(info[2 + step].w);
-          float keep = 1.f;                       // of l and O
+          const bool none = top == -INFINITY;
+          const float mu = none ? -INFINITY : top * f;
           if (m == -INFINITY) {
             m = mu;
           } else if (mu - m > 8.f) {
-            keep = ex2_approx(m - mu);
+            l *= ex2_approx(m - mu);
             m = mu;
           }
-          l *= keep;
-          if (vs > v_ref) {
-            keep *= v_ref / vs;                   // (0 at first)
-            v_ref = vs;
+          const float log_v = __log2f(__int_as_float(info[2 + step].w)), reach = none ? -INFINITY : mu + log_v;
+          float keep = 1.f;                       // of O
+          if (o_ref == -INFINITY) {
+            o_ref = reach;
+          } else if (reach - o_ref > 8.f) {
+            keep = ex2_approx(o_ref - reach);
+            o_ref = reach;
           }
           if (!fresh && __any_sync(0xffffffffu, keep != 1.f)) {
             ok = wait_warp(bar(B_V_EMPTY + (b ^ 1)), ((pages - 1) >> 1) & 1, guard, 0xd34);       // PV of the page before
             if (!ok) break;
             scale_output(t_row + O_COLUMN + 64 * half, keep);
           }
-          const float ratio = vs == v_ref ? 1.f : vs == 0.f ? 0.f : __fdividef(vs, v_ref);      // at most 1; NaN stays
-          const float offset = LIFT - (m == -INFINITY ? 0.f : m);
-          const float2 f2 = make_float2(f, f), o2 = make_float2(offset, offset), r2 = make_float2(ratio, ratio);
+          // One exponential serves both sums where their references are near each other, as they are but for wild scales.
+          const float apart = o_ref - log_v - m;
+          const bool far = !none && !(fabsf(apart) <= 60.f);
+          const float offset = reach == -INFINITY ? -INFINITY : log_v - o_ref + LIFT;
+          const float2 f2 = make_float2(f, f), o2 = make_float2(offset, offset);
           float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
@@ -522,12 +528,18 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
               y.x = ex2_approx(y.x);
               y.y = ex2_approx(y.y);
               sum = add2(sum, y);
-              y = mul2(y, r2);
               h[j] = pack_half2(y.x, y.y);
             }
             tmem_st8(t_row + 128 * b + 32 * half + 8 * c, h);
           }
-          l += sum.x + sum.y;
+          float page_sum = (sum.x + sum.y) * (none ? 1.f : ex2_approx(apart));       // none: 0, or NaN where the scores are
+          if (__any_sync(0xffffffffu, far)) {
+            float x = 0.f;
+#pragma unroll
+            for (int j = 0; j < 64; ++j) x += ex2_approx(fmaf(__uint_as_float(s[j >> 5][j & 31]), f, LIFT - m));
+            if (far) page_sum = x;
+          }
+          l += page_sum;
           tc_wait_st();
           tc_fence_before();
         }
@@ -557,7 +569,7 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
           ok = wait_warp(bar(B_SUM + quarter), ends & 1, guard, 0xd37);
           if (!ok) break;
           const float total = sum_at[row] + sum_at[128 + row];
-          const float by = total == 0.f ? 0.f : place >= 0 ? v_ref : v_ref / total;
+          const float of = ex2_approx(o_ref - m), by = total == 0.f ? 0.f : place >= 0 ? of : of / total;
           const long long out_row = (static_cast<long long>(token0) + token) * p.a.hq + head * p.group + g;
           const int* nan_at = reinterpret_cast<const int*>(gbase + OFF_NAN) + (items & 7) * 128 + 64 * half;
 #pragma unroll 1

@@ -292,7 +292,7 @@ def _random_ids(seed, hkv, lens, seq, topk, tile, total):
     return ids
 
 
-def _check_attention(sp, q, c, table, seq, cu, ids=None, tile=1, causal=True, scale=None, max_q=None, gpu_q=None):
+def _check_attention(sp, q, c, table, seq, cu, ids=None, tile=1, causal=True, scale=None, max_q=None, gpu_q=None, floor=0.0, tiny=0.0):
     cache = _on_gpu(sp, c)
     total, hq = q.shape[:2]
     out = torch.full((total, hq, 128), 7.0, dtype=torch.bfloat16, device="cuda")
@@ -318,6 +318,8 @@ def _check_attention(sp, q, c, table, seq, cu, ids=None, tile=1, causal=True, sc
     # Outputs: each probability carries exp(2 score error) and half a step of its 8-bit mantissa (2^-8), the output half a
     # step of bf16 (2^-8).
     bound = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2 * score[..., None]) * spread * 1.01 + 1e-30
+    if floor:
+        bound = bound + floor * spread.nan_to_num(0).amax(-1, keepdim=True) + tiny
     assert ((out - want).abs()[ok] <= bound[ok]).all(), ((out - want).abs() / bound)[ok].max()
     return out, lse
 
@@ -575,3 +577,92 @@ def test_a_step_in_a_graph(sp):
         for x, y in zip(got, want):
             assert torch.equal(x, y)
         assert torch.equal(_bits(cache[0].k), _bits(cache[1].k)) and torch.equal(cache[0].k_scale, cache[1].k_scale)
+
+
+# ------------------------------------------------------------------ items of many rows
+_MANY_ROWS = [(1, 16, [20, 3], [700, 150]), (2, 40, [3, 1, 2], [390, 129, 300]), (1, 64, [5], [513])]
+
+
+@pytest.mark.parametrize("hkv,group,lens,seq", _MANY_ROWS)
+def test_attention_of_many_rows_special_scores(sp, hkv, group, lens, seq):
+    q, c, table, s, cu = _problem(31 + group, hkv, group, lens, seq)
+    # The weights of these items have 16 bits, 2^6 and more for the row's largest product W of probability and scale: one below
+    # 2^-14 is off by 2^-25, half the smallest step, so by 2^-31 W. An output sums that over its keys, times codes of 448 at
+    # most. W times the largest code of its key is among the row's spreads. A
+    # probability below 2^-126 of the row's largest is 0 where parts are joined in 32 bits, whatever its value's scale.
+    floor = max(seq) * 448 * 2.0 ** -31 / c["v"].float().abs().amax(-1).min().item()
+    first, second = int(table[0, 0]), int(table[0, 1])
+    for scales in ((1.0, 1e4, 1e30, 1.0), (1e4, 1.0, 1.0, 1e30), (1.0, 1.0, 1e-30, 1e30), (1.0, 1.0, 0.0, 1.0), (0.0, 1.0, 1.0, 0.0),
+                   (30.0, 60.0, 2.0, 3.0), (1.0, 1.0, 1.0, 0.0)):
+        c["k_scale"][first], c["k_scale"][second], c["v_scale"][first], c["v_scale"][second] = scales
+        tiny = max(seq) * 448 * 2.0 ** -126 * max(scales[2:])
+        _check_attention(sp, q, c, table, s, cu, max_q=max(lens), floor=floor, tiny=tiny)
+        _check_attention(sp, q, c, table, s, cu, max_q=max(lens), causal=False, floor=floor, tiny=tiny)
+    c["v_scale"][:] = 0.0
+    _check_attention(sp, q, c, table, s, cu, max_q=max(lens))
+    c["v_scale"][:] = 1.0
+    q[0, 1] = 0
+    q[-1, group - 1, 7] = math.nan                                     # a row of NaN stays by itself
+    _check_attention(sp, q, c, table, s, cu, max_q=max(lens), scale=-0.2, floor=floor)
+
+
+@pytest.mark.parametrize("hkv,group,lens,seq", _MANY_ROWS)
+def test_attention_of_many_rows_hidden_nan(sp, hkv, group, lens, seq):
+    """NaN codes in keys and values that some of an item's rows see, and behind the sequence."""
+    q, c, table, s, cu = _problem(37 + group, hkv, group, lens, seq)
+    want = _check_attention(sp, q, c, table, s, cu, max_q=max(lens))
+    nan = torch.tensor(0x7F, dtype=torch.uint8)
+    for name in ("k", "v"):
+        bits = c[name].view(torch.uint8)
+        for r, n in enumerate(seq):
+            if n % PAGE:
+                bits[int(table[r, n // PAGE]), :, n % PAGE:] = nan
+    got = _check_attention(sp, q, c, table, s, cu, max_q=max(lens))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    last = seq[0] - 1                                                  # only the last token of request 0 sees it
+    for name in ("k", "v"):
+        broken = {n: t.clone() for n, t in c.items()}
+        broken[name].view(torch.uint8)[int(table[0, last // PAGE]), hkv - 1, last % PAGE, 77] = nan
+        out, _ = _check_attention(sp, q, broken, table, s, cu, max_q=max(lens))
+        assert out[lens[0] - 1].isnan().any() and torch.equal(out[:lens[0] - 1], want[0][:lens[0] - 1])
+
+
+def test_attention_of_many_short_items(sp):
+    """Items of a page each: the roles of a CTA are items apart. The same bits every time, whatever the hint."""
+    lens, seq = [9, 1, 2, 2, 0, 35, 35, 0, 19, 0], [9, 1327, 2, 122, 101, 1401, 287, 0, 19, 1151]
+    q, c, table, s, cu = _problem(41, 2, 40, lens, seq)
+    for max_q in (1, None):
+        _check_attention(sp, q, c, table, s, cu, max_q=max_q)
+        cache, args = _on_gpu(sp, c), [t.cuda() for t in (table, s, cu)]
+        first = sp.paged_attention(q.cuda(), cache, *args, max_seqlen_q=max_q)
+        gq = q.cuda()
+        for _ in range(200):
+            assert torch.equal(sp.paged_attention(gq, cache, *args, max_seqlen_q=max_q), first)
+
+
+def test_attention_of_many_rows_in_a_graph_on_another_stream_and_twice_at_once(sp):
+    q, c, table, s, cu = _problem(43, 1, 8, [70, 16, 1], [5000, 900, 20])
+    ids = _random_ids(3, 1, [70, 16, 1], [5000, 900, 20], 6, 16, 87).cuda()
+    cache, args, gq = _on_gpu(sp, c), [t.cuda() for t in (table, s, cu)], q.cuda()
+    for kw in (dict(), dict(ids=ids, tile=16)):
+        want = sp.paged_attention(gq, cache, *args, **kw)
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        torch.cuda.synchronize()
+        got = []
+        for _ in range(10):
+            for st in streams:
+                with torch.cuda.stream(st):
+                    got.append(sp.paged_attention(gq, cache, *args, **kw))
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, want) for g in got)
+        out, graphs = torch.empty_like(want), []
+        for _ in range(2):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                sp.paged_attention(gq, cache, *args, out=out, **kw)
+            graphs.append(g)
+        for g in graphs + graphs:
+            out.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
