@@ -27,6 +27,11 @@
 // CTA (two to an SM, so that one's exchanges and waits lie under the other's exponentials): four softmax warps, a loader warp
 // (TMA, one 16 KB tile of K or V to a slot of a ring), an MMA warp, two warps that bring and split the queries of the next item.
 // What the loader tells of items and pages goes through a ring of its own, in batches of 32 pages.
+//
+// What bounds it: HBM where pages are read once by 16 rows of heads (64 requests of 8192 to 32768 keys, 4 KV heads of 16: 1.41 GB
+// in 220 us, 6.4 TB/s; with 64 listed pages each 0.54 GB in 98 us, 5.5 TB/s). The softmax, about 1400 cycles a page and CTA pair,
+// is just under that, and bounds items whose pages come from the L2 cache. One row of 1 Mi keys: 58 us, 8 of them the merge of
+// its parts. A call of 6 pages takes 12.5 us: latencies of two launches, of finding a share and of one page's chain.
 #include "paged_attention.cuh"
 
 namespace sb {

@@ -11,14 +11,18 @@
 // costs the others no bits. Sums are kept relative to m. m and o are maxima of a row, of x and of x + log2 v_scale, that follow
 // where those rise by more than 8. O stays in tensor memory and is rescaled when o follows.
 //
-// Two threads of the softmax warps own a row, 64 keys each: S is read once, maximum and sum need one exchange between two
-// warps. (One thread a row, two passes over S and two CTAs to an SM took 6500 cycles a step; the narrow kernel's threads own
-// keys, and a step of 64 rows took it 3300.)
+// Two threads of the softmax warps own a row, 64 keys each: S is read once, the maximum and the sum need one exchange between two
+// warps. (One thread a row, two passes over S: 138 us with two CTAs to an SM, 127 us with two groups of warps at alternate pages;
+// this 108.)
 //
-// CTA (one to an SM): eight softmax warps; eight that scale an item's queries and convert a page's codes
-// from a ring in shared memory; an MMA warp, which
-// issues QK of a page ahead of PV of the page before; a warp that walks over the share's pages and one that brings them (bulk
-// copies, a tile of K or V is 16 KB in a row).
+// What bounds it: a page's chain of softmax steps, 3000 cycles (exponentials 1400, of which the MUFU unit is taken 1024, maximum
+// and exchange 600, factors 450, hand-over 400), where its two products take 1000. 4 prompts of 512 to 1024 tokens, 16 heads,
+// lists of 16 pages for tiles of 16 tokens (50 GFLOP): 108 us, 0.47 PFLOP/s; an item's end costs two pages' time.
+//
+// CTA (one to an SM): eight softmax warps; eight that scale an item's queries and convert a page's codes from a ring in shared
+// memory, four K and four V; an MMA warp, which issues QK of a page ahead of PV of the page before; a warp that walks over the
+// share's pages and one that brings them (bulk copies, a tile of K or V is 16 KB in a row). A role may be a page or two ahead of
+// another, and a wait tells only one phase from the next: barriers that such roles share are kept by page or item.
 #include "paged_attention.cuh"
 
 namespace sb {
