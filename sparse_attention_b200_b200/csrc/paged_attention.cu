@@ -626,10 +626,10 @@ __global__ void __launch_bounds__(Config::THREADS, Config::CTAS)
           if (unset) m = mu;
           if (lane < 16) {
             const float w = none ? 0.f : ex2_approx(mu - m);
-            factors[lane] = f;
+            factors[lane] = none ? 1.f : f;          // (a scale may be NaN)
             factors[16 + lane] = none ? 0.f : 8.f - mu;
             factors[32 + lane] = w;
-            factors[48 + lane] = w * __int_as_float(x[3]) * 0.00390625f;
+            factors[48 + lane] = none ? 0.f : w * __int_as_float(x[3]) * 0.00390625f;
           }
           __syncwarp();
           uint32_t ph[4], pl[4];

@@ -496,6 +496,7 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
           float f = f_row * __int_as_float(info[2 + step].z);
           if (f == 0.f) f = 1e-37f;               // hidden keys stay hidden with a scale of 0
           const bool none = top == -INFINITY;
+          if (none) f = 1.f;                      // (the page's scale may be NaN)
           const float mu = none ? -INFINITY : top * f;
           if (m == -INFINITY) {
             m = mu;

@@ -666,3 +666,47 @@ def test_attention_of_many_rows_in_a_graph_on_another_stream_and_twice_at_once(s
             g.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("hkv,group,lens,seq", [(2, 4, [4], [130]), (1, 40, [4], [130])])
+def test_attention_scale_of_a_page_that_some_tokens_do_not_see(sp, hkv, group, lens, seq):
+    q, c, table, s, cu = _problem(47, hkv, group, lens, seq)
+    want = _check_attention(sp, q, c, table, s, cu)
+    for name in ("k_scale", "v_scale"):
+        for bad in (math.nan, math.inf):
+            broken = {n: t.clone() for n, t in c.items()}
+            broken[name][int(table[0, 1])] = bad                       # tokens 2 and 3 see the second page
+            cache = _on_gpu(sp, broken)
+            for max_q in (1, 4):
+                out, lse = sp.paged_attention(q.cuda(), cache, table.cuda(), s.cuda(), cu.cuda(), max_seqlen_q=max_q,
+                                              return_lse=True)
+                assert torch.equal(out[:2].cpu().double(), want[0][:2]) and torch.equal(lse[:2].cpu().double(), want[1][:2])
+
+
+@pytest.mark.parametrize("group,tokens", [(4, 1), (16, 8)])
+def test_attention_of_shares_of_many_pages(sp, group, tokens):
+    """More than 32 pages of an item in a share. Requests are alike, over the same pages."""
+    hkv, batch, keys = 2, 64, 64 * PAGE - 5
+    q, c, table, s, cu = _problem(53, hkv, group, [tokens], [keys])
+    want, want_lse, spread, size = ref.paged_attention(q, c["k"], c["v"], c["k_scale"], c["v_scale"], table, s, cu)
+    lens = [tokens] * (batch * 5)
+    out, lse = sp.paged_attention(q.repeat(len(lens), 1, 1).cuda(), _on_gpu(sp, c), table.repeat(len(lens), 1).cuda(),
+                                  s.repeat(len(lens)).cuda(), _cu(lens).cuda(), max_seqlen_q=tokens, return_lse=True)
+    sp.device_status()
+    out = out.view(len(lens), tokens, hkv * group, 128).cpu().double()
+    lse = lse.view(len(lens), tokens, hkv * group).cpu().double()
+    # as in _check_attention
+    score = 2.0 ** -15 * size + 1e-6
+    assert ((lse - want_lse).abs() <= score + 2.0 ** -20 * want_lse.abs()).all()
+    bound = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2 * score[..., None]) * spread * 1.01 + 1e-30
+    assert ((out - want).abs() <= bound).all()
+
+
+def test_attention_of_many_rows_strided_and_padded(sp):
+    q, c, table, s, cu = _problem(59, 2, 4, [30, 12], [200, 300])
+    q = torch.cat([q, torch.full((6, 8, 128), math.nan, dtype=torch.bfloat16)])
+    _check_attention(sp, q, c, table, s, cu)                           # rows behind the last token stay
+    fused = torch.full((48, 14, 136), math.nan, dtype=torch.bfloat16)
+    fused[:, 3:11, :128] = q
+    _check_attention(sp, q, c, table, s, cu, scale=0.3, gpu_q=fused.cuda()[:, 3:11, :128])
+    _check_attention(sp, q, c, table, s, cu, scale=0.0)
