@@ -577,7 +577,7 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
           const float of = ex2_approx(o_ref - m), by = total == 0.f ? 0.f : place >= 0 ? of : of / total;
           const long long out_row = (static_cast<long long>(token0) + token) * p.a.hq + head * p.group + g;
           const int* nan_at = reinterpret_cast<const int*>(gbase + OFF_NAN) + (items & 7) * 128 + 64 * half;
-#pragma unroll 1
+#pragma unroll
           for (int c = 0; c < 4; ++c) {
             uint32_t o[16];
             if (fresh) {
