@@ -599,6 +599,7 @@ __global__ void __launch_bounds__(Config::THREADS, Config::CTAS)
           if (f == 0.f) f = 1e-37f;                  // hidden keys stay hidden with a scale of 0
           const bool none = top == -INFINITY, unset = m == -INFINITY;
           float mu = none ? -INFINITY : fmaf(fabsf(top), 0.00394f, top) * f;       // 2^-8 and a little
+          float over = 1.f;                          // 0: s is relative to mu already
           // The sums stay relative to the item's first page: fp32 has room for 2^40 above it, and what lies below loses nothing.
           if (__any_sync(0xffffffffu, !none && (fabsf(mu) > 100.f || (!unset && mu - m > 40.f)))) {
             // Rare: scores above that, or so large that the rounding up is more than a factor of 1.5. The maxima in fp32; all
@@ -613,21 +614,28 @@ __global__ void __launch_bounds__(Config::THREADS, Config::CTAS)
             top = fmaxf(fmaxf(exact[r16], exact[16 + r16]), fmaxf(exact[32 + r16], exact[48 + r16]));
             if (!none) mu = top * f;
             const bool jump = !unset && mu - m > 40.f;
-            if (lane < 16) factors[lane] = jump ? ex2_approx(m - mu) : 1.f;
+            if (lane < 16) {
+              factors[lane] = jump ? ex2_approx(m - mu) : 1.f;
+              factors[16 + lane] = none ? 0.f : top;
+            }
             if (jump) m = mu;
             __syncwarp();
+            // The scores relative to their maximum before they are scaled: s f - mu in one rounding is what mu was rounded by at
+            // the maximum, more than the exponent's range where scores are huge.
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
               acc[j] *= factors[j];
               l[j] *= factors[j];
+              s[j] -= factors[16 + j];
             }
+            over = 0.f;
             __syncwarp();
           }
           if (unset) m = mu;
           if (lane < 16) {
             const float w = none ? 0.f : ex2_approx(mu - m);
             factors[lane] = none ? 1.f : f;          // (a scale may be NaN)
-            factors[16 + lane] = none ? 0.f : 8.f - mu;
+            factors[16 + lane] = none ? 0.f : fmaf(-over, mu, 8.f);
             factors[32 + lane] = w;
             factors[48 + lane] = none ? 0.f : w * __int_as_float(x[3]) * 0.00390625f;
           }

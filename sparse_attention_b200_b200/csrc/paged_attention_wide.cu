@@ -8,8 +8,8 @@
 // two (largest feature in [128, 256)) and is exact in f16 but for features below 2^-22 of the largest, which lose up to 2^-33
 // of it. The page's key scale joins the row's factor of the softmax. Outputs are sums of exp2(x + log2 v_scale - o + 6) and the
 // codes, the weight in f16 (2^-11, floor 2^-31 of the row's largest): a page whose values are huge and whose weights are nothing
-// costs the others no bits. Sums are kept relative to m. m and o are maxima of a row, of x and of x + log2 v_scale, that follow
-// where those rise by more than 8. O stays in tensor memory and is rescaled when o follows.
+// costs the others no bits. Sums are kept relative to m. m and o are maxima of a row, of x and of x + log2 v_scale (counted from
+// m), that follow where those rise by more than 8. O stays in tensor memory and is rescaled when o follows.
 //
 // Two threads of the softmax warps own a row, 64 keys each: S is read once, the maximum and the sum need one exchange between two
 // warps. (One thread a row, two passes over S: 138 us with two CTAs to an SM, 127 us with two groups of warps at alternate pages;
@@ -47,7 +47,7 @@ constexpr int OFF_FLAG = OFF_BAR + BARS * 8;      // int [2]: for the MMA warp, 
 constexpr int OFF_MISC = (OFF_FLAG + 8 + 15) / 16 * 16;
 constexpr int SMEM = OFF_MISC + 64 + 1024;        // 1024: alignment of the tiles
 static_assert(SMEM <= 227 * 1024 - 512, "shared memory of an SM");
-constexpr int TMEM_COLUMNS = 512;                 // S of two pages (and P over its first half), O
+constexpr int TMEM_COLUMNS = 512;                 // S of two pages (and P over it, 32 columns of every 64), O
 constexpr int O_COLUMN = 256;
 constexpr float LIFT = 6.f;                       // probabilities are exp2(x - m + 6): up to 2^14 before m follows
 
@@ -64,9 +64,11 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
                "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
 }
+// Saturates: scores so huge that their references are rounded by whole numbers may leave a weight above 2^16.
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
+  uint32_t d;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
 }
 // A tile of codes (128 rows of 128 bytes, shared memory) into f16 by 128 threads: eight chunks of 16 codes each. Eight threads
 // of a warp read and write two rows, in 16-byte pieces that meet no bank twice.
@@ -122,6 +124,27 @@ __device__ __forceinline__ void scale_output(uint32_t taddr, float by) {
     for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * by);
     tmem_st16(taddr + c, o);
   }
+}
+
+// Probabilities of 64 keys over their scores, and their sum, with exponents of their own. Scores are taken relative to their
+// maximum before they are scaled: s f - mu in one rounding is what mu was rounded by at the maximum, more than the exponent's
+// range where scores are huge.
+__device__ __forceinline__ float rare_page(uint32_t taddr, float f, float top, float offset, float offset_l) {
+  float sum = 0.f;
+#pragma unroll 1
+  for (int c = 0; c < 4; ++c) {
+    uint32_t s[16], h[8];
+    tmem_ld16(taddr + 16 * c, s);
+    tc_wait_ld();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float x = __uint_as_float(s[2 * j]) - top, y = __uint_as_float(s[2 * j + 1]) - top;
+      sum += ex2_approx(fmaf(x, f, offset_l)) + ex2_approx(fmaf(y, f, offset_l));
+      h[j] = pack_half2(ex2_approx(fmaf(x, f, offset)), ex2_approx(fmaf(y, f, offset)));
+    }
+    tmem_st8(taddr + 8 * c, h);
+  }
+  return sum;
 }
 
 __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Params p, int* status) {
@@ -288,7 +311,7 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
         const bool fresh = second & 1 ? fresh1 : fresh0;
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
-          mma_ts_lo<HI>(tmem + O_COLUMN, tmem + (second & 1) * 128 + kk * 8, v + kk * (2048 >> 4), ID_PV, !fresh || kk > 0);
+          mma_ts_lo<HI>(tmem + O_COLUMN, tmem + (second & 1) * 128 + (kk >> 2) * 64 + (kk & 3) * 8, v + kk * (2048 >> 4), ID_PV, !fresh || kk > 0);
         tc_commit(bar(B_V_EMPTY + (second & 1)));
       }
       __syncwarp();
@@ -441,7 +464,7 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
     bool ok = true, fresh = true, odd_values = false;
     uint32_t batches = 0;
     int items = 0, ends = 0, pages = 0, joint = 0;       // joint: pages of which this warp had rows
-    float m = -INFINITY, o_ref = -INFINITY, l = 0.f, f_row = 0.f;          // what l and O are relative to
+    float m = -INFINITY, o = -INFINITY, l = 0.f, f_row = 0.f;      // what l is relative to, and O, counted from m
     while (ok) {
       const uint32_t e = batches % BATCHES;
       ok = wait_warp(bar(B_INFO_FULL + e), (batches / BATCHES) & 1, guard, 0xd30);
@@ -452,7 +475,7 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
       if (flags & FIRST) {
         fresh = true;
         odd_values = false;
-        m = o_ref = -INFINITY;
+        m = o = -INFINITY;
         l = 0.f;
       }
       const bool idle = 32 * quarter >= rows;     // none of this warp's rows is one
@@ -469,11 +492,12 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
         const int seen = info[2 + step].y, valid = seen & 0xffff, limit = seen >> 16;
         if (!idle) {
           tc_fence_after();
+          const uint32_t t_s = t_row + 128 * b + 64 * half;         // this half's S, and P over it
           if (valid < 128 || limit < 128)
-            mask_scores(t_row + 128 * b + 64 * half, min(p.a.causal ? limit + token : limit, valid) - 64 * half);
+            mask_scores(t_s, min(p.a.causal ? limit + token : limit, valid) - 64 * half);
           uint32_t s[2][32];
-          tmem_ld32(t_row + 128 * b + 64 * half, s[0]);
-          tmem_ld32(t_row + 128 * b + 64 * half + 32, s[1]);
+          tmem_ld32(t_s, s[0]);
+          tmem_ld32(t_s + 32, s[1]);
           tc_wait_ld();
           float top = -INFINITY, other = -INFINITY;
 #pragma unroll
@@ -482,15 +506,12 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
             other = max3(other, __uint_as_float(s[1][j]), __uint_as_float(s[1][j + 1]));
           }
           top = fmaxf(top, other);
-          // Both halves of a row's S are in registers behind this: P goes over the first.
           const int turn = joint & 1;
           maxima[(2 * turn + half) * 128 + row] = top;
-          tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(B_MAX + 2 * quarter + turn));
           ok = wait_warp(bar(B_MAX + 2 * quarter + turn), (joint >> 1) & 1, guard, 0xd33);
           if (!ok) break;
-          tc_fence_after();
           ++joint;
           top = fmaxf(top, maxima[(2 * turn + (half ^ 1)) * 128 + row]);
           float f = f_row * __int_as_float(info[2 + step].z);
@@ -502,49 +523,46 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
             m = mu;
           } else if (mu - m > 8.f) {
             l *= ex2_approx(m - mu);
+            o -= mu - m;
             m = mu;
           }
-          const float log_v = __log2f(__int_as_float(info[2 + step].w)), reach = none ? -INFINITY : mu + log_v;
+          const float log_v = __log2f(__int_as_float(info[2 + step].w)), reach = none ? -INFINITY : mu - m + log_v;
           float keep = 1.f;                       // of O
-          if (o_ref == -INFINITY) {
-            o_ref = reach;
-          } else if (reach - o_ref > 8.f) {
-            keep = ex2_approx(o_ref - reach);
-            o_ref = reach;
+          if (o == -INFINITY) {
+            o = reach;
+          } else if (reach - o > 8.f) {
+            keep = ex2_approx(o - reach);
+            o = reach;
           }
           if (!fresh && __any_sync(0xffffffffu, keep != 1.f)) {
             ok = wait_warp(bar(B_V_EMPTY + (b ^ 1)), ((pages - 1) >> 1) & 1, guard, 0xd34);       // PV of the page before
             if (!ok) break;
             scale_output(t_row + O_COLUMN + 64 * half, keep);
           }
-          // One exponential serves both sums where their references are near each other, as they are but for wild scales.
-          const float apart = o_ref - log_v - m;
-          const bool far = !none && !(fabsf(apart) <= 60.f);
-          const float offset = reach == -INFINITY ? -INFINITY : log_v - o_ref + LIFT;
-          const float2 f2 = make_float2(f, f), o2 = make_float2(offset, offset);
-          float2 sum = make_float2(0.f, 0.f);
+          const float apart = o - log_v;
+          // One exponential serves both sums, but where their references are far apart or the scores huge.
+          if (__any_sync(0xffffffffu, !none && !(fabsf(apart) <= 60.f && fabsf(mu) <= 65536.f))) {
+            l += rare_page(t_s, f, none ? 0.f : top, reach == -INFINITY ? -INFINITY : reach - o + LIFT, none ? -INFINITY : mu - m + LIFT);
+          } else {
+            const float offset = reach == -INFINITY ? -INFINITY : log_v - o + LIFT - m;
+            const float2 f2 = make_float2(f, f), o2 = make_float2(offset, offset);
+            float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t h[8];
+            for (int c = 0; c < 4; ++c) {
+              uint32_t h[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int k = 16 * (c & 1) + 2 * j;
-              float2 y = fma2(make_float2(__uint_as_float(s[c >> 1][k]), __uint_as_float(s[c >> 1][k + 1])), f2, o2);
-              y.x = ex2_approx(y.x);
-              y.y = ex2_approx(y.y);
-              sum = add2(sum, y);
-              h[j] = pack_half2(y.x, y.y);
+              for (int j = 0; j < 8; ++j) {
+                const int k = 16 * (c & 1) + 2 * j;
+                float2 y = fma2(make_float2(__uint_as_float(s[c >> 1][k]), __uint_as_float(s[c >> 1][k + 1])), f2, o2);
+                y.x = ex2_approx(y.x);
+                y.y = ex2_approx(y.y);
+                sum = add2(sum, y);
+                h[j] = pack_half2(y.x, y.y);
+              }
+              tmem_st8(t_s + 8 * c, h);
             }
-            tmem_st8(t_row + 128 * b + 32 * half + 8 * c, h);
+            l += (sum.x + sum.y) * (none ? 1.f : ex2_approx(apart));             // none: 0, or NaN where the scores are
           }
-          float page_sum = (sum.x + sum.y) * (none ? 1.f : ex2_approx(apart));       // none: 0, or NaN where the scores are
-          if (__any_sync(0xffffffffu, far)) {
-            float x = 0.f;
-#pragma unroll
-            for (int j = 0; j < 64; ++j) x += ex2_approx(fmaf(__uint_as_float(s[j >> 5][j & 31]), f, LIFT - m));
-            if (far) page_sum = x;
-          }
-          l += page_sum;
           tc_wait_st();
           tc_fence_before();
         }
@@ -574,41 +592,41 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
           ok = wait_warp(bar(B_SUM + quarter), ends & 1, guard, 0xd37);
           if (!ok) break;
           const float total = sum_at[row] + sum_at[128 + row];
-          const float of = ex2_approx(o_ref - m), by = total == 0.f ? 0.f : place >= 0 ? of : of / total;
+          const float of = ex2_approx(o), by = total == 0.f ? 0.f : place >= 0 ? of : of / total;
           const long long out_row = (static_cast<long long>(token0) + token) * p.a.hq + head * p.group + g;
           const int* nan_at = reinterpret_cast<const int*>(gbase + OFF_NAN) + (items & 7) * 128 + 64 * half;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            uint32_t o[16];
+            uint32_t x[16];
             if (fresh) {
 #pragma unroll
-              for (int j = 0; j < 16; ++j) o[j] = 0;
+              for (int j = 0; j < 16; ++j) x[j] = 0;
             } else {
-              tmem_ld16(t_row + O_COLUMN + 64 * half + 16 * c, o);
+              tmem_ld16(t_row + O_COLUMN + 64 * half + 16 * c, x);
               tc_wait_ld();
             }
 #pragma unroll
-            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(total == 0.f ? 0.f : __uint_as_float(o[j]) * by);
+            for (int j = 0; j < 16; ++j) x[j] = __float_as_uint(total == 0.f ? 0.f : __uint_as_float(x[j]) * by);
             if (odd_values) {
 #pragma unroll
               for (int j = 0; j < 16; ++j)
-                if (nan_at[16 * c + j] < token) o[j] = 0x7fffffffu;
+                if (nan_at[16 * c + j] < token) x[j] = 0x7fffffffu;
             }
             if (row < rows) {
               if (place >= 0) {
                 float4* to = reinterpret_cast<float4*>(p.part_o + (static_cast<long long>(place) * WIDE_ROWS + row) * 128 + 64 * half + 16 * c);
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                  to[j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]), __uint_as_float(o[4 * j + 2]),
-                                      __uint_as_float(o[4 * j + 3]));
+                  to[j] = make_float4(__uint_as_float(x[4 * j]), __uint_as_float(x[4 * j + 1]), __uint_as_float(x[4 * j + 2]),
+                                      __uint_as_float(x[4 * j + 3]));
               } else {
                 uint4* to = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.a.out) + out_row * 128 + 64 * half + 16 * c);
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
-                  to[j] = make_uint4(pack_bf16x2(__uint_as_float(o[8 * j]), __uint_as_float(o[8 * j + 1])),
-                                     pack_bf16x2(__uint_as_float(o[8 * j + 2]), __uint_as_float(o[8 * j + 3])),
-                                     pack_bf16x2(__uint_as_float(o[8 * j + 4]), __uint_as_float(o[8 * j + 5])),
-                                     pack_bf16x2(__uint_as_float(o[8 * j + 6]), __uint_as_float(o[8 * j + 7])));
+                  to[j] = make_uint4(pack_bf16x2(__uint_as_float(x[8 * j]), __uint_as_float(x[8 * j + 1])),
+                                     pack_bf16x2(__uint_as_float(x[8 * j + 2]), __uint_as_float(x[8 * j + 3])),
+                                     pack_bf16x2(__uint_as_float(x[8 * j + 4]), __uint_as_float(x[8 * j + 5])),
+                                     pack_bf16x2(__uint_as_float(x[8 * j + 6]), __uint_as_float(x[8 * j + 7])));
               }
             }
           }

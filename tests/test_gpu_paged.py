@@ -710,3 +710,16 @@ def test_attention_of_many_rows_strided_and_padded(sp):
     fused[:, 3:11, :128] = q
     _check_attention(sp, q, c, table, s, cu, scale=0.3, gpu_q=fused.cuda()[:, 3:11, :128])
     _check_attention(sp, q, c, table, s, cu, scale=0.0)
+
+
+@pytest.mark.parametrize("hkv,group,lens,seq", [(1, 4, [2], [500]), (1, 16, [20], [700])])
+def test_attention_of_huge_scores(sp, hkv, group, lens, seq):
+    """Scores whose differences are beyond 32 bits: the rows stay finite, within the values that they see."""
+    q, c, table, s, cu = _problem(61, hkv, group, lens, seq)
+    for scale in (1e4, 1e6, 1e8, 1e12, 1e30):
+        cache = _on_gpu(sp, c)
+        out, lse = sp.paged_attention(q.cuda(), cache, table.cuda(), s.cuda(), cu.cuda(), scale=scale, return_lse=True)
+        assert out.isfinite().all() and lse.isfinite().all()
+        most = (c["v"].float().abs() * c["v_scale"][..., None, None].float()).max().item()
+        assert out.abs().max() <= 1.01 * most
+        _check_attention(sp, q, c, table, s, cu, scale=scale)
