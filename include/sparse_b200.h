@@ -411,7 +411,7 @@ int sparse_b200_indexer_summary_noalloc(const void* q, const void* k, float* sco
  * select_pages: scores [Hidx, score_pages, total_q] fp32 (sparse_b200_fp4_scores_varlen) -> page_ids. The score of a page for
  * a list is the largest over the list's tokens and the Hidx / Hkv index heads of the KV head. The first `sink` and last
  * `recent` pages that the list's last token sees are always listed, the others by (score descending, page ascending); pages
- * with no score above -inf are not. A list is ascending, -1 behind; rows without a tile are -1.
+ * with no score above -inf are not. A list is ascending, -1 behind; rows without a tile are -1. score_pages <= 51199.
  *
  * paged_attention: q [total_q, Hq, 128] bf16 (strides in elements, multiples of 8) against all pages of its request
  * (page_ids NULL) or the listed ones; causal: token i of n sees keys j <= i + seq_len - n. A page listed twice counts twice,

@@ -30,7 +30,7 @@
 //
 // What bounds it: HBM where pages are read once by 16 rows of heads (64 requests of 8192 to 32768 keys, 4 KV heads of 16: 1.41 GB
 // in 220 us, 6.4 TB/s; with 64 listed pages each 0.54 GB in 98 us, 5.5 TB/s). The softmax, about 1400 cycles a page and CTA pair,
-// is just under that, and bounds items whose pages come from the L2 cache. One row of 1 Mi keys: 58 us, 8 of them the merge of
+// is just under that, and bounds items whose pages come from the L2 cache. One row of 1 Mi keys: 57 us, 7 of them the merge of
 // its parts. A call of 6 pages takes 12.5 us: latencies of two launches, of finding a share and of one page's chain.
 #include "paged_attention.cuh"
 
@@ -823,12 +823,18 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) paged_merge_kernel(const Par
       top = now;
       acc *= keep;
       l *= keep;
-#pragma unroll 8
-      for (int i = 0; i < count; ++i) {
-        const float o = p.part_o[part_row(warp + MERGE_WARPS * (c + i), row) * 128 + d];
-        const float wi = __shfl_sync(0xffffffffu, w, i), li = __shfl_sync(0xffffffffu, ml.y, i);
-        acc = fmaf(wi, o, acc);
-        l = fmaf(wi, li, l);
+      // 16 loads in flight, the last ones too (a loop's remainder would wait for each): lanes beyond the parts have weight 0
+      for (int i0 = 0; i0 < count; i0 += 16) {
+        float o[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          o[j] = i0 + j < count ? p.part_o[part_row(warp + MERGE_WARPS * (c + i0 + j), row) * 128 + d] : 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float wi = __shfl_sync(0xffffffffu, w, i0 + j), li = __shfl_sync(0xffffffffu, ml.y, i0 + j);
+          acc = fmaf(wi, o[j], acc);
+          l = fmaf(wi, li, l);
+        }
       }
     }
     s_acc[warp][lane] = acc;
