@@ -11,7 +11,7 @@
 // What bounds it: a dependent chain of a few loads and two block scans; the arrays are small. Every CTA therefore runs the
 // scans over all requests itself (they sit in L2) instead of waiting for another launch, keeps the sums in shared memory
 // and writes its share of the slots and pages, whose requests it finds by binary search there. 48 requests of a token each:
-// 6.3 us in a graph, 768 requests of up to 128 tokens and 32768 keys (1.2 MB): 10.3 us; the call's host side takes 20.
+// 6.3 us in a graph, 768 requests of up to 128 tokens and 32768 keys (1.2 MB): 10.3 us; the call's host side takes 18.
 #include "internal.h"
 #include "paged.cuh"
 

@@ -147,18 +147,19 @@ def extend_pages(block_table, seq_lens, new_lens, free_pages, free_count, *, tot
     if total_q < 0 or total_pages < 0:
         _bad("table sizes must not be negative")
     with _on(dev):
-        slots = torch.empty(total_q, dtype=torch.int64, device=dev)
-        buffer = torch.empty(4 * batch + 5 + total_pages, dtype=torch.int32, device=dev)
-        seq, cu_q, cu_k, cu_pages, count, status, kv = torch.split_with_sizes(
-            buffer, (batch, batch + 1, batch + 1, batch + 1, 1, 1, total_pages))
-        at, step = buffer.data_ptr(), 4 * batch + 4
+        # one allocation, the 64-bit slots first
+        buffer = torch.empty(2 * total_q + 4 * batch + 5 + total_pages, dtype=torch.int32, device=dev)
+        slots, seq, cu_q, cu_k, cu_pages, count, status, kv = torch.unsafe_split_with_sizes(
+            buffer, (2 * total_q, batch, batch + 1, batch + 1, batch + 1, 1, 1, total_pages))
+        at_slots, step = buffer.data_ptr(), 4 * batch + 4
+        at = at_slots + 8 * total_q
         at_q = at + 4 * batch
         at_count = at_q + 3 * step
         _lib.check(_entry("extend_pages")(
             table, stride, width, seq_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(), free_pages.numel(),
-            free_count.data_ptr(), at, at_q, at_q + step, at_q + 2 * step, at_count + 8, slots.data_ptr(), at_count, at_count + 4,
+            free_count.data_ptr(), at, at_q, at_q + step, at_q + 2 * step, at_count + 8, at_slots, at_count, at_count + 4,
             batch, total_q, total_pages, _stream(dev)))
-    return PageBatch(seq, cu_q, cu_k, cu_pages, kv, slots, count, status)
+    return PageBatch(seq, cu_q, cu_k, cu_pages, kv, slots.view(torch.int64), count, status)
 
 
 def append_tokens(cache, k, v, cu_seqlens_q, slots):
@@ -239,7 +240,7 @@ def paged_attention(q, cache, block_table, seq_lens, cu_seqlens_q, ids=None, *, 
     max_q = total if max_seqlen_q is None else int(max_seqlen_q)
     with _on(dev):
         if out is None:
-            out = torch.empty((total, hq, 128), dtype=torch.bfloat16, device=dev)
+            out = torch.empty_like(q) if q.is_contiguous() else torch.empty((total, hq, 128), dtype=torch.bfloat16, device=dev)
         else:
             _dense("out", out, torch.bfloat16, (total, hq, 128), dev)
             for t in (q, cache.k, cache.v):
