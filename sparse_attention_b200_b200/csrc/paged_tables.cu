@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(THREADS) extend_pages_kernel(
     const int k = granted ? o + n : o;      // o + n <= 128 width, or n == 0
     s_old[r] = o;
     s_taken[r] = granted ? static_cast<int>(before) : -1;
-    if (granted) used = static_cast<int>(before + n_need);
+    if (granted && n_need > 0) used = static_cast<int>(before + n_need);     // (without need: `before` counts refused requests too)
     if (first) seq_out[r] = k;
     mine = add(mine, {n, k, static_cast<int>(min(pages_of(k), static_cast<long long>(width)))});
     before += n_need;
