@@ -399,7 +399,7 @@ int sparse_b200_indexer_summary_noalloc(const void* q, const void* k, float* sco
  * cu_seqlens_q / cu_seqlens_k / cu_page_offsets [B + 1], kv_indices [total_pages] (pages of all requests in order, -1
  * behind), slots [total_q] (page * 128 + row of every new token, -1 behind), free_count_out [1], status [1]: 1 pages ran out,
  * 2 a table row is too short, 4 more new tokens than total_q, 8 more pages than total_pages, 16 a sum is beyond int32 (kept
- * at its largest). The inputs other than block_table stay as they are, so a call may be repeated.
+ * at its largest). The inputs other than block_table stay as they are, so a call may be repeated. B * table_width < 2^31.
  *
  * append_tokens: k, v [total_q, Hkv, 128] bf16 rows (strides in elements, multiples of 8; a row itself is dense) into the
  * pages that slots names: the first token's slot of a request and of each page after it count, rows follow in order. Scale of

@@ -725,6 +725,7 @@ int sparse_b200_extend_pages(int32_t* block_table, int64_t table_stride, int tab
   REQUIRE(total_pages >= 0 && free_capacity >= 0, "negative page count");
   REQUIRE(table_width > 0 && table_width < (1 << 24) && table_stride >= table_width,
           "a table row holds 1 to 2^24 - 1 pages and is at most as long as the row stride");
+  REQUIRE(static_cast<long long>(batch) * table_width < (1LL << 31), "the pages of a step must fit int32 (requests * table width)");
   REQUIRE(seq_lens_out != seq_lens && free_count_out != free_count, "lengths and free count are not updated in place");
   return launch_extend_pages(block_table, table_stride, table_width, seq_lens, new_lens, free_pages, free_capacity,
                              free_count, seq_lens_out, cu_seqlens_q, cu_seqlens_k, cu_page_offsets, kv_indices,

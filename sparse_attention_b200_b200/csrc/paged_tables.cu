@@ -22,7 +22,7 @@ constexpr int THREADS = 256;
 
 struct Sums {
   long long new_tokens, kv_tokens;
-  int pages;
+  int pages;                             // at most batch * width, below 2^31
 };
 
 __device__ __forceinline__ Sums add(const Sums& a, const Sums& b) {
@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(THREADS) extend_pages_kernel(
     const int o = old_of(r), n = new_of(r);
     const int k = granted ? o + n : o;      // o + n <= 128 width, or n == 0
     s_old[r] = o;
-    s_taken[r] = granted ? static_cast<int>(before) : -1;
+    s_taken[r] = granted ? static_cast<int>(before) : -1;      // (needs add up to batch * width at most)
     if (granted && n_need > 0) used = static_cast<int>(before + n_need);     // (without need: `before` counts refused requests too)
     if (first) seq_out[r] = k;
     mine = add(mine, {n, k, static_cast<int>(min(pages_of(k), static_cast<long long>(width)))});
@@ -138,9 +138,10 @@ __global__ void __launch_bounds__(THREADS) extend_pages_kernel(
     if (j >= held) return s_taken[r] < 0 ? -1 : __ldg(free_pages + (available - 1 - s_taken[r] - (j - held)));
     return table[r * table_stride + j];
   };
-  const int stride = gridDim.x * THREADS, start = blockIdx.x * THREADS + tid;
-  const int all_pages = max(s_pages[batch], total_pages);
-  for (int j = start; j < all_pages; j += stride) {
+  const unsigned stride = gridDim.x * THREADS, start = blockIdx.x * THREADS + tid;      // (unsigned: ends may be near 2^31)
+  const unsigned all_pages = max(s_pages[batch], total_pages);
+  for (unsigned i = start; i < all_pages; i += stride) {
+    const int j = static_cast<int>(i);
     int page = -1;
     if (j < s_pages[batch]) {
       const int r = upper_bound(s_pages, batch + 1, j) - 1;
@@ -151,7 +152,8 @@ __global__ void __launch_bounds__(THREADS) extend_pages_kernel(
     }
     if (j < total_pages) kv_indices[j] = page;
   }
-  for (int t = start; t < total_q; t += stride) {
+  for (unsigned i = start; i < static_cast<unsigned>(total_q); i += stride) {
+    const int t = static_cast<int>(i);
     long long slot = -1;
     if (t < s_q[batch]) {
       const int r = upper_bound(s_q, batch + 1, t) - 1;
@@ -180,8 +182,8 @@ int launch_extend_pages(int32_t* table, long long table_stride, int width, const
       return set_error(SB_ERR_CUDA, "shared memory of the page tables kernel");
     ctx->paged_attr[0] = 1;
   }
-  const int most = max(total_q, total_pages);
-  const int grid = max(1, min((most + 4 * THREADS - 1) / (4 * THREADS), ctx->sm_count));
+  const long long most = max(total_q, total_pages);
+  const int grid = static_cast<int>(max(1LL, min((most + 4 * THREADS - 1) / (4 * THREADS), static_cast<long long>(ctx->sm_count))));
   extend_pages_kernel<<<grid, THREADS, smem, stream>>>(table, table_stride, width, seq, added, free_pages, free_capacity,
                                                        free_count, seq_out, cu_q, cu_k, cu_pages, kv_indices, slots,
                                                        free_out, status, batch, total_q, total_pages);

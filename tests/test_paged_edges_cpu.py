@@ -1,0 +1,25 @@
+"""More refusals of the paged serving path at the C boundary: no GPU."""
+import ctypes
+
+import pytest
+
+P, OTHER = ctypes.c_void_p(4096), ctypes.c_void_p(8192)
+I64 = ctypes.c_int64
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from sparse_attention_b200_b200 import _lib
+    return _lib.lib()
+
+
+def _refused(lib, rc, word):
+    from sparse_attention_b200_b200 import _lib
+    assert rc == _lib.ERR_INVALID and word in lib.sparse_b200_last_error(), (rc, lib.sparse_b200_last_error())
+
+
+@pytest.mark.parametrize("batch,width", [(4096, 1 << 19), (300, 1 << 23), (129, (1 << 24) - 1)])
+def test_extend_pages_refuses_more_pages_than_int32(lib, batch, width):
+    """The pages of a step are counted in 32 bits (cu_page_offsets)."""
+    rc = lib.sparse_b200_extend_pages(P, I64(width), width, P, P, P, 4, P, OTHER, P, P, P, P, P, OTHER, P, batch, 4, 4, None)
+    _refused(lib, rc, b"int32")
