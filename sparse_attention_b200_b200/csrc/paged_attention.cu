@@ -579,7 +579,7 @@ __global__ void __launch_bounds__(Config::THREADS, Config::CTAS)
           const uint32_t top = pair_maxima(pairs, lane);
           if (lane < 8) reinterpret_cast<uint32_t*>(maxima + b * C::SOFTMAX_WARPS * 16 + warp * 16)[lane] = top;
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar(C::B_MAX + b));
+          if (!masked && lane == 0) mbar_arrive(bar(C::B_MAX + b));
         }
         // under the other warps' maxima: the output of the page before
         if (pending >= 0) {
@@ -590,6 +590,13 @@ __global__ void __launch_bounds__(Config::THREADS, Config::CTAS)
         asm volatile("" : "+r"(again));              // one copy of add_output for pages and ends
         if (again) {
           const int b = pages & 1;
+          if (masked) {
+            // Behind a page that some rows do not see all of: its probabilities are read by all four warps until its output is
+            // added (visible_sums), and a warp that has the maxima of this page overwrites its own.
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(C::B_MAX + b));
+            masked = 0;
+          }
           ok = wait_warp(bar(C::B_MAX + b), (pages >> 1) & 1, guard, 0xc36);
           if (!ok) break;
           const __nv_bfloat16* mx = maxima + b * C::SOFTMAX_WARPS * 16 + r16;
@@ -692,6 +699,7 @@ __global__ void __launch_bounds__(Config::THREADS, Config::CTAS)
           continue;
         }
         // the item's end
+        masked = 0;
         if (item_pages) {
           __syncwarp();
           if (lane == 0) mbar_arrive(bar(C::B_Q_EMPTY + (items & 1)));

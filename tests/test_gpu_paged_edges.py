@@ -89,3 +89,62 @@ def test_pages_are_neither_lost_nor_made_over_many_steps(sp):
         names = [p for r, h in enumerate(held) for p in table[r, :h].tolist()] + free[:int(count)].tolist()
         assert sorted(names) == list(range(pages))
     assert short
+
+
+# ------------------------------------------------------------------ paged_attention
+def _cache(gen, pages, hkv):
+    codes = lambda: (100 * torch.randn((pages, hkv, PAGE, 128), generator=gen)).clamp(-448, 448).to(torch.float8_e4m3fn)  # noqa: E731
+    scales = lambda: torch.exp2(torch.randint(-9, -5, (pages, hkv), generator=gen).float())  # noqa: E731
+    return dict(k=codes(), v=codes(), k_scale=scales(), v_scale=scales())
+
+
+def _on_gpu(sp, c):
+    return sp.PagedCache.from_tensors(*(c[n].cuda() for n in ("k", "v", "k_scale", "v_scale")))
+
+
+def _alike(sp, n, q, c, table, seq, ids=None, max_q=None, **kw):
+    """out, lse (64 bits) of n requests that are all alike: [n, tokens, Hq, 128], [n, tokens, Hq]. A share then holds whole items,
+    where the pages of one request alone would each be a share's own."""
+    tokens, hq = q.shape[:2]
+    out, lse = sp.paged_attention(q.repeat(n, 1, 1).cuda(), _on_gpu(sp, c), table.repeat(n, 1).cuda(), seq.repeat(n).cuda(),
+                                  _cu([tokens] * n).cuda(), None if ids is None else ids.repeat(1, n, 1).cuda(),
+                                  max_seqlen_q=tokens if max_q is None else max_q, return_lse=True, **kw)
+    sp.device_status()
+    return out.view(n, tokens, hq, 128).cpu().double(), lse.view(n, tokens, hq).cpu().double()
+
+
+def _bounds(want, want_lse, spread, size):
+    """As in test_gpu_paged.py, for queries without features far below their row's largest: a score is a sum of 128 products in
+    32 bits (each addition 2^-24 of the magnitudes at most), a weight carries twice a score's error and 2^-8, an output 2^-8."""
+    score = 2.0 ** -15 * size + 1e-6
+    return 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2 * score[..., None]) * spread * 1.01 + 1e-30, score + 2.0 ** -20 * want_lse.abs()
+
+
+@pytest.mark.parametrize("tokens,seq,key,order", [
+    (3, 129, 127, None), (4, 130, 127, None), (4, 130, 128, None), (4, 257, 255, None), (2, 300, 299, [2, 0, 1]),
+    (4, 300, 297, [2, 1, 0]),
+])
+@pytest.mark.parametrize("group", [1, 4])
+def test_hidden_nan_values_with_further_pages_behind(sp, group, tokens, seq, key, order):
+    """A NaN among the values that some tokens of an item do not see, in a page that is not the item's last: their sums are done
+    again while the item goes on."""
+    gen = torch.Generator().manual_seed(seq + key)
+    hkv, held = 2, -(-seq // PAGE)
+    c = _cache(gen, held, hkv)
+    table, s = torch.randperm(held, generator=gen).to(torch.int32)[None], _i32([seq])
+    q = torch.randn((tokens, hkv * group, 128), generator=gen).to(torch.bfloat16)
+    bits = c["v"].view(torch.uint8)
+    for d in (5, 40, 41, 127):
+        bits[int(table[0, key // PAGE]), :, key % PAGE, d] = 0x7F
+    # a list for all tokens: tile = tokens, whose lists are two rows apart
+    tile = 1 if order is None else tokens
+    ids = None if order is None else _i32(order).expand(hkv, 2, -1).contiguous()
+    oracle = lambda v: ref.paged_attention(q, c["k"], v, c["k_scale"], c["v_scale"], table, s, _cu([tokens]), ids, tile)  # noqa: E731
+    want, want_lse, spread, size = oracle(c["v"])
+    out, lse = _alike(sp, 600, q, c, table, s, ids, tile=tile)
+    assert not want[0].isnan().any() and want[-1].isnan().any()
+    assert torch.equal(out.isnan(), want.isnan().expand_as(out))
+    spread = oracle(torch.nan_to_num(c["v"].double(), 0.0))[2]          # of the rows that do not see it, at its features too
+    bound, bound_lse = _bounds(want, want_lse, spread, size)
+    assert ((out - want).abs() <= bound)[:, ~want.isnan()].all()
+    assert ((lse - want_lse).abs() <= bound_lse).all()
