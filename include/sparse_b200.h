@@ -399,7 +399,9 @@ int sparse_b200_indexer_summary_noalloc(const void* q, const void* k, float* sco
  * cu_seqlens_q / cu_seqlens_k / cu_page_offsets [B + 1], kv_indices [total_pages] (pages of all requests in order, -1
  * behind), slots [total_q] (page * 128 + row of every new token, -1 behind), free_count_out [1], status [1]: 1 pages ran out,
  * 2 a table row is too short, 4 more new tokens than total_q, 8 more pages than total_pages, 16 a sum is beyond int32 (kept
- * at its largest). The inputs other than block_table stay as they are, so a call may be repeated. B * table_width < 2^31.
+ * at its largest). With 4 or 8 the step's tables are cut off: slots and kv_indices hold the first entries, and cu_page_offsets
+ * does not go beyond total_pages, so that who reads kv_indices by it (the scorer) stays within; the requests that are cut have
+ * no meaningful results. The inputs other than block_table stay as they are, so a call may be repeated. B * table_width < 2^31.
  *
  * append_tokens: k, v [total_q, Hkv, 128] bf16 rows (strides in elements, multiples of 8; a row itself is dense) into the
  * pages that slots names: the first token's slot of a request and of each page after it count, rows follow in order. Scale of

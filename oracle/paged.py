@@ -42,6 +42,7 @@ def extend_pages(table, seq, new, free_pages, free_count, total_q, total_pages):
     status |= (4 if cu_q[-1] > total_q else 0) | (8 if cu_p[-1] > total_pages else 0)
     pad = lambda x, size: (x + [-1] * size)[:size]  # noqa: E731
     i32 = lambda x: torch.tensor(x, dtype=torch.int32)  # noqa: E731
+    cu_p = [min(x, total_pages) for x in cu_p]           # kv_indices has no more
     return dict(table=table, seq_lens=i32(seq_out), cu_seqlens_q=i32(cu_q), cu_seqlens_k=i32(cu_k), cu_page_offsets=i32(cu_p),
                 kv_indices=i32(pad(kv, total_pages)), slots=torch.tensor(pad(slots, total_q), dtype=torch.int64),
                 free_count=i32([left]), status=i32([status]))

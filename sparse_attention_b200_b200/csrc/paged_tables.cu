@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(THREADS) extend_pages_kernel(
     if (first) {
       cu_q[r] = saturated(upto.new_tokens);
       cu_k[r] = saturated(upto.kv_tokens);
-      cu_pages[r] = upto.pages;
+      cu_pages[r] = min(upto.pages, total_pages);      // (who reads kv_indices by it stays within)
     }
     upto = add(upto, {n, k, static_cast<int>(min(pages_of(k), static_cast<long long>(width)))});
   }
@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(THREADS) extend_pages_kernel(
     if (first) {
       cu_q[batch] = saturated(upto.new_tokens);
       cu_k[batch] = saturated(upto.kv_tokens);
-      cu_pages[batch] = upto.pages;
+      cu_pages[batch] = min(upto.pages, total_pages);
       *free_out = static_cast<int>(available) - s_used;
       *status = s_status | (upto.new_tokens > total_q ? 4 : 0) | (upto.pages > total_pages ? 8 : 0) |
                 (upto.kv_tokens > 0x7fffffffLL || upto.new_tokens > 0x7fffffffLL ? 16 : 0);

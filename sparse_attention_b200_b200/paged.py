@@ -134,8 +134,8 @@ def extend_pages(block_table, seq_lens, new_lens, free_pages, free_count, *, tot
     [free_count], and the tables of the step. block_table [B, W] is extended in place; everything else is new (PageBatch):
     seq_lens with the new tokens, cu_seqlens_q / cu_seqlens_k / cu_page_offsets [B+1], kv_indices [total_pages], slots
     [total_q] int64, free_count [1], status [1] (STATUS_* bits; 0: all is well). total_q and total_pages are the sizes of the
-    tables; what is behind the last token or page is -1. A request that gets no pages is refused: its length stays, its slots
-    are -1."""
+    tables; what is behind the last token or page is -1, and cu_page_offsets never goes beyond total_pages (STATUS_PAGES says
+    that pages were left out). A request that gets no pages is refused: its length stays, its slots are -1."""
     batch, dev = seq_lens.numel(), seq_lens.device
     if not seq_lens.is_cuda or batch == 0:
         _bad("seq_lens must be a CUDA tensor of at least one request")

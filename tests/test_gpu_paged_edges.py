@@ -72,6 +72,17 @@ def test_large_batches_that_find_too_few_pages(sp, batch, spare):
     _check_extend(sp, old, new, table, free, count, sum(new) + 5, sum(-(-(a + b) // PAGE) for a, b in zip(old, new)) + 3)
 
 
+@pytest.mark.parametrize("old,new,total_pages", [([500], [1], 1), ([10, 20, 300], [700, 300, 1], 4), ([0, 5], [128, 600], 0),
+                                                 ([128] * 300, [1] * 300, 450)])
+def test_page_offsets_stay_within_the_page_list(sp, old, new, total_pages):
+    """What reads kv_indices by cu_page_offsets (the scorer) knows no other size of it. The block table gets all pages."""
+    table, free, count = _tables(random.Random(5), old, 16, 400)
+    got, _ = _check_extend(sp, old, new, table, free, count, sum(new), total_pages)
+    assert int(got.status) == sp.paged.STATUS_PAGES
+    offsets = got.cu_page_offsets.cpu()
+    assert (offsets[1:] >= offsets[:-1]).all() and int(offsets[-1]) == total_pages == got.kv_indices.numel()
+
+
 def test_pages_are_neither_lost_nor_made_over_many_steps(sp):
     rng = random.Random(9)
     batch, width, pages = 300, 12, 700
