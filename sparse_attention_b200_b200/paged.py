@@ -283,16 +283,18 @@ def paged_step(q, k, v, cache, block_table, batch, *, topk=None, tile=1, max_seq
 
 
 def quantize_rows(q, hidx):
-    """Packed rows q [T,Hq,128] bf16 (contiguous) -> NVFP4 query index vectors (codes [T,hidx,64], scales [T,hidx,8]): the
-    mean over the Hq/hidx heads of a group, as indexers.quantize_queries for whole sequences."""
+    """Packed rows q [T,Hq,128] bf16 (strides as everywhere here; rows that are not contiguous are copied first) -> NVFP4 query
+    index vectors (codes [T,hidx,64], scales [T,hidx,8]): the mean over the Hq/hidx heads of a group, as
+    indexers.quantize_queries for whole sequences."""
     _rows("q", q, None)
     total, hq = q.shape[:2]
-    if hq % hidx or not q.is_contiguous():
-        _bad("q must be contiguous and Hq a multiple of the index head count")
+    if hidx < 1 or hq % hidx or hq < hidx:
+        _bad("Hq must be a multiple of the index head count")
     with _on(q.device):
         codes = torch.empty((total, hidx, 64), dtype=torch.uint8, device=q.device)
         scales = torch.empty((total, hidx, 8), dtype=torch.float8_e4m3fn, device=q.device)
         if total:      # T batches of one token
+            q = q.contiguous()
             _lib.check(_lib.lib().sparse_b200_nvfp4_quantize(_lib.ptr(q), _lib.ptr(codes), _lib.ptr(scales), total, hidx,
                                                              hq // hidx, 1, 0, ctypes.c_void_p(_stream(q.device))))
     return codes, scales

@@ -159,3 +159,55 @@ def test_hidden_nan_values_with_further_pages_behind(sp, group, tokens, seq, key
     bound, bound_lse = _bounds(want, want_lse, spread, size)
     assert ((out - want).abs() <= bound)[:, ~want.isnan()].all()
     assert ((lse - want_lse).abs() <= bound_lse).all()
+
+
+# ------------------------------------------------------------------ the whole step
+def _step(sp, lens, old, hkv, group, seed=1, index=True, wide=136):
+    """A step's arguments over a fused projection whose rows are padded: q, k, v (views), cache, table, tables of the step."""
+    gen = torch.Generator().manual_seed(seed)
+    pages = sum(-(-(a + b) // PAGE) for a, b in zip(old, lens)) + 2
+    cache = sp.PagedCache(pages, hkv, index=index)
+    for t in (cache.k, cache.v):
+        t.view(torch.uint8).copy_(torch.randint(0, 0x70, t.shape, generator=gen).to(torch.uint8))
+    if index:
+        cache.k_index.copy_(torch.randint(0, 256, cache.k_index.shape, generator=gen).to(torch.uint8))
+        cache.k_index_scale.view(torch.uint8).fill_(0x38)
+    width = max(-(-(a + b) // PAGE) for a, b in zip(old, lens)) + 1
+    table, at = torch.full((len(lens), width), -1, dtype=torch.int32), 0
+    for r, o in enumerate(old):
+        table[r, :-(-o // PAGE)] = torch.arange(at, at + -(-o // PAGE))
+        at += -(-o // PAGE)
+    table = table.cuda()
+    b = sp.extend_pages(table, _i32(old).cuda(), _i32(lens).cuda(), torch.arange(at, pages, dtype=torch.int32).cuda(),
+                        _i32([pages - at]).cuda(), total_q=sum(lens), total_pages=pages)
+    x = torch.randn((sum(lens), hkv * (group + 2), wide), generator=gen).to(torch.bfloat16).cuda()
+    hq = hkv * group
+    return x[:, :hq, :128], x[:, hq:hq + hkv, :128], x[:, hq + hkv:, :128], cache, table, b
+
+
+def _copy(sp, cache):
+    return sp.PagedCache.from_tensors(*(None if t is None else t.clone() for t in (
+        cache.k, cache.v, cache.k_scale, cache.v_scale, cache.k_index, cache.k_index_scale)))
+
+
+def _same_bits(x, y):
+    return all((a is None and b is None) or torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+               for a, b in zip((x.k, x.v, x.k_scale, x.v_scale, x.k_index, x.k_index_scale),
+                               (y.k, y.v, y.k_scale, y.v_scale, y.k_index, y.k_index_scale)))
+
+
+@pytest.mark.parametrize("topk,tile", [(None, 1), (3, 1), (3, 16)])
+def test_a_step_takes_views_of_a_fused_projection(sp, topk, tile):
+    q, k, v, cache, table, b = _step(sp, [20, 1, 3], [700, 900, 0], 2, 4)
+    other = _copy(sp, cache)
+    kw = dict(topk=topk, tile=tile, max_seqlen_q=20, max_seqlen_k=901)
+    out, ids = sp.paged_step(q, k, v, cache, table, b, **kw)
+    want, want_ids = sp.paged_step(q.contiguous(), k.contiguous(), v.contiguous(), other, table, b, **kw)
+    assert torch.equal(out, want) and _same_bits(cache, other)
+    assert (ids is None and want_ids is None) or torch.equal(ids, want_ids)
+    codes, scales = sp.quantize_rows(q, 2)
+    want = sp.quantize_rows(q.contiguous(), 2)
+    assert torch.equal(codes, want[0]) and torch.equal(scales.view(torch.uint8), want[1].view(torch.uint8))
+    for bad in (0, -2, 3, 16):
+        with pytest.raises(sp.SparseB200Error):
+            sp.quantize_rows(q, bad)
