@@ -14,6 +14,7 @@ import collections
 import contextlib
 import ctypes
 import functools
+import math
 
 import torch
 
@@ -181,6 +182,18 @@ def list_rows(total_q, batch, tile):
     return total_q if tile == 1 else total_q // tile + batch
 
 
+MOST_PAGES = 51199          # of a request whose pages select_pages takes
+
+
+def _check_selection(pages, kv_heads, topk, tile, sink, recent):
+    if tile < 1 or tile > 128 or tile & (tile - 1) or kv_heads < 1 or topk < 1:
+        _bad("tile must be a power of two from 1 to 128, KV heads and topk positive")
+    if sink < 0 or recent < 0 or sink + recent > topk:
+        _bad("sink and recent pages must fit the list")
+    if pages < 1 or pages > MOST_PAGES:
+        _bad(f"the page selection takes 1 to {MOST_PAGES} pages of a request")
+
+
 def select_pages(scores, cu_seqlens_q, seq_lens, *, kv_heads, topk, tile=1, sink=1, recent=1, causal=True, ids=None):
     """scores [Hidx, pages, T] fp32 (fp4_block_scores_varlen) -> ids [kv_heads, list_rows(T, B, tile), topk] int32: for every
     `tile` consecutive tokens of a request the best pages by (score descending, page ascending), written ascending with -1
@@ -191,8 +204,7 @@ def select_pages(scores, cu_seqlens_q, seq_lens, *, kv_heads, topk, tile=1, sink
     dev, batch = scores.device, seq_lens.numel()
     _dense("seq_lens", seq_lens, torch.int32, (batch,), dev)
     _dense("cu_seqlens_q", cu_seqlens_q, torch.int32, (batch + 1,), dev)
-    if tile < 1 or tile & (tile - 1) or kv_heads < 1 or topk < 1:
-        _bad("tile must be a power of two from 1 to 128, KV heads and topk positive")
+    _check_selection(pages, kv_heads, topk, tile, sink, recent)
     shape = (kv_heads, list_rows(total, batch, tile), topk)
     with _on(dev):
         if ids is None:
@@ -216,6 +228,13 @@ def _workspace_bytes(device, hq, hkv, tile, max_q, listed):
     return n
 
 
+def _check_queries(q, cache):
+    rows, hq, hkv = _rows("q", q, None, cache.device), q.shape[1], cache.kv_heads
+    if hq < hkv or hq % hkv or hq // hkv > 64:
+        _bad("Hq must be a multiple of Hkv, at most 64 query heads to a KV head")
+    return rows
+
+
 def paged_attention(q, cache, block_table, seq_lens, cu_seqlens_q, ids=None, *, tile=1, max_seqlen_q=None, causal=True,
                     scale=None, out=None, lse=None, return_lse=False):
     """softmax(scale q k^T) v of q [T,Hq,128] bf16 over the pages of each request (ids=None) or the listed ones (ids
@@ -224,10 +243,8 @@ def paged_attention(q, cache, block_table, seq_lens, cu_seqlens_q, ids=None, *, 
     the last token of out and lse are left as they were. max_seqlen_q: the largest number of new tokens, for how many of them
     share a pass over a page (default: T). scale: default 128^-0.5."""
     hkv, dev, batch = cache.kv_heads, cache.device, seq_lens.numel()
-    rows = _rows("q", q, None, dev)
+    rows = _check_queries(q, cache)
     total, hq = q.shape[:2]
-    if hq < hkv or hq % hkv or hq // hkv > 64:
-        _bad("Hq must be a multiple of Hkv, at most 64 query heads to a KV head")
     _dense("seq_lens", seq_lens, torch.int32, (batch,), dev)
     _dense("cu_seqlens_q", cu_seqlens_q, torch.int32, (batch + 1,), dev)
     table = _table(block_table, batch, dev)
@@ -265,16 +282,30 @@ def paged_step(q, k, v, cache, block_table, batch, *, topk=None, tile=1, max_seq
     """One layer's step over a PageBatch: append k, v to the cache, score the pages of every request with the NVFP4 index
     vectors (one index head per KV head: the mean of its query heads), select topk of them and attend. topk=None: attend to
     whole sequences, without index vectors. Returns (out, ids)."""
-    append_tokens(cache, k, v, batch.cu_seqlens_q, batch.slots)
-    ids = None
+    # what a later stage would refuse is refused before the cache has changed
+    _check_queries(q, cache)
+    _table(block_table, batch.seq_lens.numel(), cache.device)
+    if scale is not None and not math.isfinite(scale):
+        _bad("scale must be finite")
+    if cache.pages * cache.kv_heads * PAGE >= 1 << 31:
+        _bad("rows of the cache must fit int32")
+    tokens = q.shape[0]
     if topk is not None:
         if cache.k_index is None:
             _bad("selection needs a cache with index vectors")
-        total, hq = int(q.shape[0]), int(q.shape[1])
-        codes, scales = quantize_rows(q, cache.kv_heads)
-        scores = fp4_block_scores_varlen(codes, cache.k_index, scales, cache.k_index_scale, batch.cu_seqlens_q,
-                                         batch.cu_seqlens_k, batch.cu_page_offsets, max_seqlen_q=max_seqlen_q,
-                                         max_seqlen_k=max_seqlen_k, kv_indices=batch.kv_indices, causal=True, exact=False)
+        if tokens and (max_seqlen_q < 1 or max_seqlen_k < 1 or batch.kv_indices.numel() == 0):
+            _bad("lengths and the page list of a step with tokens must not be empty")
+        _check_selection(max((max_seqlen_k + PAGE - 1) // PAGE, 1), cache.kv_heads, topk, tile, sink, recent)
+    append_tokens(cache, k, v, batch.cu_seqlens_q, batch.slots)
+    ids = None
+    if topk is not None:
+        if tokens:
+            codes, scales = quantize_rows(q, cache.kv_heads)
+            scores = fp4_block_scores_varlen(codes, cache.k_index, scales, cache.k_index_scale, batch.cu_seqlens_q,
+                                             batch.cu_seqlens_k, batch.cu_page_offsets, max_seqlen_q=max_seqlen_q,
+                                             max_seqlen_k=max_seqlen_k, kv_indices=batch.kv_indices, causal=True, exact=False)
+        else:
+            scores = torch.empty((cache.kv_heads, 1, 0), dtype=torch.float32, device=cache.device)
         ids = select_pages(scores, batch.cu_seqlens_q, batch.seq_lens, kv_heads=cache.kv_heads, topk=topk, tile=tile,
                            sink=sink, recent=recent)
     out = paged_attention(q, cache, block_table, batch.seq_lens, batch.cu_seqlens_q, ids, tile=tile,

@@ -211,3 +211,39 @@ def test_a_step_takes_views_of_a_fused_projection(sp, topk, tile):
     for bad in (0, -2, 3, 16):
         with pytest.raises(sp.SparseB200Error):
             sp.quantize_rows(q, bad)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(topk=0), dict(topk=3, tile=3), dict(topk=3, tile=256), dict(topk=2, sink=2, recent=1), dict(topk=2, sink=-1),
+    dict(topk=2, sink=2 ** 32), dict(topk=3, max_seqlen_q=0), dict(topk=3, max_seqlen_k=0), dict(topk=3, max_seqlen_k=51200 * PAGE),
+    dict(scale=math.nan), dict(scale=-math.inf), dict(topk=3, q="heads"), dict(q="strides"), dict(q="group"), dict(table="rows"),
+    dict(topk=3, index=False), dict(topk=3, table="no pages"),
+])
+def test_a_refused_step_leaves_the_cache_as_it_was(sp, bad):
+    bad = dict(bad)
+    q, k, v, cache, table, b = _step(sp, [2, 1], [300, 127], 2, 4, index=bad.pop("index", True))
+    q = {"heads": q[:, :3], "strides": q[..., ::2], "group": q[:, :2].repeat(1, 65, 1)}.get(bad.pop("q", None), q)
+    change = bad.pop("table", None)
+    if change == "rows":
+        table = table[:1]
+    elif change == "no pages":
+        b = b._replace(kv_indices=b.kv_indices[:0])
+    before = _copy(sp, cache)
+    with pytest.raises(sp.SparseB200Error):
+        sp.paged_step(q, k, v, cache, table, b, **{**dict(max_seqlen_q=2, max_seqlen_k=302), **bad})
+    torch.cuda.synchronize()
+    assert _same_bits(cache, before)
+
+
+@pytest.mark.parametrize("topk,tile", [(None, 1), (3, 1), (3, 16)])
+@pytest.mark.parametrize("rows", [0, 2])
+def test_a_step_without_tokens(sp, topk, tile, rows):
+    """No request has a new token, with and without rows of padding."""
+    old, hkv = [200, 3], 2
+    q, k, v, cache, table, _ = _step(sp, [1, 1], old, hkv, 4)
+    b = sp.extend_pages(table, _i32(old).cuda(), _i32([0, 0]).cuda(), _i32([4]).cuda(), _i32([1]).cuda(), total_q=rows, total_pages=3)
+    before = _copy(sp, cache)
+    out, ids = sp.paged_step(q[:rows], k[:rows], v[:rows], cache, table, b, topk=topk, tile=tile, max_seqlen_q=1, max_seqlen_k=200)
+    sp.device_status()
+    assert out.shape == (rows, 8, 128) and _same_bits(cache, before)
+    assert ids is None if topk is None else ids.shape == (hkv, sp.list_rows(rows, 2, tile), topk) and (ids == -1).all()
