@@ -770,6 +770,7 @@ int sparse_b200_select_pages(const float* scores, const int32_t* cu_seqlens_q, c
   if (rc) return rc;
   REQUIRE(hkv > 0 && hkv <= 65535 && hidx >= hkv && hidx % hkv == 0, "index heads must be a positive multiple of KV heads");
   REQUIRE(score_pages > 0, "page count must be positive");
+  REQUIRE(score_pages <= SELECT_MOST_PAGES, "too many pages for the page selection (51199 at most)");
   REQUIRE(sink >= 0 && recent >= 0 && sink <= topk && recent <= topk - sink, "sink and recent pages must fit the list");
   REQUIRE(static_cast<long long>(total_q / tile + batch) * topk < (1LL << 40), "lists too large");
   if (total_q == 0 && tile == 1) return SB_OK;

@@ -12,6 +12,8 @@ inline int check_kernel_launch() {
 }
 
 constexpr int PAGED_MAX_BATCH = 4096;      // requests of a step: their sums are held in shared memory
+constexpr int SELECT_SMEM = 200 * 1024;    // of a CTA that holds the keys of whole lists
+constexpr int SELECT_MOST_PAGES = SELECT_SMEM / 4 - 1;       // one list of (pages | 1) keys: 51199
 
 // First place in the ascending a[0..n) whose value is above x.
 __device__ __forceinline__ int upper_bound(const int* a, int n, int x) {

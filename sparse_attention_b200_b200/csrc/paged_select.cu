@@ -314,12 +314,11 @@ __global__ void __launch_bounds__(512) select_few_kernel(SelectArgs a) {
     write_list<KEYS>(keys + i * pitch, s_seen[i], a.topk, a.ids + (static_cast<long long>(head) * a.lists + row0 + i) * a.topk);
 }
 
-constexpr int SMEM_MOST = 200 * 1024;
 template <int ROWS, int KEYS>
 int launch_few(const SelectArgs& a, int heads, cudaStream_t stream) {
   const auto kernel = select_few_kernel<ROWS, KEYS>;
   const int smem = ROWS * (a.pages | 1) * 4;
-  if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MOST) != cudaSuccess)
+  if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SELECT_SMEM) != cudaSuccess)
     return set_error(SB_ERR_CUDA, "shared memory of the page selection");
   kernel<<<dim3((a.lists + ROWS - 1) / ROWS, heads), 512, smem, stream>>>(a);
   return check_kernel_launch();
@@ -343,10 +342,9 @@ int launch_select_pages(const float* scores, const int32_t* cu_q, const int32_t*
     if (pages <= 2 * 64) return launch_many<2>(a, heads, stream);
     if (pages <= 8 * 64) return launch_many<8>(a, heads, stream);
   }
-  const auto fits = [&](int rows) { return rows * (pages | 1) * 4 <= SMEM_MOST; };
+  const auto fits = [&](int rows) { return rows * (pages | 1) * 4 <= SELECT_SMEM; };
   if (fits(4)) return pages <= 256 ? launch_few<4, 8>(a, heads, stream) : launch_few<4, 0>(a, heads, stream);
-  if (fits(1)) return launch_few<1, 0>(a, heads, stream);
-  return set_error(SB_ERR_INVALID, "too many pages for the page selection (51199 at most)");
+  return launch_few<1, 0>(a, heads, stream);       // (SELECT_MOST_PAGES)
 }
 
 }  // namespace sb

@@ -102,6 +102,18 @@ def test_pages_are_neither_lost_nor_made_over_many_steps(sp):
     assert short
 
 
+# ------------------------------------------------------------------ select_pages
+@pytest.mark.parametrize("pages", [12798, 12799, 12800, 51199])
+def test_select_pages_of_the_longest_sequences(sp, pages):
+    """Around four lists to a CTA, and the most that one list may see."""
+    gen = torch.Generator(device="cuda").manual_seed(pages)
+    x = torch.randn((1, pages, 3), device="cuda", generator=gen)
+    got = sp.select_pages(x, _cu([3]).cuda(), _i32([pages * PAGE]).cuda(), kv_heads=1, topk=30, sink=0, recent=0, causal=False)
+    assert torch.equal(got.long(), x.transpose(1, 2).topk(30, -1).indices.sort(-1).values)
+    with pytest.raises(sp.SparseB200Error):
+        sp.select_pages(torch.empty((1, 51200, 1), device="cuda"), _cu([1]).cuda(), _i32([5]).cuda(), kv_heads=1, topk=3)
+
+
 # ------------------------------------------------------------------ paged_attention
 def _cache(gen, pages, hkv):
     codes = lambda: (100 * torch.randn((pages, hkv, PAGE, 128), generator=gen)).clamp(-448, 448).to(torch.float8_e4m3fn)  # noqa: E731

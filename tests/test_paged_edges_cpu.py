@@ -23,3 +23,10 @@ def test_extend_pages_refuses_more_pages_than_int32(lib, batch, width):
     """The pages of a step are counted in 32 bits (cu_page_offsets)."""
     rc = lib.sparse_b200_extend_pages(P, I64(width), width, P, P, P, 4, P, OTHER, P, P, P, P, P, OTHER, P, batch, 4, 4, None)
     _refused(lib, rc, b"int32")
+
+
+@pytest.mark.parametrize("pages", [51200, 1 << 26, 1 << 28, (1 << 31) - 1])
+def test_select_pages_refuses_more_pages_than_it_holds(lib, pages):
+    """Before anything is computed from the size: four lists of 2^28 pages are 2^32 bytes."""
+    rc = lib.sparse_b200_select_pages(P, P, P, P, 2, 1, 1, pages, 4, 4, 1, 1, 1, 1, None)
+    _refused(lib, rc, b"too many pages")
