@@ -382,11 +382,11 @@ int sparse_b200_indexer_summary_noalloc(const void* q, const void* k, float* sco
  * scorer reads a paged key cache that nothing else there writes, selects from or attends to.
  *
  * A page holds 128 tokens. k_pages, v_pages [pages, Hkv, 128, 128] e4m3 codes, k_scale, v_scale [pages, Hkv] fp32: a value is
- * its code times its page's scale. k_index [pages, Hkv, 128, 64] u8 and k_index_scale [pages, Hkv, 128, 8] e4m3 are the NVFP4
- * index vectors of the keys, as sparse_b200_fp4_scores_varlen reads them. block_table [B, table_stride] int32: the pages of a
- * request in order, table_width of them at most. seq_lens [B]: keys of a request, new ones included, unless said otherwise.
- * Rows of new tokens are packed request after request; cu_seqlens_q [B + 1] gives their places, rows behind the last one are
- * not read and not written. B <= 4096.
+ * its code times its page's scale, which is finite and not negative. k_index [pages, Hkv, 128, 64] u8 and k_index_scale
+ * [pages, Hkv, 128, 8] e4m3 are the NVFP4 index vectors of the keys, as sparse_b200_fp4_scores_varlen reads them. block_table
+ * [B, table_stride] int32: the pages of a request in order, table_width of them at most. seq_lens [B]: keys of a request, new
+ * ones included, unless said otherwise. Rows of new tokens are packed request after request; cu_seqlens_q [B + 1] gives their
+ * places, rows behind the last one are not read and not written. B <= 4096.
  *
  * Lists: `tile` (a power of two, 1 to 128) consecutive tokens of a request share a list of pages, given as places in the
  * request's block table row. page_ids [Hkv, rows, TopK]: with tile 1 the list of a token has the token's row (rows =
@@ -406,8 +406,9 @@ int sparse_b200_indexer_summary_noalloc(const void* q, const void* k, float* sco
  * append_tokens: k, v [total_q, Hkv, 128] bf16 rows (strides in elements, multiples of 8; a row itself is dense) into the
  * pages that slots names: the first token's slot of a request and of each page after it count, rows follow in order. Scale of
  * a page: the smallest power of two (at least 2^-100) with which the largest finite magnitude of its rows is at most 448;
- * where new rows make it grow, the rows before them are rescaled. Codes are rounded to nearest even, +-inf becomes +-448 times
- * the scale, NaN stays NaN. Rows behind the new ones are left as they were. Two requests must not append to one page.
+ * where new rows make it grow, the rows before them are rescaled (with a scale of 0 they are zeros). A larger scale that the
+ * page has is kept with its rows, whatever wrote it. Codes are rounded to nearest even, +-inf becomes +-448 times the scale,
+ * NaN stays NaN. Rows behind the new ones are left as they were. Two requests must not append to one page.
  * k_index / k_index_scale may be NULL.
  *
  * select_pages: scores [Hidx, score_pages, total_q] fp32 (sparse_b200_fp4_scores_varlen) -> page_ids. The score of a page for
@@ -419,10 +420,9 @@ int sparse_b200_indexer_summary_noalloc(const void* q, const void* k, float* sco
  * (page_ids NULL) or the listed ones; causal: token i of n sees keys j <= i + seq_len - n. A page listed twice counts twice,
  * entries that are not pages of the request are skipped. out [total_q, Hq, 128] bf16, lse [total_q, Hq] fp32 or NULL; a row
  * that sees no key, or only keys of score -inf, is 0 with LSE -inf. What lies in the cache behind a request's last key, or is
- * hidden from a token, does not reach its row, whatever its bits. Scales are not negative; a query row with an infinite or NaN
- * feature ends as NaN. Hq / Hkv <= 64. max_seqlen_q (a hint: the largest number of
- * new tokens) sets how many tokens share a pass over a page. workspace: sparse_b200_paged_attention_workspace_bytes bytes
- * that are the call's own while it runs. */
+ * hidden from a token, does not reach its row, whatever its bits. A query row with an infinite or NaN feature ends as NaN.
+ * Hq / Hkv <= 64. max_seqlen_q (a hint: the largest number of new tokens) sets how many tokens share a pass over a page.
+ * workspace: sparse_b200_paged_attention_workspace_bytes bytes that are the call's own while it runs. */
 int sparse_b200_extend_pages(int32_t* block_table, int64_t table_stride, int table_width, const int32_t* seq_lens,
                              const int32_t* new_lens, const int32_t* free_pages, int free_capacity,
                              const int32_t* free_count, int32_t* seq_lens_out, int32_t* cu_seqlens_q,

@@ -8,6 +8,8 @@
 //   rows before the run in its page (a run that does not begin at row 0): s = max(s, old s), and where s grew the codes of
 //   those rows are multiplied by old s / s and rounded again
 //   code = e4m3(x / s), to nearest even, +-inf to +-448, NaN stays NaN
+// A page whose scale was set elsewhere keeps it while it is large enough, a power of two or not: its new rows are multiplied by
+// 1 / s in 32 bits then. Scales are finite and not negative.
 // A scale that is a power of two costs no precision (e4m3 is a floating format) and makes growth exact but for codes that
 // become subnormal: a page that is filled token by token is not rounded over and over.
 //
@@ -119,8 +121,8 @@ __global__ void __launch_bounds__(THREADS) append_tokens_kernel(AppendArgs a) {
   if (offset > 0 && old >= s) {
     s = old;
     inv = 1.0f / old;
-  } else if (offset > 0 && old > 0.f) {
-    const float by = old * inv;                            // powers of two: exact
+  } else if (offset > 0) {
+    const float by = old * inv;                            // powers of two: exact; a page of scale 0 held zeros
     for (int i = tid; i < offset * 8; i += THREADS) {
       uint4* at = reinterpret_cast<uint4*>(rows) + i;
       uint4 c = *at;

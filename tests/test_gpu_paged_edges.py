@@ -102,6 +102,34 @@ def test_pages_are_neither_lost_nor_made_over_many_steps(sp):
     assert short
 
 
+# ------------------------------------------------------------------ append_tokens
+@pytest.mark.parametrize("old", [0.0, 2.0 ** -110, 2.0 ** -9, 0.013, 3.0])
+def test_rows_behind_those_of_a_page_with_any_scale(sp, old):
+    """Scales that were set elsewhere: 0 (its rows are zeros and stay so), below the lowest that is written, no power of two."""
+    gen = torch.Generator().manual_seed(7)
+    hkv, before, n = 2, 37, 50
+    c = _cache(gen, 2, hkv)
+    c["k"].view(torch.uint8)[0, :, 3, 9] = 0x7F                        # a NaN stays one
+    for name in ("k_scale", "v_scale"):
+        c[name][0] = old
+    x = torch.randn((2, n, hkv, 128), generator=gen).to(torch.bfloat16)
+    x[1] = 0                                                           # values of nothing: their scale is the lowest, or the page's
+    cache = _on_gpu(sp, c)
+    slots = torch.arange(before, before + n)
+    sp.append_tokens(cache, x[0].cuda(), x[1].cuda(), _i32([0, n]).cuda(), slots.cuda())
+    for rows, name in zip(x, ("k", "v")):
+        want, want_scale = ref.append_tokens(c[name], c[name + "_scale"], rows, _i32([0, n]), slots)
+        got = getattr(cache, name).cpu().double()
+        assert torch.equal(getattr(cache, name + "_scale").cpu().double(), want_scale)
+        assert torch.equal(got.isnan(), want.isnan())
+        got, want = got.nan_to_num(0.0), want.nan_to_num(0.0)
+        if math.frexp(old)[0] in (0.0, 0.5):
+            assert torch.equal(got, want)
+        else:                                                          # 1 / s and the product are rounded in 32 bits: a tie may fall the other way
+            step = torch.exp2(torch.frexp(want)[1].clamp(min=-5).double() - 4)
+            assert ((got - want).abs() <= step).all() and (got == want).double().mean() > 0.999
+
+
 # ------------------------------------------------------------------ select_pages
 @pytest.mark.parametrize("pages", [12798, 12799, 12800, 51199])
 def test_select_pages_of_the_longest_sequences(sp, pages):
