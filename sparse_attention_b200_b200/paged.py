@@ -91,7 +91,15 @@ def _table(block_table, batch, device):
 class PagedCache:
     """Keys and values of one layer in pages of 128 tokens: e4m3 codes k, v [pages,Hkv,128,128] and scales k_scale, v_scale
     [pages,Hkv] fp32, and with index=True the NVFP4 index vectors of the keys, k_index [pages,Hkv,128,64] u8 and
-    k_index_scale [pages,Hkv,128,8] e4m3, as fp4_block_scores_varlen takes them."""
+    k_index_scale [pages,Hkv,128,8] e4m3, as fp4_block_scores_varlen takes them. Its tensors are the cache's own for good: they
+    may be written to, not replaced (a cache over others is another from_tensors)."""
+
+    _FIXED = frozenset(("k", "v", "k_scale", "v_scale", "k_index", "k_index_scale", "pages", "kv_heads", "device", "addresses"))
+
+    def __setattr__(self, name, value):
+        if name in self._FIXED:
+            _bad(f"{name} of a cache cannot be replaced: use PagedCache.from_tensors")
+        object.__setattr__(self, name, value)
 
     def __init__(self, pages, kv_heads, device="cuda", index=True):
         if pages <= 0 or kv_heads <= 0:
@@ -114,8 +122,8 @@ class PagedCache:
     def _set(self, k, v, k_scale, v_scale, k_index, k_index_scale):
         if k.dim() != 4 or tuple(k.shape[2:]) != (PAGE, 128) or not k.is_cuda:
             _bad("cache pages must be CUDA tensors [pages,Hkv,128,128]")
-        self.pages, self.kv_heads, self.device = int(k.shape[0]), int(k.shape[1]), k.device
-        lead = (self.pages, self.kv_heads)
+        pages, kv_heads = int(k.shape[0]), int(k.shape[1])
+        lead = (pages, kv_heads)
         _dense("k", k, torch.float8_e4m3fn, (*lead, PAGE, 128), k.device)
         _dense("v", v, torch.float8_e4m3fn, (*lead, PAGE, 128), k.device)
         _dense("k_scale", k_scale, torch.float32, lead, k.device)
@@ -125,9 +133,14 @@ class PagedCache:
         if k_index is not None:
             _dense("k_index", k_index, torch.uint8, (*lead, PAGE, 64), k.device)
             _dense("k_index_scale", k_index_scale, torch.float8_e4m3fn, (*lead, PAGE, 8), k.device)
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.k_index, self.k_index_scale = k_index, k_index_scale
-        self.addresses = tuple(0 if x is None else x.data_ptr() for x in (k, v, k_scale, v_scale, k_index, k_index_scale))
+        self.__dict__.update(k=k, v=v, k_scale=k_scale, v_scale=v_scale, k_index=k_index, k_index_scale=k_index_scale, pages=pages,
+                             kv_heads=kv_heads, device=k.device)
+
+    @property
+    def addresses(self):
+        """Of codes, scales and index vectors (0: none), as they are at the time of a call."""
+        at = self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr()
+        return (*at, 0, 0) if self.k_index is None else (*at, self.k_index.data_ptr(), self.k_index_scale.data_ptr())
 
 
 def extend_pages(block_table, seq_lens, new_lens, free_pages, free_count, *, total_q, total_pages):

@@ -130,6 +130,25 @@ def test_rows_behind_those_of_a_page_with_any_scale(sp, old):
             assert ((got - want).abs() <= step).all() and (got == want).double().mean() > 0.999
 
 
+def test_the_tensors_of_a_cache_stay_its_own(sp):
+    gen = torch.Generator().manual_seed(8)
+    cache = _on_gpu(sp, _cache(gen, 3, 2))
+    for name in ("k", "v", "k_scale", "v_scale", "k_index", "k_index_scale", "pages", "kv_heads", "device"):
+        held = getattr(cache, name)
+        with pytest.raises(sp.SparseB200Error):
+            setattr(cache, name, held)
+        assert getattr(cache, name) is held
+    cache.layer = 3                                                    # a user's own mark
+    # a tensor whose memory moves under the cache: the calls find it
+    more = cache.k.clone()
+    cache.k.data = more.clone()
+    x = torch.randn((5, 2, 128), generator=gen).to(torch.bfloat16).cuda()
+    sp.append_tokens(cache, x, x, _i32([0, 5]).cuda(), torch.arange(128, 133).cuda())
+    assert not torch.equal(cache.k.view(torch.uint8)[1, :, :5], more.view(torch.uint8)[1, :, :5])
+    cache.k.view(torch.uint8)[1, :, :5] = more.view(torch.uint8)[1, :, :5]
+    assert torch.equal(cache.k.view(torch.uint8), more.view(torch.uint8))
+
+
 # ------------------------------------------------------------------ select_pages
 @pytest.mark.parametrize("pages", [12798, 12799, 12800, 51199])
 def test_select_pages_of_the_longest_sequences(sp, pages):
