@@ -395,10 +395,12 @@ int sparse_b200_indexer_summary_noalloc(const void* q, const void* k, float* sco
  * extend_pages: pages for the new tokens, and every table of a step, from the lengths. seq_lens here are the tokens that the
  * cache holds so far, new_lens the new ones; negative lengths count as 0. New pages are taken from the end of free_pages
  * [free_count], by request; block_table gets them. A request whose pages do not fit its table row, or are not free (counted
- * over the requests before it, in order), is refused: its length stays, its slots are -1. Written: seq_lens_out [B],
- * cu_seqlens_q / cu_seqlens_k / cu_page_offsets [B + 1], kv_indices [total_pages] (pages of all requests in order, -1
- * behind), slots [total_q] (page * 128 + row of every new token, -1 behind), free_count_out [1], status [1]: 1 pages ran out,
- * 2 a table row is too short, 4 more new tokens than total_q, 8 more pages than total_pages, 16 a sum is beyond int32 (kept
+ * over the requests before it, in order), is refused: its length stays, its slots are -1. Its tokens keep their rows in the
+ * step, and what the other operators give for them (the attention takes them for the last tokens that the cache holds) means
+ * nothing: a slot of -1 marks such rows. Other requests are not touched by it. Written: seq_lens_out [B], cu_seqlens_q /
+ * cu_seqlens_k / cu_page_offsets [B + 1], kv_indices [total_pages] (pages of all requests in order, -1 behind), slots
+ * [total_q] (page * 128 + row of every new token, -1 behind), free_count_out [1], status [1]: 1 pages ran out, 2 a table row
+ * is too short, 4 more new tokens than total_q, 8 more pages than total_pages, 16 a sum is beyond int32 (kept
  * at its largest). With 4 or 8 the step's tables are cut off: slots and kv_indices hold the first entries, and cu_page_offsets
  * does not go beyond total_pages, so that who reads kv_indices by it (the scorer) stays within; the requests that are cut have
  * no meaningful results. The inputs other than block_table stay as they are, so a call may be repeated. B * table_width < 2^31.

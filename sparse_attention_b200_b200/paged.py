@@ -149,7 +149,8 @@ def extend_pages(block_table, seq_lens, new_lens, free_pages, free_count, *, tot
     seq_lens with the new tokens, cu_seqlens_q / cu_seqlens_k / cu_page_offsets [B+1], kv_indices [total_pages], slots
     [total_q] int64, free_count [1], status [1] (STATUS_* bits; 0: all is well). total_q and total_pages are the sizes of the
     tables; what is behind the last token or page is -1, and cu_page_offsets never goes beyond total_pages (STATUS_PAGES says
-    that pages were left out). A request that gets no pages is refused: its length stays, its slots are -1."""
+    that pages were left out). A request that gets no pages is refused: its length stays, its slots are -1, and what a step
+    gives for its rows means nothing."""
     batch, dev = seq_lens.numel(), seq_lens.device
     if not seq_lens.is_cuda or batch == 0:
         _bad("seq_lens must be a CUDA tensor of at least one request")
@@ -294,7 +295,8 @@ def paged_step(q, k, v, cache, block_table, batch, *, topk=None, tile=1, max_seq
                scale=None):
     """One layer's step over a PageBatch: append k, v to the cache, score the pages of every request with the NVFP4 index
     vectors (one index head per KV head: the mean of its query heads), select topk of them and attend. topk=None: attend to
-    whole sequences, without index vectors. Returns (out, ids)."""
+    whole sequences, without index vectors. Returns (out, ids); rows whose slot is -1 (a refused request's, and those behind the
+    last token) have no meaning."""
     # what a later stage would refuse is refused before the cache has changed
     _check_queries(q, cache)
     _table(block_table, batch.seq_lens.numel(), cache.device)

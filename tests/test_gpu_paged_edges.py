@@ -306,3 +306,42 @@ def test_a_step_without_tokens(sp, topk, tile, rows):
     sp.device_status()
     assert out.shape == (rows, 8, 128) and _same_bits(cache, before)
     assert ids is None if topk is None else ids.shape == (hkv, sp.list_rows(rows, 2, tile), topk) and (ids == -1).all()
+
+
+@pytest.mark.parametrize("topk", [None, 3])
+def test_a_refused_request_does_not_touch_the_others(sp, topk):
+    """The one in the middle finds no pages: rows and pages of the others are those of a step without it, and a step of its own
+    with pages then gives what it would have given at once."""
+    hkv, group, old, lens, pages = 2, 4, [300, 250, 600], [1, 200, 2], 16      # of these 3 + 2 + 5 are held, request 1 needs 2
+    q, k, v, cache, table, _ = _step(sp, lens, old, hkv, group)
+    grown = lambda t: torch.cat([t, t])[:pages].contiguous()  # noqa: E731
+    cache = sp.PagedCache.from_tensors(*(grown(t.view(torch.uint8)).view(t.dtype) for t in (
+        cache.k, cache.v, cache.k_scale, cache.v_scale, cache.k_index, cache.k_index_scale)))
+    free = torch.arange(10, pages, dtype=torch.int32).cuda()
+
+    def step(cache, table, seq, rows, lens, spare):
+        b = sp.extend_pages(table, _i32(seq).cuda(), _i32(lens).cuda(), free, _i32([spare]).cuda(), total_q=sum(lens),
+                            total_pages=pages)
+        out, _ = sp.paged_step(q[rows], k[rows], v[rows], cache, table, b, topk=topk, max_seqlen_q=200, max_seqlen_k=602)
+        return b, out
+
+    def close(x, y, cache):
+        """Another batch is cut into other shares, whose parts are joined in 32 bits: the same weights but for those of 16 bits
+        (2^-11 each, relative to another reference), and each side rounds to bf16 once (2^-8 of it)."""
+        most = (cache.v.float().abs() * cache.v_scale[..., None, None]).max().item()
+        x, y = x.double(), y.double()
+        assert ((x - y).abs() <= 2.0 ** -7 * torch.maximum(x.abs(), y.abs()) + 2.0 ** -10 * most).all()
+    both, without, at_once = _copy(sp, cache), _copy(sp, cache), _copy(sp, cache)
+    t1, t2, t3 = table.clone(), table.clone(), table.clone()
+    b, out = step(both, t1, old, slice(0, 203), lens, 1)
+    assert int(b.status) == sp.paged.STATUS_NO_PAGES and int(b.free_count) == 1 and b.seq_lens.tolist() == [301, 250, 602]
+    rest = [0, 201, 202]
+    assert (b.slots[1:201] == -1).all() and (b.slots[rest] >= 0).all()
+    _, want = step(without, t2, old, rest, [1, 0, 2], 1)
+    assert _same_bits(both, without) and torch.equal(t1, t2)
+    close(out[rest], want, both)
+    b, out = step(both, t1, [301, 250, 602], slice(1, 201), [0, 200, 0], 6)
+    assert int(b.status) == 0 and int(b.free_count) == 4
+    b, want = step(at_once, t3, old, slice(0, 203), lens, 6)
+    assert _same_bits(both, at_once) and torch.equal(t1, t3)
+    close(out, want[1:201], both)
