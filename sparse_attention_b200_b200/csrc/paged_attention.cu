@@ -8,11 +8,12 @@
 // token of a few heads fills the instruction:
 //   S^T [128 keys, R] = K [128 keys, 128] Q^T       O^T [128 features, R] = V^T [128 features, 128 keys] P^T
 // The tensor core multiplies e4m3 by e4m3 (kind::f8f6f4), and the codes of a page are its operands as they lie in memory:
-// nothing is dequantised. The other operand is split in two e4m3 terms in columns of their own, x = hi + lo / 16: a bf16 has
-// eight significant bits and an e4m3 code four, so a query (scaled by a power of two to [128, 256) by its row's largest
-// feature) is carried exactly but for features below 2^-22 of the largest; a probability (times 256, against the maximum of
-// its own page, so that no page's weights fall below the format's range) is cut at four bits and the rest rounded to four:
-// within 2^-8 of its value, half a step of bf16. Sums and outputs are fp32; every page's output is added to registers with the
+// nothing is dequantised. The other operand is split in two e4m3 terms in columns of their own, x = hi + lo / 16, hi rounded to
+// nearest and lo the rest: a bf16 has eight significant bits and an e4m3 code four, so a query (scaled by a power of two to
+// [128, 256) by its row's largest feature) is carried exactly where a feature is 2^-13 of the largest or more, and within 2^-21
+// of the largest (half of lo's smallest step) where it is less; a probability (times 256, against the maximum of its own page,
+// so that no page's weights fall below the format's range) within 2^-9 + 2^-11 of its value down to 2^-14 of the page's largest,
+// and within 2^-22 of the largest below. Sums and outputs are fp32; every page's output is added to registers with the
 // page's own factor exp2(page maximum - maximum of the item's first page) * v_scale.
 //
 // A softmax thread owns a key (a TMEM lane of S^T) and the 16 rows; a row's maximum over the page is taken in bf16 pairs by
@@ -159,6 +160,10 @@ __device__ __noinline__ bool load_tile(uint32_t full, uint32_t empty, uint32_t p
   }
   __syncwarp();
   return true;
+}
+__device__ __forceinline__ uint32_t e4m3x2(__half2 x) { return __nv_cvt_halfraw2_to_fp8x2(x, __NV_SATFINITE, __NV_E4M3); }
+__device__ __forceinline__ __half2 half2_of(uint32_t codes) {
+  return __half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(codes), __NV_E4M3));
 }
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
@@ -665,11 +670,9 @@ __global__ void __launch_bounds__(Config::THREADS, Config::CTAS)
               const float2 n = fma2(v, i ? make_float2(w4.z, w4.w) : make_float2(w4.x, w4.y), make_float2(l[j], l[j + 1]));
               l[j] = n.x;
               l[j + 1] = n.y;
-              const float2 cut = make_float2(__uint_as_float(__float_as_uint(v.x) & 0xfff00000u),     // four significant bits
-                                             __uint_as_float(__float_as_uint(v.y) & 0xfff00000u));
-              const float2 rest = fma2(v, make_float2(16.f, 16.f), mul2(cut, make_float2(-16.f, -16.f)));
-              hi[i] = e4m3x2(cut.x, cut.y);
-              lo[i] = e4m3x2(rest.x, rest.y);
+              const __half2 w = __float22half2_rn(v);      // 2^-11; what is left of it by its upper term is exact
+              hi[i] = e4m3x2(w);
+              lo[i] = e4m3x2(__hfma2(half2_of(hi[i]), __float2half2_rn(-16.f), __hmul2(w, __float2half2_rn(16.f))));
             }
             ph[j4] = __byte_perm(hi[0], hi[1], 0x5410);
             pl[j4] = __byte_perm(lo[0], lo[1], 0x5410);

@@ -345,3 +345,57 @@ def test_a_refused_request_does_not_touch_the_others(sp, topk):
     b, want = step(at_once, t3, old, slice(0, 203), lens, 6)
     assert _same_bits(both, at_once) and torch.equal(t1, t3)
     close(out, want[1:201], both)
+
+
+# ------------------------------------------------------------------ precision of small weights and features
+@pytest.mark.parametrize("depth", [4.3, 11.9, 14.4, 15.2, 16.3, 17.42, 18.6, 19.7, 20.5])
+@pytest.mark.parametrize("group", [1, 4, 40])
+def test_values_of_small_weights_beside_a_key_that_takes_all(sp, group, depth):
+    """A key of weight 1 and value 0 (as a first token often is) in a page whose other weights are 2^-depth: the output is their
+    values'. A weight is within 2^-8 of itself, or 2^-22 of the page's largest (the smallest step of its lower e4m3 term is 2^-13
+    where the largest is 256, its half 2^-14)."""
+    gen = torch.Generator().manual_seed(1)
+    c = _cache(gen, 2, 1)
+    c["k"].view(torch.uint8)[:] = 0
+    c["k"][:, 0, 0, 0] = 16.0
+    c["v"] = (0.5 + torch.rand(c["v"].shape, generator=gen) / 2).to(torch.float8_e4m3fn)
+    c["v"][:, 0, 0] = 0.0
+    c["k_scale"][:], c["v_scale"][:] = 1.0, 1.0
+    q = torch.zeros((1, group, 128), dtype=torch.bfloat16)
+    q[:, :, 0] = 1.0
+    for seq in (128, 200, 256):
+        table, s, scale = _i32([[1, 0]]), _i32([seq]), depth * math.log(2) / 16
+        want, want_lse, spread, size = ref.paged_attention(q, c["k"], c["v"], c["k_scale"], c["v_scale"], table, s, _cu([1]),
+                                                           scale=scale)
+        bound, bound_lse = _bounds(want, want_lse, spread, size)
+        # p of the page's largest is 1 / (sum of exp2 of the depths); it times 2^-22 for each of the keys' values
+        weights = torch.full((seq,), 2.0 ** -depth, dtype=torch.float64)
+        weights[::PAGE] = 1.0
+        values = torch.cat([c["v"][1, 0], c["v"][0, 0]])[:seq].double().abs().sum(0)
+        bound = bound + 2.0 ** -22 * values / weights.sum()
+        out, lse = _alike(sp, 300, q, c, table, s, scale=scale)
+        assert ((out - want).abs() <= bound).all(), ((out - want).abs() / bound).max()
+        assert ((lse - want_lse).abs() <= bound_lse).all()
+
+
+@pytest.mark.parametrize("below", [10, 14, 16, 18, 20])
+@pytest.mark.parametrize("group", [1, 4, 40])
+def test_scores_of_features_far_below_their_rows_largest(sp, group, below):
+    """One feature of a query row, at which the keys are 0, is 2^below times the others: those make up the scores. A feature is
+    off by half the smallest step of its lower e4m3 term, 2^-14 where the largest is 128 or more: 2^-21 of the largest."""
+    gen = torch.Generator().manual_seed(below)
+    seq = 200
+    c = _cache(gen, 2, 1)
+    c["k"][..., 77] = 0.0
+    c["k_scale"][:] = 2.0 ** -6
+    q = torch.randn((1, group, 128), generator=gen).clamp(-1.9, 1.9)
+    q[:, :, 77] = 2.0 ** below * torch.linspace(1.0, 1.99, group)
+    q, table, s = q.to(torch.bfloat16), _i32([[1, 0]]), _i32([seq])
+    want, want_lse, spread, size = ref.paged_attention(q, c["k"], c["v"], c["k_scale"], c["v_scale"], table, s, _cu([1]))
+    keys = torch.cat([c["k"][p, 0].double() * c["k_scale"][p, 0].double() for p in (1, 0)])[:seq].abs().sum(1).max()
+    score = 2.0 ** -17 * size + 2.0 ** -21 * q.double().abs().amax(-1) * keys * 128 ** -0.5
+    out, lse = _alike(sp, 300, q, c, table, s)
+    assert ((lse - want_lse).abs() <= score + 2.0 ** -20 * want_lse.abs()).all()
+    off = torch.expm1(2 * score)[..., None]
+    bound = 2.0 ** -8 * want.abs() + (2.0 ** -8 + off) * spread * 1.01
+    assert ((out - want).abs() <= bound).all(), ((out - want).abs() / bound).max()
