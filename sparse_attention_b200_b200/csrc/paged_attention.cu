@@ -614,7 +614,9 @@ __global__ void __launch_bounds__(Config::THREADS, Config::CTAS)
           float mu = none ? -INFINITY : fmaf(fabsf(top), 0.00394f, top) * f;       // 2^-8 and a little
           float over = 1.f;                          // 0: s is relative to mu already
           // The sums stay relative to the item's first page: fp32 has room for 2^40 above it, and what lies below loses nothing.
-          if (__any_sync(0xffffffffu, !none && (fabsf(mu) > 100.f || (!unset && mu - m > 40.f)))) {
+          // Less where the page's values are huge: a rise times its value scale stays below 2^90, or the reference follows.
+          const float room = static_cast<float>(max(min(216 - (x[3] >> 23 & 255), 40), 0));        // 90 - exponent - 1
+          if (__any_sync(0xffffffffu, !none && (fabsf(mu) > 100.f || (!unset && mu - m > room)))) {
             // Rare: scores above that, or so large that the rounding up is more than a factor of 1.5. The maxima in fp32; all
             // four warps of the group are here.
             float* exact = reinterpret_cast<float*>(gbase + C::OFF_EXACT);
@@ -626,7 +628,7 @@ __global__ void __launch_bounds__(Config::THREADS, Config::CTAS)
             if (!ok) break;
             top = fmaxf(fmaxf(exact[r16], exact[16 + r16]), fmaxf(exact[32 + r16], exact[48 + r16]));
             if (!none) mu = top * f;
-            const bool jump = !unset && mu - m > 40.f;
+            const bool jump = !unset && mu - m > room;
             if (lane < 16) {
               factors[lane] = jump ? ex2_approx(m - mu) : 1.f;
               factors[16 + lane] = none ? 0.f : top;

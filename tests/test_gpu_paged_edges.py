@@ -399,3 +399,31 @@ def test_scores_of_features_far_below_their_rows_largest(sp, group, below):
     off = torch.expm1(2 * score)[..., None]
     bound = 2.0 ** -8 * want.abs() + (2.0 ** -8 + off) * spread * 1.01
     assert ((out - want).abs() <= bound).all(), ((out - want).abs() / bound).max()
+
+
+@pytest.mark.parametrize("v_scales", [(1.0, 1e30), (1e30, 1.0), (2.0 ** 108, 2.0 ** 108), (2.0 ** -100, 2.0 ** 108)])
+@pytest.mark.parametrize("rise", [0.0, 7.5, 20.0, 39.0, 45.0, 100.0])
+@pytest.mark.parametrize("group", [1, 4])
+def test_sums_of_huge_values_stay_finite(sp, group, rise, v_scales):
+    """Pages whose values are up to 2^117 and whose weights are 2^rise those of the page before: sums hold keys * largest value,
+    below 2^127 here, and never a page's rise on top of it."""
+    gen = torch.Generator().manual_seed(2)
+    c = _cache(gen, 3, 1)
+    c["k"].view(torch.uint8)[:] = 0
+    c["k"][1, 0, :, 0], c["k"][2, 0, :, 0] = 8.0, 16.0                  # page 0, then 1, then 2: each rises over the one before
+    c["k_scale"][:] = 1.0
+    c["v_scale"][:] = torch.tensor([v_scales[0], v_scales[1], v_scales[0]])[:, None]
+    q = torch.zeros((1, group, 128), dtype=torch.bfloat16)
+    q[:, :, 0] = 1.0
+    table, scale = _i32([[0, 1, 2]]), rise * math.log(2) / 8
+    for seq in (256, 384):
+        want, want_lse, spread, size = ref.paged_attention(q, c["k"], c["v"], c["k_scale"], c["v_scale"], table, _i32([seq]), _cu([1]),
+                                                           scale=scale)
+        bound, bound_lse = _bounds(want, want_lse, spread, size)
+        # weights of 16 bits: 2^-31 of the row's largest product of weight and scale, times a code of 448, for each key
+        bound = bound + seq * 448 * 2.0 ** -31 * spread.amax(-1, keepdim=True) / 100 if group > 16 else bound
+        for n in (1, 600):                                             # parts of a page each, and whole items in a share
+            out, lse = _alike(sp, n, q, c, table, _i32([seq]), scale=scale)
+            assert out.isfinite().all()
+            assert ((out - want).abs() <= bound).all(), ((out - want).abs() / bound).max()
+            assert ((lse - want_lse).abs() <= bound_lse).all()
