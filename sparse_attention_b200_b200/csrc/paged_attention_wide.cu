@@ -592,7 +592,9 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
           ok = wait_warp(bar(B_SUM + quarter), ends & 1, guard, 0xd37);
           if (!ok) break;
           const float total = sum_at[row] + sum_at[128 + row];
-          const float of = ex2_approx(o), by = total == 0.f ? 0.f : place >= 0 ? of : of / total;
+          // Relative to m + 8, which no score exceeds: a part's sums hold keys * largest value, no more.
+          constexpr float DOWN = LIFT + 8.f, SUNK = 1.f / 16384.f;       // 2^-DOWN
+          const float of = ex2_approx(o - DOWN), by = total == 0.f ? 0.f : place >= 0 ? of : of / (total * SUNK);
           const long long out_row = (static_cast<long long>(token0) + token) * p.a.hq + head * p.group + g;
           const int* nan_at = reinterpret_cast<const int*>(gbase + OFF_NAN) + (items & 7) * 128 + 64 * half;
 #pragma unroll
@@ -633,7 +635,7 @@ __global__ void __launch_bounds__(THREADS, WIDE_CTAS) paged_wide_kernel(const Pa
           tc_fence_before();
           if (half == 0 && row < rows) {
             if (place >= 0)
-              *reinterpret_cast<float2*>(p.part_ml + (static_cast<long long>(place) * WIDE_ROWS + row) * 2) = make_float2(m - LIFT, total);
+              *reinterpret_cast<float2*>(p.part_ml + (static_cast<long long>(place) * WIDE_ROWS + row) * 2) = make_float2(m - LIFT + DOWN, total * SUNK);
             else if (p.a.lse)
               p.a.lse[out_row] = total == 0.f ? -INFINITY : (m - LIFT + log2f(total)) * 0.6931471805599453f;
           }

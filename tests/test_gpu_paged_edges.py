@@ -403,7 +403,7 @@ def test_scores_of_features_far_below_their_rows_largest(sp, group, below):
 
 @pytest.mark.parametrize("v_scales", [(1.0, 1e30), (1e30, 1.0), (2.0 ** 108, 2.0 ** 108), (2.0 ** -100, 2.0 ** 108)])
 @pytest.mark.parametrize("rise", [0.0, 7.5, 20.0, 39.0, 45.0, 100.0])
-@pytest.mark.parametrize("group", [1, 4])
+@pytest.mark.parametrize("group", [1, 4, 40])
 def test_sums_of_huge_values_stay_finite(sp, group, rise, v_scales):
     """Pages whose values are up to 2^117 and whose weights are 2^rise those of the page before: sums hold keys * largest value,
     below 2^127 here, and never a page's rise on top of it."""
