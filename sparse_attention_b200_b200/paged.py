@@ -64,28 +64,28 @@ def _dense(name, t, dtype, shape, device):
 
 def _rows(name, t, heads, device=None, total=None):
     """Packed bf16 rows [T, H, 128]: any token and head stride that keeps rows on 16 bytes."""
-    if t.dtype is not torch.bfloat16 or t.dim() != 3 or t.shape[2] != 128 or not t.is_cuda:
+    shape = t.shape
+    if t.dtype is not torch.bfloat16 or len(shape) != 3 or shape[2] != 128 or not t.is_cuda:
         _bad(f"{name} must be a bfloat16 CUDA tensor [T,H,128]")
     if device is not None and t.device != device:
         _bad(f"{name} must be on {device}")
-    if heads is not None and t.shape[1] != heads or total is not None and t.shape[0] != total:
+    if heads is not None and shape[1] != heads or total is not None and shape[0] != total:
         _bad(f"{name} must have shape [{total if total is not None else 'T'},{heads},128]")
     if t.requires_grad:
         _bad("the paged path is forward-only")
-    s, at = t.stride(), t.data_ptr()
-    if s[2] != 1 or (s[0] | s[1]) % 8 or at % 16:
+    (token, head, feature), at = t.stride(), t.data_ptr()
+    if feature != 1 or (token | head) % 8 or at % 16:
         _bad(f"{name}: rows must be dense, 16-byte aligned and at strides that are multiples of 8 elements")
-    return at, s[0], s[1]
+    return at, token, head
 
 
 def _table(block_table, batch, device):
     """Its address, row stride and width."""
-    if block_table.dtype is not torch.int32 or block_table.device != device or block_table.dim() != 2 \
-            or block_table.shape[0] != batch or block_table.shape[1] == 0 or block_table.stride(1) != 1 \
-            or batch > 1 and block_table.stride(0) < block_table.shape[1]:
+    shape, stride = block_table.shape, block_table.stride()
+    if block_table.dtype is not torch.int32 or block_table.device != device or len(shape) != 2 or shape[0] != batch \
+            or shape[1] == 0 or stride[1] != 1 or batch > 1 and stride[0] < shape[1]:
         _bad("block_table must be int32 [B, pages per request] with dense rows on the same device")
-    width = block_table.shape[1]
-    return block_table.data_ptr(), max(block_table.stride(0), width), width
+    return block_table.data_ptr(), max(stride[0], shape[1]), shape[1]
 
 
 class PagedCache:
@@ -243,10 +243,12 @@ def _workspace_bytes(device, hq, hkv, tile, max_q, listed):
 
 
 def _check_queries(q, cache):
-    rows, hq, hkv = _rows("q", q, None, cache.device), q.shape[1], cache.kv_heads
+    """Tokens, query heads, and the rows' address and strides."""
+    rows, hkv = _rows("q", q, None, cache.device), cache.kv_heads
+    total, hq, _ = q.shape
     if hq < hkv or hq % hkv or hq // hkv > 64:
         _bad("Hq must be a multiple of Hkv, at most 64 query heads to a KV head")
-    return rows
+    return total, hq, rows
 
 
 def paged_attention(q, cache, block_table, seq_lens, cu_seqlens_q, ids=None, *, tile=1, max_seqlen_q=None, causal=True,
@@ -257,8 +259,7 @@ def paged_attention(q, cache, block_table, seq_lens, cu_seqlens_q, ids=None, *, 
     the last token of out and lse are left as they were. max_seqlen_q: the largest number of new tokens, for how many of them
     share a pass over a page (default: T). scale: default 128^-0.5."""
     hkv, dev, batch = cache.kv_heads, cache.device, seq_lens.numel()
-    rows = _check_queries(q, cache)
-    total, hq = q.shape[:2]
+    total, hq, rows = _check_queries(q, cache)
     _dense("seq_lens", seq_lens, torch.int32, (batch,), dev)
     _dense("cu_seqlens_q", cu_seqlens_q, torch.int32, (batch + 1,), dev)
     table = _table(block_table, batch, dev)
@@ -298,13 +299,12 @@ def paged_step(q, k, v, cache, block_table, batch, *, topk=None, tile=1, max_seq
     whole sequences, without index vectors. Returns (out, ids); rows whose slot is -1 (a refused request's, and those behind the
     last token) have no meaning."""
     # what a later stage would refuse is refused before the cache has changed
-    _check_queries(q, cache)
+    tokens = _check_queries(q, cache)[0]
     _table(block_table, batch.seq_lens.numel(), cache.device)
     if scale is not None and not math.isfinite(scale):
         _bad("scale must be finite")
     if cache.pages * cache.kv_heads * PAGE >= 1 << 31:
         _bad("rows of the cache must fit int32")
-    tokens = q.shape[0]
     if topk is not None:
         if cache.k_index is None:
             _bad("selection needs a cache with index vectors")
