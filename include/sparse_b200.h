@@ -423,7 +423,8 @@ int sparse_b200_indexer_summary_noalloc(const void* q, const void* k, float* sco
  * entries that are not pages of the request are skipped. out [total_q, Hq, 128] bf16, lse [total_q, Hq] fp32 or NULL; a row
  * that sees no key, or only keys of score -inf, is 0 with LSE -inf. What lies in the cache behind a request's last key, or is
  * hidden from a token, does not reach its row, whatever its bits. A query row with an infinite or NaN feature ends as NaN.
- * Sums are fp32: scale * q . k, and the keys of a row times the largest magnitude of a value, have to stay below 2^127.
+ * Sums are fp32: scale * |q| |k| has to stay below 2^120, the number of keys times the largest magnitude of a value below 2^127.
+ * A weight is within 2^-8 of itself or 2^-22 of the largest of its page, a query feature within 2^-21 of its row's largest.
  * Hq / Hkv <= 64. max_seqlen_q (a hint: the largest number of new tokens) sets how many tokens share a pass over a page.
  * workspace: sparse_b200_paged_attention_workspace_bytes bytes that are the call's own while it runs. */
 int sparse_b200_extend_pages(int32_t* block_table, int64_t table_stride, int table_width, const int32_t* seq_lens,

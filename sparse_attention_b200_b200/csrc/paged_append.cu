@@ -17,8 +17,9 @@
 // (run, head) of K or of V: the rows stay in registers between the maximum and the conversion, so they are read once, and
 // nobody else touches the page's rows or scale, so nothing is ordered between CTAs. Thread = 16 features of a row (the group
 // of an NVFP4 scale): 32 B in, 16 B out, eight threads write a row of 128 B. 64 requests of up to 8 tokens: 6.3 us; 8 prompts of
-// 512 to 4096 tokens, 4 heads, with the index (55 MB): 16.7 us, 3.3 TB/s, two waves of CTAs, issue slots 59 % taken while they
-// run. K (whose index is most of the arithmetic) before V: taken in turns they took 18.6 us; 512 threads 19.6.
+// 512 to 4096 tokens, 4 heads, with the index (55 MB): 16.7 us, 3.3 TB/s, two waves of CTAs, issue slots 58 % taken: a
+// CTA loads, meets, converts and stores in turn, and waits for each. K (whose index is most of the arithmetic) before V: taken
+// in turns they took 18.6 us; 512 threads 19.6.
 #include <cuda_bf16.h>
 #include "internal.h"
 #include "nvfp4_quantize.cuh"

@@ -30,9 +30,11 @@
 // What the loader tells of items and pages goes through a ring of its own, in batches of 32 pages.
 //
 // What bounds it: HBM where pages are read once by 16 rows of heads (64 requests of 8192 to 32768 keys, 4 KV heads of 16: 1.41 GB
-// in 220 us, 6.4 TB/s; with 64 listed pages each 0.54 GB in 98 us, 5.5 TB/s). The softmax, about 1400 cycles a page and CTA pair,
-// is just under that, and bounds items whose pages come from the L2 cache. One row of 1 Mi keys: 57 us, 7 of them the merge of
-// its parts. A call of 6 pages takes 12.5 us: latencies of two launches, of finding a share and of one page's chain.
+// in 221 us, 6.4 TB/s; with 64 listed pages each 0.54 GB in 98 us, 5.5 TB/s). The softmax, about 1400 cycles a page and CTA pair,
+// is just under that. Items whose pages come from the L2 cache are bound by the latency of a page's chain: 32 requests of 1 to 8
+// tokens, 66 us, keep no unit busy for more than half of the time (DRAM 50 %, issue slots 37 %, XU 10 %, tensor pipe 7 %). One row of 1 Mi
+// keys: 57 us, 7 of them the merge of its parts. A call of 6 pages takes 12.5 us: latencies of two launches, of finding a share
+// and of one page's chain.
 #include "paged_attention.cuh"
 
 namespace sb {

@@ -5,7 +5,7 @@
 //   S [128 rows, 128 keys] = Q K^T      O [128 rows, 128 features] += P V          (kind::f16, fp32 sums, one page a step)
 //
 // Mathematics. The codes of a page become f16, exactly, on their way into shared memory. A query row is scaled by a power of
-// two (largest feature in [128, 256)) and is exact in f16 but for features below 2^-22 of the largest, which lose up to 2^-33
+// two (largest feature in [128, 256)) and is exact in f16 but for features below 2^-24 of the largest, which lose up to 2^-32
 // of it. The page's key scale joins the row's factor of the softmax. Outputs are sums of exp2(x + log2 v_scale - o + 6) and the
 // codes, the weight in f16 (2^-11, floor 2^-31 of the row's largest): a page whose values are huge and whose weights are nothing
 // costs the others no bits. Sums are kept relative to m. m and o are maxima of a row, of x and of x + log2 v_scale (counted from

@@ -17,9 +17,11 @@
 // Many lists (select_many_kernel): 32 to a CTA, a lane's list is its lane number (a page's scores of 32 lists are one 128-byte
 // line), a warp holds up to 64 pages of all of them in registers; a count is two instructions a key, a sum over the warps
 // through shared memory and one barrier for 32 lists. Few lists (select_few_kernel): four to a CTA, so that a decode step uses
-// more SMs, 512 threads for the loads; a warp then searches a list by itself (a count costs a redux, no barrier). 34,000 lists
-// of 128 pages: 24 us with the first, 33 with the second; 270 lists of 256 pages and 16 index heads: 17 and 10 us. The first is
-// bound by instruction issue (about 3500 instructions of a warp for 64 pages of 32 lists), the second by latency.
+// more SMs, 512 threads for the loads; a warp then searches a list by itself (a count costs a redux, no barrier). 32,700 lists
+// of up to 107 pages: 23 us with the first, 33 with the second; 270 lists of 256 pages and 16 index heads: 17 and 10 us. Both
+// are bound by latency: the first takes 46 % of the issue slots (about 3500 instructions of a warp for its 64 places of 32
+// lists), its warps wait for their loads and, once a count, for one another; the second for the requests that its lists belong
+// to (about nine loads, one after another), one pass over the scores and a dozen counts.
 #include "internal.h"
 #include "paged.cuh"
 
