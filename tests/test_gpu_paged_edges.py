@@ -427,3 +427,29 @@ def test_sums_of_huge_values_stay_finite(sp, group, rise, v_scales):
             assert out.isfinite().all()
             assert ((out - want).abs() <= bound).all(), ((out - want).abs() / bound).max()
             assert ((lse - want_lse).abs() <= bound_lse).all()
+
+
+@pytest.mark.parametrize("total_pages", [0, 1, 5, 9])
+def test_a_step_whose_page_list_is_cut(sp, total_pages):
+    """The scorer stays within the list; requests whose pages are all in it get what they get with the whole list."""
+    old, lens = [300, 250, 600], [1, 20, 2]                            # 3, 3 and 5 pages
+    results = []
+    for pages in (11, total_pages):
+        q, k, v, cache, table, _ = _step(sp, lens, old, 2, 4)
+        table[1, 2] = -1                                               # (the helper's own step has extended it)
+        b = sp.extend_pages(table, _i32(old).cuda(), _i32(lens).cuda(), torch.arange(10, 13, dtype=torch.int32).cuda(),
+                            _i32([3]).cuda(), total_q=23, total_pages=pages)
+        if pages == 0:
+            with pytest.raises(sp.SparseB200Error):                    # nothing to select from
+                sp.paged_step(q, k, v, cache, table, b, topk=2, max_seqlen_q=20, max_seqlen_k=602)
+            assert int(b.status) == sp.paged.STATUS_PAGES
+            return
+        results.append((b, *sp.paged_step(q, k, v, cache, table, b, topk=2, sink=0, max_seqlen_q=20, max_seqlen_k=602), cache))
+    sp.device_status()
+    (whole, out, ids, cache), (cut, out_cut, ids_cut, cache_cut) = results
+    assert int(whole.status) == 0 and int(cut.status) == sp.paged.STATUS_PAGES and _same_bits(cache, cache_cut)
+    assert torch.equal(whole.kv_indices[:total_pages], cut.kv_indices) and torch.equal(whole.slots, cut.slots)
+    for r, end in enumerate((3, 6, 11)):
+        rows = slice(int(whole.cu_seqlens_q[r]), int(whole.cu_seqlens_q[r + 1]))
+        if end <= total_pages:
+            assert torch.equal(ids[:, rows], ids_cut[:, rows]) and torch.equal(out[rows], out_cut[rows])
