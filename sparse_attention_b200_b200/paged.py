@@ -159,8 +159,8 @@ def extend_pages(block_table, seq_lens, new_lens, free_pages, free_count, *, tot
     _dense("free_pages", free_pages, torch.int32, (free_pages.numel(),), dev)
     _dense("free_count", free_count, torch.int32, (1,), dev)
     table, stride, width = _table(block_table, batch, dev)
-    if total_q < 0 or total_pages < 0:
-        _bad("table sizes must not be negative")
+    if not 0 <= total_q < 1 << 31 or not 0 <= total_pages < 1 << 31:
+        _bad("table sizes must not be negative, and fit int32")
     with _on(dev):
         # one allocation, the 64-bit slots first
         buffer = torch.empty(2 * total_q + 4 * batch + 5 + total_pages, dtype=torch.int32, device=dev)

@@ -102,6 +102,13 @@ def test_pages_are_neither_lost_nor_made_over_many_steps(sp):
     assert short
 
 
+@pytest.mark.parametrize("sizes", [(2 ** 32 + 5, 3), (5, 2 ** 32 + 3), (2 ** 31, 3), (5, -2 ** 32)])
+def test_extend_pages_refuses_sizes_beyond_32_bits(sp, sizes):
+    one = _i32([1]).cuda()
+    with pytest.raises(sp.SparseB200Error):
+        sp.extend_pages(one[None].clone(), one, one, one, one, total_q=sizes[0], total_pages=sizes[1])
+
+
 # ------------------------------------------------------------------ append_tokens
 @pytest.mark.parametrize("old", [0.0, 2.0 ** -110, 2.0 ** -9, 0.013, 3.0])
 def test_rows_behind_those_of_a_page_with_any_scale(sp, old):
