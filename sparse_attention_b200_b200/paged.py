@@ -83,7 +83,7 @@ def _table(block_table, batch, device):
     """Its address, row stride and width."""
     shape, stride = block_table.shape, block_table.stride()
     if block_table.dtype is not torch.int32 or block_table.device != device or len(shape) != 2 or shape[0] != batch \
-            or shape[1] == 0 or stride[1] != 1 or batch > 1 and stride[0] < shape[1]:
+            or not 0 < shape[1] < 1 << 24 or stride[1] != 1 or batch > 1 and stride[0] < shape[1]:
         _bad("block_table must be int32 [B, pages per request] with dense rows on the same device")
     return block_table.data_ptr(), max(stride[0], shape[1]), shape[1]
 
@@ -299,15 +299,20 @@ def paged_step(q, k, v, cache, block_table, batch, *, topk=None, tile=1, max_seq
     whole sequences, without index vectors. Returns (out, ids); rows whose slot is -1 (a refused request's, and those behind the
     last token) have no meaning."""
     # what a later stage would refuse is refused before the cache has changed
-    tokens = _check_queries(q, cache)[0]
-    _table(block_table, batch.seq_lens.numel(), cache.device)
-    if scale is not None and not math.isfinite(scale):
+    tokens, dev, requests = _check_queries(q, cache)[0], cache.device, batch.seq_lens.numel()
+    _table(block_table, requests, dev)
+    _dense("seq_lens", batch.seq_lens, torch.int32, (requests,), dev)
+    _dense("cu_seqlens_q", batch.cu_seqlens_q, torch.int32, (requests + 1,), dev)
+    if scale is not None and not abs(scale) < 2.0 ** 128 - 2.0 ** 103:        # fp32, rounded
         _bad("scale must be finite")
     if cache.pages * cache.kv_heads * PAGE >= 1 << 31:
         _bad("rows of the cache must fit int32")
     if topk is not None:
         if cache.k_index is None:
             _bad("selection needs a cache with index vectors")
+        _dense("cu_seqlens_k", batch.cu_seqlens_k, torch.int32, (requests + 1,), dev)
+        _dense("cu_page_offsets", batch.cu_page_offsets, torch.int32, (requests + 1,), dev)
+        _dense("kv_indices", batch.kv_indices, torch.int32, (batch.kv_indices.numel(),), dev)
         if tokens and (max_seqlen_q < 1 or max_seqlen_k < 1 or batch.kv_indices.numel() == 0):
             _bad("lengths and the page list of a step with tokens must not be empty")
         _check_selection(max((max_seqlen_k + PAGE - 1) // PAGE, 1), cache.kv_heads, topk, tile, sink, recent)
@@ -320,7 +325,7 @@ def paged_step(q, k, v, cache, block_table, batch, *, topk=None, tile=1, max_seq
                                              batch.cu_seqlens_k, batch.cu_page_offsets, max_seqlen_q=max_seqlen_q,
                                              max_seqlen_k=max_seqlen_k, kv_indices=batch.kv_indices, causal=True, exact=False)
         else:
-            scores = torch.empty((cache.kv_heads, 1, 0), dtype=torch.float32, device=cache.device)
+            scores = torch.empty((cache.kv_heads, 1, 0), dtype=torch.float32, device=dev)
         ids = select_pages(scores, batch.cu_seqlens_q, batch.seq_lens, kv_heads=cache.kv_heads, topk=topk, tile=tile,
                            sink=sink, recent=recent)
     out = paged_attention(q, cache, block_table, batch.seq_lens, batch.cu_seqlens_q, ids, tile=tile,

@@ -283,7 +283,9 @@ def test_a_step_takes_views_of_a_fused_projection(sp, topk, tile):
     dict(topk=0), dict(topk=3, tile=3), dict(topk=3, tile=256), dict(topk=2, sink=2, recent=1), dict(topk=2, sink=-1),
     dict(topk=2, sink=2 ** 32), dict(topk=3, max_seqlen_q=0), dict(topk=3, max_seqlen_k=0), dict(topk=3, max_seqlen_k=51200 * PAGE),
     dict(scale=math.nan), dict(scale=-math.inf), dict(topk=3, q="heads"), dict(q="strides"), dict(q="group"), dict(table="rows"),
-    dict(topk=3, index=False), dict(topk=3, table="no pages"),
+    dict(topk=3, index=False), dict(topk=3, table="no pages"), dict(scale=1e39), dict(scale=2.0 ** 128), dict(table="wide"),
+    dict(table="seq_lens"), dict(topk=3, table="cu_seqlens_k"), dict(topk=3, table="cu_page_offsets"),
+    dict(topk=3, table="kv_indices"),
 ])
 def test_a_refused_step_leaves_the_cache_as_it_was(sp, bad):
     bad = dict(bad)
@@ -294,6 +296,12 @@ def test_a_refused_step_leaves_the_cache_as_it_was(sp, bad):
         table = table[:1]
     elif change == "no pages":
         b = b._replace(kv_indices=b.kv_indices[:0])
+    elif change == "wide":
+        table = torch.zeros((2, 1 << 24), dtype=torch.int32, device="cuda")
+    elif change == "kv_indices":
+        b = b._replace(kv_indices=b.kv_indices.long())
+    elif change:
+        b = b._replace(**{change: getattr(b, change)[:1]})
     before = _copy(sp, cache)
     with pytest.raises(sp.SparseB200Error):
         sp.paged_step(q, k, v, cache, table, b, **{**dict(max_seqlen_q=2, max_seqlen_k=302), **bad})
